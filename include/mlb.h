@@ -203,6 +203,156 @@ int mlb_attention_decode_noalloc(int device, const float* q, const float* key_ca
                                  int layer, int pos, int n_heads, int n_kv_heads, int head_dim,
                                  float* out);
 
+/* ------------------------------------------------------------ rotary positions of rows
+ * RoPE for many rows at once, each at its own position, on the first rot_dim
+ * elements of every head (the rest passes through).  The angles live in a
+ * table the caller owns and fills once: cos_sin [n_positions][rot_dim / 2]
+ * (cos, sin) pairs of floats on the device, 16-byte aligned.  rope_type pairs
+ * elements as mlb_rope does, within the rotated part: MLB_ROPE_NORMAL
+ * (2i, 2i + 1), MLB_ROPE_NEOX (i, i + rot_dim / 2).  Without scaling and with
+ * rot_dim == head_dim the results are those of mlb_rope, bit for bit.  No
+ * reference counterpart (the reference rotates whole heads of one row,
+ * unscaled). */
+typedef struct {
+    int n_positions;
+    int head_dim;
+    int rot_dim;   /* even, 2..head_dim */
+    int rope_type; /* mlb_rope_type */
+    float* cos_sin;
+} mlb_rope_table;
+
+/* How a model's positions are stretched past the length it was trained on
+ * (`factor` >= 1 times; original_positions is that length).
+ *   LINEAR      every frequency / factor
+ *   NTK         theta * factor^(rot_dim / (rot_dim - 2))
+ *   YARN        frequencies that turn more than `fast` times within
+ *               original_positions stay, those below `slow` turns are divided
+ *               by factor, a linear ramp over the pair index between (32 and 1
+ *               when both are 0); cos and sin are multiplied by
+ *               attention_factor (0: 0.1 ln(factor) + 1)
+ *   WAVELENGTH  frequencies with more than `fast` turns within
+ *               original_positions stay, below `slow` turns are divided by
+ *               factor, a linear blend in the number of turns between (4 and 1
+ *               when both are 0) */
+typedef enum {
+    MLB_ROPE_SCALE_NONE = 0,
+    MLB_ROPE_SCALE_LINEAR = 1,
+    MLB_ROPE_SCALE_NTK = 2,
+    MLB_ROPE_SCALE_YARN = 3,
+    MLB_ROPE_SCALE_WAVELENGTH = 4
+} mlb_rope_scaling;
+
+typedef struct {
+    int scaling; /* mlb_rope_scaling */
+    float factor;
+    int original_positions; /* YARN and WAVELENGTH */
+    float fast;
+    float slow;
+    float attention_factor; /* YARN */
+} mlb_rope_scale;
+
+/* Fills the table for positions 0 .. n_positions - 1: angle = pos * freq in
+ * fp32 with the reference's formula (freq_i = 1 / powf(theta, 2i / rot_dim),
+ * src/context.cpp:16-25), freq scaled as above.  scale NULL: none.  Computed on
+ * the host; returns when the table is on the device. */
+int mlb_rope_table_fill(int device, const mlb_rope_table* table, float theta,
+                        const mlb_rope_scale* scale);
+/* Rotates q [rows][n_heads][head_dim] and k [rows][n_kv_heads][head_dim] (rows
+ * q_stride / k_stride floats apart, so both may sit in a fused projection's
+ * rows) at positions[rows] (device ints) into q_out / k_out.  An output equal
+ * to its input, with the same stride, works in place; other overlaps are not
+ * allowed.  q or k may be absent (n_heads or n_kv_heads 0).  A row whose
+ * position is outside the table becomes NaN. */
+int mlb_rope_rows(int device, const mlb_rope_table* table, int rows, const int* positions,
+                  const float* q, size_t q_stride, float* q_out, size_t q_out_stride, int n_heads,
+                  const float* k, size_t k_stride, float* k_out, size_t k_out_stride,
+                  int n_kv_heads);
+
+/* ------------------------------------------------------------ quantized KV cache
+ * A KV cache of n_seqs sequences in the caller's memory.
+ *   MLB_F32   k, v [n_seqs][n_layers][max_seq_len][n_kv_heads][head_dim] floats,
+ *             the layout of mlb_attention_decode_batched (k_scale, v_scale NULL)
+ *   MLB_Q8_0, MLB_Q4_0   the blocks of the quantized weights (32 elements, one
+ *             fp16 scale, a head padded with zeros to B = ceil(head_dim / 32)
+ *             blocks), quants and scales in planes of their own so that one
+ *             head's positions are contiguous: with S = max_seq_len rounded up
+ *             to 8, k, v [n_seqs][n_layers][n_kv_heads][S][B * 32] int8 or
+ *             [..][S][B * 16] nibble pairs (byte i of a block: element i low,
+ *             16 + i high, value d * (n - 8)) and k_scale, v_scale
+ *             [n_seqs][n_layers][n_kv_heads][S][B] fp16
+ * k, v, k_scale and v_scale are 16-byte aligned (MLB_F32: 4-byte).  A slot is a
+ * position within a sequence's max_seq_len.  No reference counterpart: the
+ * reference's cache is fp32 and holds one sequence. */
+typedef struct {
+    int type; /* mlb_qtype: MLB_F32, MLB_Q8_0 or MLB_Q4_0 */
+    int n_seqs;
+    int n_layers;
+    int max_seq_len;
+    int n_kv_heads;
+    int head_dim;
+    void* k;
+    void* v;
+    void* k_scale;
+    void* v_scale;
+} mlb_kv_cache;
+
+#define MLB_ALL_LAYERS (-1)
+
+/* Bytes of k (and of v) and of k_scale (and of v_scale, 0 for MLB_F32); the
+ * pointers of the descriptor are not looked at. */
+int mlb_kv_cache_bytes(const mlb_kv_cache* cache, size_t* plane_bytes, size_t* scale_bytes);
+/* Writes rows of k and v ([rows][n_kv_heads][head_dim], rows k_stride /
+ * v_stride floats apart) to slots[rows] of sequences seqs[rows] (device ints;
+ * seqs NULL: sequence 0), quantized by the rule of mlb_quantize with the scale
+ * as fp16(amax * fl(1/127)) (Q4_0: fl(1/7)), a product where mlb_quantize
+ * divides; the two differ in the last bit of about one Q4_0 scale in 40 000.
+ * MLB_F32: copied.  A row whose sequence or slot is outside the cache is skipped, so -1
+ * marks padding; the other rows must name different (sequence, slot) pairs.
+ * layer MLB_ALL_LAYERS: k and v hold `rows` rows for each layer, layer after
+ * layer, and every layer takes its own at the same slots. */
+int mlb_kv_cache_write(int device, const mlb_kv_cache* cache, int layer, int rows, const int* seqs,
+                       const int* slots, const float* k, size_t k_stride, const float* v,
+                       size_t v_stride);
+/* mlb_rope_rows and mlb_kv_cache_write in one launch: q is rotated into q_out
+ * (equal to q with the same stride: in place), k on its way into the cache.
+ * One layer at a time; n_heads 0: k and v only.  A row whose position is
+ * outside the table is not written to the cache, and its q_out is NaN. */
+int mlb_kv_cache_write_rope(int device, const mlb_kv_cache* cache, int layer, int rows,
+                            const int* seqs, const int* slots, const mlb_rope_table* table,
+                            const int* positions, const float* q, size_t q_stride, float* q_out,
+                            size_t q_out_stride, int n_heads, const float* k, size_t k_stride,
+                            const float* v, size_t v_stride);
+/* The cached rows as floats, arguments as mlb_kv_cache_write.  k or v may be
+ * NULL.  A row outside the cache reads as zeros. */
+int mlb_kv_cache_read(int device, const mlb_kv_cache* cache, int layer, int rows, const int* seqs,
+                      const int* slots, float* k, size_t k_stride, float* v, size_t v_stride);
+
+/* ------------------------------------------------------------ attention for drafted tokens
+ * One call attends with `tokens` query tokens of each of `batch` sequences over
+ * the cache: tokens = 1 is the decode step, more are a drafted chain or tree
+ * (or a piece of a prompt).  The tokens' own K and V are already in the cache,
+ * token j of sequence b at slot lens[b] + j.
+ *   out[b][t][h] = sum_s w_s V[s],  w = softmax over the slots s that (b, t)
+ *                  sees of scale * q[b][t][h] . K[s]
+ * (b, t) sees every slot below lens[b], and slot lens[b] + j when bit j % 64 of
+ * mask[b][t][j / 64] is set (mask [batch][tokens][ceil(tokens / 64)], device;
+ * NULL: j <= t).  A slot that is not seen has no effect, whatever it holds; a
+ * row that sees none is zeros.  Query head h reads KV head
+ * h / (n_heads / n_kv_heads).  q and out: row b * tokens + t,
+ * [n_heads][head_dim], rows q_stride / out_stride floats apart.  seqs[batch]
+ * (device; NULL: b) is the cache sequence of each batch entry, lens[batch]
+ * (device) its length: lens[b] < 0, or a sequence outside the cache, marks an
+ * inactive entry (zeros).  max_len is an upper bound of lens that the caller
+ * knows (larger lens are taken as max_len); slots from max_seq_len on do not
+ * exist.  scale 0: 1 / sqrt(head_dim).  head_dim up to 256.  out does not
+ * overlap q.
+ * Extends include/cuda_attention.h:10-14, which has one token of one sequence
+ * over an fp32 cache. */
+int mlb_attention_tree(int device, const mlb_kv_cache* cache, int layer, int batch, int tokens,
+                       const int* seqs, const int* lens, int max_len, const uint64_t* mask,
+                       const float* q, size_t q_stride, int n_heads, float scale, float* out,
+                       size_t out_stride);
+
 /* ------------------------------------------------------------ synthetic inputs
  * Seeded N(0, sigma) fill on the device, bit-identical to the host generator
  * used for fixtures (splitmix64 counter stream, Irwin-Hall sum of 12 uniform

@@ -21,6 +21,9 @@ MLB_ERR_DEVICE_TIMEOUT = 5
 
 F32, Q8_0, Q4_0, Q4_1 = 0, 1, 2, 3
 ROPE_NORMAL, ROPE_NEOX = 0, 1
+(ROPE_SCALE_NONE, ROPE_SCALE_LINEAR, ROPE_SCALE_NTK, ROPE_SCALE_YARN,
+ ROPE_SCALE_WAVELENGTH) = range(5)
+ALL_LAYERS = -1
 
 W_EMBEDDING, W_FINAL_NORM, W_LM_HEAD, W_ATTN_NORM = 0, 1, 2, 3
 W_WQ, W_WK, W_WV, W_BQ, W_BK, W_BV, W_WO = 4, 5, 6, 7, 8, 9, 10
@@ -47,6 +50,27 @@ class ModelConfig(ctypes.Structure):
         "max_seq_len")] + [("rope_theta", ctypes.c_float), ("rms_norm_eps", ctypes.c_float)] + [
         (n, ctypes.c_int) for n in ("rope_type", "weight_type", "qkv_bias")]
 
+
+class RopeTable(ctypes.Structure):
+    _fields_ = [("n_positions", ctypes.c_int), ("head_dim", ctypes.c_int),
+                ("rot_dim", ctypes.c_int), ("rope_type", ctypes.c_int),
+                ("cos_sin", ctypes.c_void_p)]
+
+
+class RopeScale(ctypes.Structure):
+    _fields_ = [("scaling", ctypes.c_int), ("factor", ctypes.c_float),
+                ("original_positions", ctypes.c_int), ("fast", ctypes.c_float),
+                ("slow", ctypes.c_float), ("attention_factor", ctypes.c_float)]
+
+
+class KvCache(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int) for n in (
+        "type", "n_seqs", "n_layers", "max_seq_len", "n_kv_heads", "head_dim")] + [
+        (n, ctypes.c_void_p) for n in ("k", "v", "k_scale", "v_scale")]
+
+
+_prope = ctypes.POINTER(RopeTable)
+_pkv = ctypes.POINTER(KvCache)
 
 SIGNATURES = {
     "mlb_last_error": (ctypes.c_char_p, []),
@@ -86,6 +110,15 @@ SIGNATURES = {
     "mlb_attention_decode_batched": (_i, [_i, _i, _vp, _vp, _vp, _i, _i, _i, _vp, _i, _i, _i,
                                           _i, _vp]),
     "mlb_attention_decode_noalloc": (_i, [_i, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _vp]),
+    "mlb_rope_table_fill": (_i, [_i, _prope, _f, ctypes.POINTER(RopeScale)]),
+    "mlb_rope_rows": (_i, [_i, _prope, _i, _vp, _vp, _sz, _vp, _sz, _i, _vp, _sz, _vp, _sz, _i]),
+    "mlb_kv_cache_bytes": (_i, [_pkv, _psz, _psz]),
+    "mlb_kv_cache_write": (_i, [_i, _pkv, _i, _i, _vp, _vp, _vp, _sz, _vp, _sz]),
+    "mlb_kv_cache_write_rope": (_i, [_i, _pkv, _i, _i, _vp, _vp, _prope, _vp, _vp, _sz, _vp, _sz,
+                                     _i, _vp, _sz, _vp, _sz]),
+    "mlb_kv_cache_read": (_i, [_i, _pkv, _i, _i, _vp, _vp, _vp, _sz, _vp, _sz]),
+    "mlb_attention_tree": (_i, [_i, _pkv, _i, _i, _i, _vp, _vp, _i, _vp, _vp, _sz, _i, _f, _vp,
+                                _sz]),
     "mlb_synth_normal": (_i, [_i, _vp, _sz, _u64, _u64, _d]),
     "mlb_model_create": (_i, [_i, ctypes.POINTER(ModelConfig), _pp]),
     "mlb_model_destroy": (_i, [_vp]),

@@ -76,6 +76,9 @@ struct DeviceContext {
     const void* tc_x = nullptr;
     const void* tc_ws = nullptr;
     int tc_m = 0, tc_k = 0, tc_mx = 0, tc_mtiles = 0;
+    // arrival counters of the drafted-token attention, zero between launches
+    int* tree_counters = nullptr;
+    size_t tree_counter_count = 0;
 };
 
 DeviceContext& Ctx(int device);                     // creates on first use, makes device current
@@ -132,6 +135,46 @@ __device__ __forceinline__ float WarpMax(float v) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
     return v;
+}
+
+// fp16 conversion with the reference's rounding (round half up on bit 12,
+// src/quant.cpp:17-52), not the IEEE ties-to-even of __float2half.
+__device__ __forceinline__ uint16_t F32ToF16Ref(float value) {
+    uint32_t bits = __float_as_uint(value);
+    uint32_t sign = (bits >> 16) & 0x8000u;
+    int exponent = static_cast<int>((bits >> 23) & 0xffu) - 127 + 15;
+    uint32_t mantissa = bits & 0x7fffffu;
+    if (exponent <= 0) {
+        if (exponent < -10) return static_cast<uint16_t>(sign);
+        mantissa |= 0x800000u;
+        uint32_t shifted = mantissa >> (1 - exponent);
+        if (shifted & 0x1000u) shifted += 0x2000u;
+        return static_cast<uint16_t>(sign | (shifted >> 13));
+    }
+    if (exponent >= 31) return static_cast<uint16_t>(sign | 0x7c00u);
+    if (mantissa & 0x1000u) {
+        mantissa += 0x2000u;
+        if (mantissa & 0x800000u) {
+            mantissa = 0;
+            if (++exponent >= 31) return static_cast<uint16_t>(sign | 0x7c00u);
+        }
+    }
+    return static_cast<uint16_t>(sign | (static_cast<uint32_t>(exponent) << 10) | (mantissa >> 13));
+}
+
+// 2^e as a float for -126 <= e <= 127, from its exponent bits.
+__device__ __forceinline__ float Pow2(int e) { return __uint_as_float(static_cast<uint32_t>(127 + e) << 23); }
+
+// Exponent s with (bound * 2^s) in [2^14, 2^15) (0 when bound is 0 or not finite).
+__device__ __forceinline__ int ScaleExp(float bound) {
+    if (!(bound > 0.0f) || !isfinite(bound)) return 0;
+    const int e = static_cast<int>((__float_as_uint(bound) >> 23) & 0xff) - 127;  // 2^e <= bound < 2^(e+1)
+    int s = 14 - e;
+    return s > 100 ? 100 : (s < -100 ? -100 : s);
+}
+
+__device__ __forceinline__ uint32_t PackHalf2(__half a, __half b) {
+    return static_cast<uint32_t>(__half_as_ushort(a)) | (static_cast<uint32_t>(__half_as_ushort(b)) << 16);
 }
 
 // mbarrier + bulk-copy (TMA, non-tensor, no multicast) wrappers.

@@ -151,31 +151,6 @@ __global__ void KvWriteKernel(float* kc, float* vc, size_t slot, const float* k,
 }
 
 // ---------------------------------------------------------------- quantizer
-// fp16 conversion with the reference's rounding (round half up on bit 12,
-// src/quant.cpp:17-52), not the IEEE ties-to-even of __float2half.
-__device__ uint16_t F32ToF16Ref(float value) {
-    uint32_t bits = __float_as_uint(value);
-    uint32_t sign = (bits >> 16) & 0x8000u;
-    int exponent = static_cast<int>((bits >> 23) & 0xffu) - 127 + 15;
-    uint32_t mantissa = bits & 0x7fffffu;
-    if (exponent <= 0) {
-        if (exponent < -10) return static_cast<uint16_t>(sign);
-        mantissa |= 0x800000u;
-        uint32_t shifted = mantissa >> (1 - exponent);
-        if (shifted & 0x1000u) shifted += 0x2000u;
-        return static_cast<uint16_t>(sign | (shifted >> 13));
-    }
-    if (exponent >= 31) return static_cast<uint16_t>(sign | 0x7c00u);
-    if (mantissa & 0x1000u) {
-        mantissa += 0x2000u;
-        if (mantissa & 0x800000u) {
-            mantissa = 0;
-            if (++exponent >= 31) return static_cast<uint16_t>(sign | 0x7c00u);
-        }
-    }
-    return static_cast<uint16_t>(sign | (static_cast<uint32_t>(exponent) << 10) | (mantissa >> 13));
-}
-
 // One thread per 32-element block; every fp32 operation is an explicitly
 // rounded intrinsic so no FMA contraction changes the reference's rounding.
 __global__ void QuantizeKernel(int qtype, const float* x, int rows, int cols, uint8_t* out) {

@@ -84,21 +84,6 @@ constexpr int kTcDqThreads = kTcDqWarps * 32;
 constexpr int kTcThreads = kTcDqThreads + 64;       // + x-copy warp + MMA warp
 constexpr uint64_t kTcWaitNs = 2000000000ull;
 
-// 2^e as a float for -126 <= e <= 127, from its exponent bits.
-__device__ __forceinline__ float Pow2(int e) { return __uint_as_float(static_cast<uint32_t>(127 + e) << 23); }
-
-// Exponent s with (bound * 2^s) in [2^14, 2^15) (0 when bound is 0 or not finite).
-__device__ __forceinline__ int ScaleExp(float bound) {
-    if (!(bound > 0.0f) || !isfinite(bound)) return 0;
-    const int e = static_cast<int>((__float_as_uint(bound) >> 23) & 0xff) - 127;  // 2^e <= bound < 2^(e+1)
-    int s = 14 - e;
-    return s > 100 ? 100 : (s < -100 ? -100 : s);
-}
-
-__device__ __forceinline__ uint32_t PackHalf2(__half a, __half b) {
-    return static_cast<uint32_t>(__half_as_ushort(a)) | (static_cast<uint32_t>(__half_as_ushort(b)) << 16);
-}
-
 // ---------------------------------------------------------------- x pre-pass
 // One CTA per x row of the padded tiles (mtiles * MX rows): its scale
 // exponent (largest |x| into [2^14, 2^15)), the undo factor 2^-s, and its
