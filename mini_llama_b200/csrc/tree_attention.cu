@@ -128,6 +128,7 @@ int mlb_attention_tree(int device, const mlb_kv_cache* cache, int layer, int bat
         a.out_vec = a.c.hd % 4 == 0 && vec(out, out_stride);
         a.cache_vec = a.c.hd % 4 == 0 && vec(a.c.k, 0) && vec(a.c.v, 0);
         DeviceContext& ctx = Ctx(device);
+        if (LaunchTreeMma(ctx, a)) return;
         const unsigned grid = static_cast<unsigned>(batch) * tokens * n_heads;
         if (a.c.type == MLB_F32)
             TreeRowKernel<MLB_F32><<<grid, kRowWarps * 32, 0, ctx.stream>>>(a);

@@ -47,4 +47,7 @@ __device__ __forceinline__ bool SeesDraft(const uint64_t* bits, int t, int j) {
 }
 
 
+// The matrix-instruction kernel (tree_mma.cu); false: the shape is not one of its.
+bool LaunchTreeMma(DeviceContext& ctx, const TreeArgs& a);
+
 }  // namespace mlb
