@@ -464,6 +464,7 @@ KvView CheckedKvView(const char* c, const mlb_kv_cache* cache, bool pointers) {
     const bool f32 = v.type == MLB_F32;
     const int slots = f32 ? v.max_seq : (v.max_seq + 7) / 8 * 8;
     v.head_rows = f32 ? 1 : slots;
+    v.head_slots = slots;
     v.slot_rows = f32 ? v.n_kv : 1;
     v.layer_rows = 1LL * v.n_kv * slots;
     v.seq_rows = v.layer_rows * v.n_layers;

@@ -13,6 +13,7 @@ struct KvView {
     int type, n_seqs, n_layers, max_seq, n_kv, hd, blocks;
     long long seq_rows, layer_rows;  // row strides of a sequence and of a layer
     int head_rows, slot_rows;        // row strides of a head and of a slot
+    int head_slots;                  // slots that a head's plane holds
     void *k, *v;
     __half *ks, *vs;
 

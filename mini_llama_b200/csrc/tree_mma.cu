@@ -11,7 +11,7 @@
 //          products are exact up to the fp32 sum; the slot's scale of the block
 //          multiplies that sum.
 //   softmax  running maximum and sum per row, the maximum moved only when a
-//          score passes it by 2^8 (a vote): weights are 2^(x - m + 6) <= 2^14,
+//          score passes it by 2^2 (a vote): weights are 2^(x - m + 12) <= 2^14,
 //          split into fp16 hi + lo and turned into B fragments by movmatrix.
 //   V      O^T = V^T P^T: quants as exact fp16 A fragments again (byte
 //          transposition in registers); the slot's scale of a block goes into
@@ -19,7 +19,10 @@
 //          pairs, relative to a power of two per row that covers the largest d
 //          seen.  Two MMAs per fragment.
 // fp32 caches take the same path with mma.m16n8k8 on tf32 hi + lo pairs (three
-// products; no ranges to mind).
+// products; no ranges to mind).  A unit's weighted values are summed in fresh
+// accumulators and added to the running ones in fp32 with rounding to nearest:
+// the matrix unit's own additions truncate, which over a long context would
+// cost several times the fp32 rounding.
 //
 // The units of 16 slots of all (sequence, KV head, row group) items are one
 // list, cut evenly over the CTAs (the lengths are on the device, so every CTA
@@ -39,9 +42,10 @@ namespace {
 constexpr int kUnit = 16;          // slots of a matrix step
 constexpr int kRows = 8;           // query rows of a tile
 constexpr float kStart = -1.7e38f; // running maximum before the first score (finite: no inf - inf)
-constexpr float kLag = 8.0f;       // how far scores may pass the running maximum, in powers of two
-constexpr float kOffset = 6.0f;    // weights are relative to 2^6
-constexpr int kAhead = 3;          // steps of a warp that the L2 prefetch runs ahead
+constexpr float kLag = 2.0f;       // how far scores may pass the running maximum, in powers of two
+constexpr float kOffset = 12.0f;   // weights are relative to 2^12: at most 2^14, and the fp16 pairs resolve
+                                   // 2^-37 of the largest, for slots that weigh little where the heavy ones hold zeros
+constexpr int kAhead = 3;          // rounds that the L2 prefetch runs ahead
 constexpr float kLog2e = 1.4426950408889634f;
 
 struct TreeSplit {
@@ -50,6 +54,7 @@ struct TreeSplit {
     int rows;      // R
     float* parts;  // two partial results per CTA
     int* counters; // per item
+    uint32_t magic;
 };
 
 __device__ __forceinline__ void Mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -66,6 +71,28 @@ __device__ __forceinline__ void MmaTf32(float (&d)[4], const uint32_t (&a)[4], u
         "{%0, %1, %2, %3};"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// The same with a zero accumulator.
+__device__ __forceinline__ void MmaFirst(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+        "{%10, %10, %10, %10};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
+}
+
+__device__ __forceinline__ void MmaTf32First(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+        "{%10, %10, %10, %10};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
+}
+
+__device__ __forceinline__ void AddTo(float (&o)[4], const float (&d)[4]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o[i] += d[i];
 }
 
 __device__ __forceinline__ uint32_t Transpose8x8(uint32_t v) {
@@ -91,51 +118,55 @@ __device__ __forceinline__ void SplitHalf(float x, float y, uint32_t& hi, uint32
     lo = H2(__floats2half2_rn(x - f.x, y - f.y));
 }
 
-// x as tf32 (rounded to nearest) and the rest.
+// x as tf32 (rounded to nearest, halves up) and the rest, whose low 13 bits the
+// matrix unit does not read: together 2^-21 relative at worst.
 __device__ __forceinline__ void SplitTf32(float x, uint32_t& hi, uint32_t& lo) {
-    asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(hi) : "f"(x));
-    asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(lo) : "f"(x - __uint_as_float(hi)));
+    hi = (__float_as_uint(x) + 0x1000u) & 0xffffe000u;
+    lo = __float_as_uint(x - __uint_as_float(hi));
 }
 
-// Four int8 (biased by 128: each byte q + 128) as two half pairs (bytes 0 1, 2 3):
-// 0x6400 + u is the half 1024 + u.
-__device__ __forceinline__ void BytesToHalf(uint32_t biased, uint32_t& p01, uint32_t& p23) {
-    const __half2 off = AsHalf2(0x64806480u);  // 1024 + 128
-    p01 = H2(__hsub2(AsHalf2(__byte_perm(biased, 0x64u, 0x4140)), off));
-    p23 = H2(__hsub2(AsHalf2(__byte_perm(biased, 0x64u, 0x4342)), off));
+// int8 in bytes 0 and 2 of w as a half pair: byte ^ 0x80 is q + 128, and the half
+// 0x6400 + u is 1024 + u.  `magic` (kMagic8, kMagic4) comes from the kernel's
+// parameters: as a literal it would not fit the one logic instruction beside the
+// mask.
+constexpr uint32_t kMagic8 = 0x64806480u, kMagic4 = 0x64006400u;
+__device__ __forceinline__ uint32_t EvenBytes(uint32_t w, uint32_t magic) {
+    return H2(__hsub2(AsHalf2((w & 0x00ff00ffu) ^ magic), AsHalf2(kMagic8)));  // - (1024 + 128)
 }
 
 // The nibbles of bytes 0 and 2: low ones n - 8, high ones n - 8.
-__device__ __forceinline__ uint32_t LowNibbles(uint32_t w) {
-    return H2(__hsub2(AsHalf2((w & 0x000F000Fu) | 0x64006400u), AsHalf2(0x64086408u)));  // 1024 + n - 1032
+__device__ __forceinline__ uint32_t LowNibbles(uint32_t w, uint32_t magic) {
+    return H2(__hsub2(AsHalf2((w & 0x000F000Fu) | magic), AsHalf2(0x64086408u)));  // 1024 + n - 1032
 }
-__device__ __forceinline__ uint32_t HighNibbles(uint32_t w) {
+__device__ __forceinline__ uint32_t HighNibbles(uint32_t w, uint32_t magic) {
     // (1024 + 16 n) / 16 - 72
-    return H2(__hfma2(AsHalf2((w & 0x00F000F0u) | 0x64006400u), AsHalf2(0x2C002C00u), AsHalf2(0xD480D480u)));
+    return H2(__hfma2(AsHalf2((w & 0x00F000F0u) | magic), AsHalf2(0x2C002C00u), AsHalf2(0xD480D480u)));
 }
 
+// The fp16 scales of one slot's blocks, two to a word.
 template <int NB>
-__device__ __forceinline__ void LoadScales(const __half* p, uint16_t (&d)[NB]) {
+__device__ __forceinline__ void LoadScales(const __half* p, uint32_t (&d)[(NB + 1) / 2]) {
     if constexpr (NB % 4 == 0) {
 #pragma unroll
         for (int i = 0; i < NB / 4; ++i) {
             const uint2 w = __ldg(reinterpret_cast<const uint2*>(p) + i);
-            d[4 * i] = w.x & 0xffff;
-            d[4 * i + 1] = w.x >> 16;
-            d[4 * i + 2] = w.y & 0xffff;
-            d[4 * i + 3] = w.y >> 16;
+            d[2 * i] = w.x;
+            d[2 * i + 1] = w.y;
         }
     } else if constexpr (NB % 2 == 0) {
 #pragma unroll
-        for (int i = 0; i < NB / 2; ++i) {
-            const uint32_t w = __ldg(reinterpret_cast<const uint32_t*>(p) + i);
-            d[2 * i] = w & 0xffff;
-            d[2 * i + 1] = w >> 16;
-        }
+        for (int i = 0; i < NB / 2; ++i) d[i] = __ldg(reinterpret_cast<const uint32_t*>(p) + i);
     } else {
+        const unsigned short* h = reinterpret_cast<const unsigned short*>(p);
 #pragma unroll
-        for (int i = 0; i < NB; ++i) d[i] = __ldg(reinterpret_cast<const unsigned short*>(p) + i);
+        for (int i = 0; i < NB / 2; ++i) d[i] = __ldg(h + 2 * i) | (uint32_t(__ldg(h + 2 * i + 1)) << 16);
+        d[NB / 2] = __ldg(h + NB - 1);
     }
+}
+
+template <int N>
+__device__ __forceinline__ float ScaleOf(const uint32_t (&d)[N], int b) {
+    return b & 1 ? __high2float(AsHalf2(d[b >> 1])) : __low2float(AsHalf2(d[b >> 1]));
 }
 
 // The rows, lengths and mask that a warp's step needs, common to both forms.
@@ -153,17 +184,17 @@ __device__ __forceinline__ bool Sees(const Step& s, int t, int slot) {
 }
 
 // Scores S (C fragment: rows slot g, g + 8; columns query 2c, 2c + 1) to weights
-// 2^(x - m + offset), with the running maxima m and sums l of the two columns;
+// 2^(x - m + offset), slots from `low` on, with the running maxima m and sums l of the two columns;
 // `rescale` gets the factors of a moved maximum.
 template <typename Rescale>
-__device__ __forceinline__ void Weights(const Step& s, int p0, float (&x)[4], float cs0, float cs1, float offset,
+__device__ __forceinline__ void Weights(const Step& s, int p0, int low, float (&x)[4], float cs0, float cs1, float offset,
                                         float (&m)[2], float (&l)[2], Rescale&& rescale) {
-    if (p0 + kUnit > s.len) {  // drafted slots, or the end
+    if (low + kUnit > s.len) {  // drafted slots, or the end
         const int a = p0 + s.g, b = a + 8;
-        if (!Sees(s, s.t0, a)) x[0] = -INFINITY;
-        if (!Sees(s, s.t1, a)) x[1] = -INFINITY;
-        if (!Sees(s, s.t0, b)) x[2] = -INFINITY;
-        if (!Sees(s, s.t1, b)) x[3] = -INFINITY;
+        if (a < low || !Sees(s, s.t0, a)) x[0] = -INFINITY;
+        if (a < low || !Sees(s, s.t1, a)) x[1] = -INFINITY;
+        if (b < low || !Sees(s, s.t0, b)) x[2] = -INFINITY;
+        if (b < low || !Sees(s, s.t1, b)) x[3] = -INFINITY;
     }
     float top0 = fmaxf(x[0], x[2]) * cs0, top1 = fmaxf(x[1], x[3]) * cs1;
     if (__any_sync(0xffffffffu, top0 > m[0] + kLag || top1 > m[1] + kLag)) {
@@ -196,15 +227,18 @@ struct QuantWarp {
     static constexpr int kQuantBytes = TYPE == MLB_Q8_0 ? 32 : 16;
     static constexpr int kKWords = TYPE == MLB_Q8_0 ? 2 : 1;
 
-    uint32_t qh[NB][2][2], ql[NB][2][2];
     float o[NB][2][4];
     float m[2], l[2], cs[2];
     int e;         // of row g: P' is relative to 2^e
+    float bound;   // 2^e
+    __half2 down;  // 2^-e
     uint32_t kw[2][NB][kKWords];
-    uint16_t kd[2][NB];
+    uint32_t kd[2][(NB + 1) / 2];
     const uint8_t *k, *v;
     const __half *ks, *vs;
     int stored;
+    uint32_t magic;
+    const uint4* qs;  // Q fragments of the tile: [block][half][lane] (hi, hi, lo, lo)
 
     // First of the four output elements of row tile j (0, 1) of a block that
     // the thread holds in o[.][j][0..1] (its row g) and o[.][j][2..3] (g + 8).
@@ -212,13 +246,8 @@ struct QuantWarp {
         return TYPE == MLB_Q8_0 ? 4 * g + 2 * j + half : 16 * j + 2 * g + half;
     }
 
-    __device__ __forceinline__ void Begin(const TreeArgs& a, const Step& s, int seq, int head, const float* q) {
-        const long long row = a.c.Row(seq, a.layer, head, 0);
-        k = static_cast<const uint8_t*>(a.c.k) + row * NB * kQuantBytes;
-        v = static_cast<const uint8_t*>(a.c.v) + row * NB * kQuantBytes;
-        ks = a.c.ks + row * NB;
-        vs = a.c.vs + row * NB;
-        stored = a.c.head_rows;
+    __device__ __forceinline__ static void LayOut(const TreeArgs& a, const Step& s, const float* q, uint4* frags,
+                                                  float* undos) {
         // the thread's elements of its row g, in the order of the K fragments
         float x[NB][8], top = 0.0f;
 #pragma unroll
@@ -252,25 +281,46 @@ struct QuantWarp {
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
                 const float* y = &x[b][4 * i];
-                // Q8_0: elements in order; Q4_0: bytes 0 and 2, then 1 and 3 of a word
-                const int y1 = TYPE == MLB_Q8_0 ? 1 : 2, y2 = TYPE == MLB_Q8_0 ? 2 : 1;
-                SplitHalf(y[0] * sc, y[y1] * sc, qh[b][i][0], ql[b][i][0]);
-                SplitHalf(y[y2] * sc, y[3] * sc, qh[b][i][1], ql[b][i][1]);
+                // bytes 0 and 2, then 1 and 3 of a word
+                uint4 f;
+                SplitHalf(y[0] * sc, y[2] * sc, f.x, f.z);
+                SplitHalf(y[1] * sc, y[3] * sc, f.y, f.w);
+                frags[(2 * b + i) * 32 + s.lane] = f;
             }
-        cs[0] = __shfl_sync(0xffffffffu, undo, 8 * s.c);
-        cs[1] = __shfl_sync(0xffffffffu, undo, 8 * s.c + 4);
+        if (s.c == 0) undos[s.g] = undo;
+    }
+
+    // `write`: the warp that lays out the tile's Q fragments.
+    __device__ __forceinline__ void Begin(const TreeArgs& a, const TreeSplit& sp, const Step& s, int seq, int head,
+                                          const float* q, uint4* frags, float* undos, bool write) {
+        qs = frags + s.lane;
+        magic = sp.magic;
+        const long long row = a.c.Row(seq, a.layer, head, 0);
+        k = static_cast<const uint8_t*>(a.c.k) + row * NB * kQuantBytes;
+        v = static_cast<const uint8_t*>(a.c.v) + row * NB * kQuantBytes;
+        ks = a.c.ks + row * NB;
+        vs = a.c.vs + row * NB;
+        stored = a.c.head_rows;
+        if (write) LayOut(a, s, q, frags, undos);
         m[0] = m[1] = kStart;
         l[0] = l[1] = 0.0f;
-        e = -15;
+        SetPower(-15);
 #pragma unroll
         for (int b = 0; b < NB; ++b)
 #pragma unroll
             for (int i = 0; i < 8; ++i) o[b][i >> 2][i & 3] = 0.0f;
     }
 
-    __device__ __forceinline__ void Prefetch(const Step& s, int p0) const {
-        if (s.lane != 0 || p0 >= s.slots) return;
-        const uint32_t n = min(kUnit, stored - p0);  // a multiple of 8
+    __device__ __forceinline__ void SetPower(int to) {
+        e = to;
+        bound = Pow2(to);
+        down = __float2half2_rn(Pow2(-to));
+    }
+
+    // Slots p0 .. p1 - 1 (p0 a multiple of 16) into the L2.
+    __device__ __forceinline__ void Prefetch(const Step& s, int p0, int p1) const {
+        if (s.lane != 0) return;
+        const uint32_t n = min((p1 + 7) & ~7, stored) - p0;
         BulkPrefetchL2(k + size_t(p0) * NB * kQuantBytes, n * NB * kQuantBytes);
         BulkPrefetchL2(v + size_t(p0) * NB * kQuantBytes, n * NB * kQuantBytes);
         BulkPrefetchL2(ks + size_t(p0) * NB, n * NB * 2);
@@ -278,21 +328,22 @@ struct QuantWarp {
     }
 
     __device__ __forceinline__ void LoadK(const Step& s, int p0) {
+        const uint8_t* row = k + size_t(p0 + s.g) * (NB * kQuantBytes) + 4 * kKWords * s.c;
+        const __half* sc = ks + size_t(p0 + s.g) * NB;
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
-            const int p = min(p0 + s.g + 8 * r, stored - 1);
-            const uint8_t* at = k + size_t(p) * NB * kQuantBytes;
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
+                const uint8_t* at = row + 8 * r * (NB * kQuantBytes) + b * kQuantBytes;
                 if constexpr (TYPE == MLB_Q8_0) {
-                    const uint2 w = __ldg(reinterpret_cast<const uint2*>(at + b * 32 + 8 * s.c));
+                    const uint2 w = __ldg(reinterpret_cast<const uint2*>(at));
                     kw[r][b][0] = w.x;
                     kw[r][b][1] = w.y;
                 } else {
-                    kw[r][b][0] = __ldg(reinterpret_cast<const uint32_t*>(at + b * 16 + 4 * s.c));
+                    kw[r][b][0] = __ldg(reinterpret_cast<const uint32_t*>(at));
                 }
             }
-            LoadScales<NB>(ks + size_t(p) * NB, kd[r]);
+            LoadScales<NB>(sc + 8 * r * NB, kd[r]);
         }
     }
 
@@ -304,22 +355,26 @@ struct QuantWarp {
 #pragma unroll
             for (int r = 0; r < 2; ++r) {
                 if constexpr (TYPE == MLB_Q8_0) {
-                    BytesToHalf(kw[r][b][0] ^ 0x80808080u, f[0][r], f[0][2 + r]);
-                    BytesToHalf(kw[r][b][1] ^ 0x80808080u, f[1][r], f[1][2 + r]);
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        f[i][r] = EvenBytes(kw[r][b][i], magic);
+                        f[i][2 + r] = EvenBytes(kw[r][b][i] >> 8, magic);
+                    }
                 } else {
                     const uint32_t w = kw[r][b][0], u = w >> 8;
-                    f[0][r] = LowNibbles(w);
-                    f[0][2 + r] = LowNibbles(u);
-                    f[1][r] = HighNibbles(w);
-                    f[1][2 + r] = HighNibbles(u);
+                    f[0][r] = LowNibbles(w, magic);
+                    f[0][2 + r] = LowNibbles(u, magic);
+                    f[1][r] = HighNibbles(w, magic);
+                    f[1][2 + r] = HighNibbles(u, magic);
                 }
             }
-            float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-            Mma(d, f[0], qh[b][0][0], qh[b][0][1]);
-            Mma(d, f[1], qh[b][1][0], qh[b][1][1]);
-            Mma(d, f[0], ql[b][0][0], ql[b][0][1]);
-            Mma(d, f[1], ql[b][1][0], ql[b][1][1]);
-            const float d0 = HalfBits(kd[0][b]), d1 = HalfBits(kd[1][b]);
+            float d[4];
+            const uint4 q0 = qs[(2 * b) * 32], q1 = qs[(2 * b + 1) * 32];
+            MmaFirst(d, f[0], q0.z, q0.w);
+            Mma(d, f[1], q1.z, q1.w);
+            Mma(d, f[0], q0.x, q0.y);
+            Mma(d, f[1], q1.x, q1.y);
+            const float d0 = ScaleOf(kd[0], b), d1 = ScaleOf(kd[1], b);
             x[0] = fmaf(d0, d[0], x[0]);
             x[1] = fmaf(d0, d[1], x[1]);
             x[2] = fmaf(d1, d[2], x[2]);
@@ -339,30 +394,42 @@ struct QuantWarp {
             }
     }
 
-    // One unit of slots from p0; its K is loaded, `next` is the K to load.
-    __device__ __forceinline__ void Unit(const Step& s, int p0, int next) {
+    // After the barrier that follows Begin.
+    __device__ __forceinline__ void Ready(const Step& s, const float* undos) {
+        cs[0] = undos[2 * s.c];
+        cs[1] = undos[2 * s.c + 1];
+    }
+
+    // One unit of slots from p0, those below `low` another's; its K is loaded,
+    // `next` is the K to load.
+    __device__ __forceinline__ void Unit(const Step& s, int p0, int low, int next) {
+        // slots 2c, 2c + 1, 2c + 8, 2c + 9
         uint32_t vw[NB][TYPE == MLB_Q8_0 ? 4 : 2];
-        uint16_t vd[4][NB];
-        const int at[4] = {min(p0 + 2 * s.c, stored - 1), min(p0 + 2 * s.c + 1, stored - 1),
-                           min(p0 + 2 * s.c + 8, stored - 1), min(p0 + 2 * s.c + 9, stored - 1)};
+        uint32_t vd[4][(NB + 1) / 2];
+        {
+            const int p = p0 + 2 * s.c;
+            const uint8_t* row = v + size_t(p) * (NB * kQuantBytes) + (kQuantBytes / 8) * s.g;
+            const __half* sc = vs + size_t(p) * NB;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            LoadScales<NB>(vs + size_t(at[i]) * NB, vd[i]);
+            for (int i = 0; i < 4; ++i) {
+                const int more = (i & 1) + (i >> 1) * 8;
+                LoadScales<NB>(sc + more * NB, vd[i]);
 #pragma unroll
-            for (int b = 0; b < NB; ++b) {
-                const uint8_t* p = v + size_t(at[i]) * NB * kQuantBytes + b * kQuantBytes;
-                if constexpr (TYPE == MLB_Q8_0) {
-                    vw[b][i] = __ldg(reinterpret_cast<const uint32_t*>(p + 4 * s.g));
-                } else {
-                    const uint32_t w = __ldg(reinterpret_cast<const unsigned short*>(p + 2 * s.g));
-                    vw[b][i >> 1] = i & 1 ? vw[b][i >> 1] | (w << 16) : w;
+                for (int b = 0; b < NB; ++b) {
+                    const uint8_t* at = row + more * (NB * kQuantBytes) + b * kQuantBytes;
+                    if constexpr (TYPE == MLB_Q8_0) {
+                        vw[b][i] = __ldg(reinterpret_cast<const uint32_t*>(at));
+                    } else {
+                        const uint32_t w = __ldg(reinterpret_cast<const unsigned short*>(at));
+                        vw[b][i >> 1] = i & 1 ? vw[b][i >> 1] | (w << 16) : w;
+                    }
                 }
             }
         }
         float x[4];
         Scores(x);
         if (next >= 0) LoadK(s, next);
-        Weights(s, p0, x, cs[0], cs[1], kOffset, m, l, [&](float r0, float r1) { ScaleColumns(r0, r1); });
+        Weights(s, p0, low, x, cs[0], cs[1], kOffset, m, l, [&](float r0, float r1) { ScaleColumns(r0, r1); });
         // weights as B fragments: row (query) g, slots 2c, 2c + 1 (+ 8)
         uint32_t ph0, pl0, ph1, pl1;
         SplitHalf(x[0], x[1], ph0, pl0);
@@ -372,29 +439,33 @@ struct QuantWarp {
         pl0 = Transpose8x8(pl0);
         pl1 = Transpose8x8(pl1);
         uint32_t d0[NB], d1[NB];
-        uint32_t see0 = 0xffffffffu, see1 = 0xffffffffu;
-        if (p0 + kUnit > s.len) {  // a slot that is not seen may hold any scale, NaN too
-            see0 = __hne2_mask(AsHalf2(ph0), AsHalf2(0u));
-            see1 = __hne2_mask(AsHalf2(ph1), AsHalf2(0u));
-        }
-        __half2 big = AsHalf2(0u);
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
-            d0[b] = (uint32_t(vd[0][b]) | (uint32_t(vd[1][b]) << 16)) & see0;
-            d1[b] = (uint32_t(vd[2][b]) | (uint32_t(vd[3][b]) << 16)) & see1;
-            big = __hmax2(big, __hmax2(AsHalf2(d0[b]), AsHalf2(d1[b])));
+            const int pick = b & 1 ? 0x7632 : 0x5410;  // block b of two slots
+            d0[b] = __byte_perm(vd[0][b >> 1], vd[1][b >> 1], pick);
+            d1[b] = __byte_perm(vd[2][b >> 1], vd[3][b >> 1], pick);
         }
+        if (low + kUnit > s.len) {  // a slot that is not seen may hold any scale, NaN too
+            const uint32_t see0 = __hne2_mask(AsHalf2(ph0), AsHalf2(0u)), see1 = __hne2_mask(AsHalf2(ph1), AsHalf2(0u));
+#pragma unroll
+            for (int b = 0; b < NB; ++b) {
+                d0[b] &= see0;
+                d1[b] &= see1;
+            }
+        }
+        __half2 big = __hmax2(AsHalf2(d0[0]), AsHalf2(d1[0]));
+#pragma unroll
+        for (int b = 1; b < NB; ++b) big = __hmax2(big, __hmax2(AsHalf2(d0[b]), AsHalf2(d1[b])));
         const float top = fmaxf(__low2float(big), __high2float(big));
-        if (__any_sync(0xffffffffu, top > Pow2(e))) {
+        if (__any_sync(0xffffffffu, top > bound)) {
             float t = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
             t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 2));
             // 2^ne > t, ne within the powers that a half can scale by
             const int ne = max(e, min(15, max(-15, static_cast<int>(__float_as_uint(t) >> 23) - 126)));
             const float f = Pow2(e - ne);
-            e = ne;
+            SetPower(ne);
             ScaleColumns(__shfl_sync(0xffffffffu, f, 8 * s.c), __shfl_sync(0xffffffffu, f, 8 * s.c + 4));
         }
-        const __half2 down = __float2half2_rn(Pow2(-e));
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
             const __half2 s0 = __hmul2(AsHalf2(d0[b]), down), s1 = __hmul2(AsHalf2(d1[b]), down);
@@ -404,25 +475,31 @@ struct QuantWarp {
             uint32_t f[2][4];
             if constexpr (TYPE == MLB_Q8_0) {
 #pragma unroll
-                for (int r = 0; r < 2; ++r) {  // slots 2c, 2c + 1, then + 8
-                    const uint32_t w0 = vw[b][2 * r] ^ 0x80808080u, w1 = vw[b][2 * r + 1] ^ 0x80808080u;
-                    BytesToHalf(__byte_perm(w0, w1, 0x5140), f[0][2 * r], f[0][2 * r + 1]);
-                    BytesToHalf(__byte_perm(w0, w1, 0x7362), f[1][2 * r], f[1][2 * r + 1]);
+                for (int r = 0; r < 2; ++r) {  // slots 2c, 2c + 1, then + 8: bytes of the two side by side
+                    const uint32_t low = __byte_perm(vw[b][2 * r], vw[b][2 * r + 1], 0x5410);
+                    const uint32_t high = __byte_perm(vw[b][2 * r], vw[b][2 * r + 1], 0x7632);
+                    f[0][2 * r] = EvenBytes(low, magic);
+                    f[0][2 * r + 1] = EvenBytes(low >> 8, magic);
+                    f[1][2 * r] = EvenBytes(high, magic);
+                    f[1][2 * r + 1] = EvenBytes(high >> 8, magic);
                 }
             } else {
 #pragma unroll
                 for (int r = 0; r < 2; ++r) {
                     const uint32_t w = vw[b][r], u = w >> 8;
-                    f[0][2 * r] = LowNibbles(w);
-                    f[0][2 * r + 1] = LowNibbles(u);
-                    f[1][2 * r] = HighNibbles(w);
-                    f[1][2 * r + 1] = HighNibbles(u);
+                    f[0][2 * r] = LowNibbles(w, magic);
+                    f[0][2 * r + 1] = LowNibbles(u, magic);
+                    f[1][2 * r] = HighNibbles(w, magic);
+                    f[1][2 * r + 1] = HighNibbles(u, magic);
                 }
             }
-            Mma(o[b][0], f[0], H2(h0), H2(h1));
-            Mma(o[b][1], f[1], H2(h0), H2(h1));
-            Mma(o[b][0], f[0], l0, l1);
-            Mma(o[b][1], f[1], l0, l1);
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                float d[4];
+                MmaFirst(d, f[j], l0, l1);
+                Mma(d, f[j], H2(h0), H2(h1));
+                AddTo(o[b][j], d);
+            }
         }
     }
 
@@ -440,17 +517,17 @@ struct F32Warp {
     float m[2], l[2], cs[2];
     const float *k, *v;
     size_t pitch;  // floats between slots
-    int hd, last;
+    int hd;
 
     __device__ __forceinline__ static int Dim(int g, int j, int half) { return 4 * g + 2 * j + half; }
 
-    __device__ __forceinline__ void Begin(const TreeArgs& a, const Step& s, int seq, int head, const float* qr) {
+    __device__ __forceinline__ void Begin(const TreeArgs& a, const TreeSplit&, const Step& s, int seq, int head,
+                                          const float* qr, uint4*, float*, bool) {
         const long long row = a.c.Row(seq, a.layer, head, 0);
         k = static_cast<const float*>(a.c.k) + row * a.c.hd;
         v = static_cast<const float*>(a.c.v) + row * a.c.hd;
         pitch = size_t(a.c.n_kv) * a.c.hd;
         hd = a.c.hd;
-        last = a.c.max_seq - 1;
 #pragma unroll
         for (int b = 0; b < NB; ++b)
 #pragma unroll
@@ -464,18 +541,18 @@ struct F32Warp {
         l[0] = l[1] = 0.0f;
     }
 
-    __device__ __forceinline__ void Prefetch(const Step& s, int p0) const {
-        // a lane per 128-byte line of the unit's rows
+    __device__ __forceinline__ void Prefetch(const Step& s, int p0, int p1) const {
+        // a lane per 128-byte line of the slots' rows
         const int lines = (hd * 4 + 127) / 128;
-        for (int i = s.lane; i < kUnit * lines; i += 32) {
+        for (int i = s.lane; i < (p1 - p0) * lines; i += 32) {
             const int p = p0 + i / lines;
-            if (p >= s.slots) break;
             const size_t at = size_t(p) * pitch + (i % lines) * 32;
             asm volatile("prefetch.global.L2 [%0];" ::"l"(k + at));
             asm volatile("prefetch.global.L2 [%0];" ::"l"(v + at));
         }
     }
 
+    __device__ __forceinline__ void Ready(const Step&, const float*) {}
     __device__ __forceinline__ void LoadK(const Step&, int) {}
 
     __device__ __forceinline__ void ScaleColumns(float r0, float r1) {
@@ -494,12 +571,12 @@ struct F32Warp {
         return d < hd ? __ldg(reinterpret_cast<const float4*>(p + d)) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     }
 
-    __device__ __forceinline__ void Unit(const Step& s, int p0, int) {
-        float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    __device__ __forceinline__ void Unit(const Step& s, int p0, int low, int) {
+        float x[4] = {0.0f, 0.0f, 0.0f, 0.0f}, rest[4] = {0.0f, 0.0f, 0.0f, 0.0f};
         float4 kr[2][NB][2];
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
-            const float* row = k + size_t(min(p0 + s.g + 8 * r, last)) * pitch;
+            const float* row = k + size_t(p0 + s.g + 8 * r) * pitch;
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
                 kr[r][b][0] = Load(row, b * 32 + 8 * s.c);
@@ -518,19 +595,20 @@ struct F32Warp {
                 SplitTf32(i & 1 ? rb.w : rb.y, h[3], w[3]);
                 SplitTf32(q[b][2 * i], qh[0], qw[0]);
                 SplitTf32(q[b][2 * i + 1], qh[1], qw[1]);
-                MmaTf32(x, w, qh[0], qh[1]);
-                MmaTf32(x, h, qw[0], qw[1]);
+                MmaTf32(rest, w, qh[0], qh[1]);
+                MmaTf32(rest, h, qw[0], qw[1]);
                 MmaTf32(x, h, qh[0], qh[1]);
             }
+        AddTo(x, rest);
         float4 vr[4][NB];  // slots c, c + 4, c + 8, c + 12
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const float* row = v + size_t(min(p0 + s.c + 4 * i, last)) * pitch;
+            const float* row = v + size_t(p0 + s.c + 4 * i) * pitch;
 #pragma unroll
             for (int b = 0; b < NB; ++b) vr[i][b] = Load(row, b * 32 + 4 * s.g);
         }
-        Weights(s, p0, x, cs[0], cs[1], 0.0f, m, l, [&](float r0, float r1) { ScaleColumns(r0, r1); });
-        if (p0 + kUnit > s.len) {
+        Weights(s, p0, low, x, cs[0], cs[1], 0.0f, m, l, [&](float r0, float r1) { ScaleColumns(r0, r1); });
+        if (low + kUnit > s.len) {
             bool odd = false;  // a slot that some rows do not see may hold NaN or infinities
 #pragma unroll
             for (int i = 0; i < 4; ++i)
@@ -551,32 +629,33 @@ struct F32Warp {
             const float even = __shfl_sync(0xffffffffu, x[i & 2], src), odd = __shfl_sync(0xffffffffu, x[(i & 2) + 1], src);
             pw[i] = s.g & 1 ? odd : even;
         }
+        uint32_t ph[4], pl[4];
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            uint32_t ph[2], pl[2];
-            SplitTf32(pw[2 * i], ph[0], pl[0]);
-            SplitTf32(pw[2 * i + 1], ph[1], pl[1]);
+        for (int i = 0; i < 4; ++i) SplitTf32(pw[i], ph[i], pl[i]);
 #pragma unroll
-            for (int b = 0; b < NB; ++b) {
-                const float4 va = vr[2 * i][b], vb = vr[2 * i + 1][b];
+        for (int b = 0; b < NB; ++b)
 #pragma unroll
-                for (int j = 0; j < 2; ++j) {
+            for (int j = 0; j < 2; ++j) {
+                float d[4];
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const float4 va = vr[2 * i][b], vb = vr[2 * i + 1][b];
                     uint32_t h[4], w[4];
                     SplitTf32(j ? va.z : va.x, h[0], w[0]);
                     SplitTf32(j ? va.w : va.y, h[1], w[1]);
                     SplitTf32(j ? vb.z : vb.x, h[2], w[2]);
                     SplitTf32(j ? vb.w : vb.y, h[3], w[3]);
-                    MmaTf32(o[b][j], w, ph[0], ph[1]);
-                    MmaTf32(o[b][j], h, pl[0], pl[1]);
-                    MmaTf32(o[b][j], h, ph[0], ph[1]);
+                    i == 0 ? MmaTf32First(d, w, ph[0], ph[1]) : MmaTf32(d, w, ph[2], ph[3]);
+                    MmaTf32(d, h, pl[2 * i], pl[2 * i + 1]);
+                    MmaTf32(d, h, ph[2 * i], ph[2 * i + 1]);
                 }
+                AddTo(o[b][j], d);
             }
-        }
     }
 
     // The weighted values of one unit slot by slot, those of weight 0 left out.
     __device__ __forceinline__ void Plainly(const Step& s, int p0, const float (&x)[4]) {
-        for (int i = 0; i < kUnit && p0 + i < s.slots; ++i) {
+        for (int i = 0; i < kUnit && p0 + i < s.slots; ++i) {  // weights of slots below `low` are 0
             const int src = 4 * (i & 7) + s.c;
             const float w0 = __shfl_sync(0xffffffffu, i < 8 ? x[0] : x[2], src);
             const float w1 = __shfl_sync(0xffffffffu, i < 8 ? x[1] : x[3], src);
@@ -664,6 +743,8 @@ __global__ void __launch_bounds__(NW * 32, 1) TreeMmaKernel(TreeArgs a, TreeSpli
     float* so = reinterpret_cast<float*>(smem4);  // [NW][kRows][kPitch]
     float* sm = so + NW * kRows * kPitch;         // [NW][kRows]
     float* sl = sm + NW * kRows;
+    float* su = sl + NW * kRows;                            // [4][kRows]
+    uint4* sq = reinterpret_cast<uint4*>(su + 4 * kRows);   // [wq][2 NB][32], quantized caches
     __shared__ int s_last;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int nt = warp % sp.wq, wp = warp / sp.wq, wps = NW / sp.wq;
@@ -737,20 +818,31 @@ __global__ void __launch_bounds__(NW * 32, 1) TreeMmaKernel(TreeArgs a, TreeSpli
         s.t0 = (tile + 2 * s.c) / a.group;
         s.t1 = (tile + 2 * s.c + 1) / a.group;
         float* to = so + (warp * kRows + 2 * s.c) * kPitch;
-        if (tile < sp.rows) {
+        const bool live = tile < sp.rows;
+        if (live) {
             const int r = tile + s.g;
             const float* q = r < sp.rows ? a.q + (size_t(b) * a.tokens + r / a.group) * a.q_stride +
                                                size_t(head * a.group + r % a.group) * a.c.hd
                                          : nullptr;
+            w.Begin(a, sp, s, e.seq, head, q, sq + nt * 2 * NB * 32, su + nt * kRows, wp == 0);
+            // the last unit of the plane may hold 8 slots only: it starts earlier and leaves out the others
+            const int top = a.c.head_slots - kUnit;
+            // a round is a unit of every warp; the warps take turns to prefetch one
+            const int span = wps * kUnit;
+            if (nt == 0 && wp < kAhead && u0 * kUnit + (wp + 1) * span < e.slots && (wp + 1) * wps < u1 - u0)
+                w.Prefetch(s, u0 * kUnit + (wp + 1) * span, min(min(u0 * kUnit + (wp + 2) * span, u1 * kUnit), e.slots));
+            if (u0 + wp < u1) w.LoadK(s, min((u0 + wp) * kUnit, top));
+        }
+        if (TYPE != MLB_F32) __syncthreads();
+        if (live) {
+            w.Ready(s, su + nt * kRows);
+            const int top = a.c.head_slots - kUnit, span = wps * kUnit;
             int u = u0 + wp;
-            w.Begin(a, s, e.seq, head, q);
-            if (u < u1) w.LoadK(s, u * kUnit);
-            if (nt == 0)
-                for (int i = 1; i < kAhead; ++i)
-                    if (u + i * wps < u1) w.Prefetch(s, (u + i * wps) * kUnit);
-            for (; u < u1; u += wps) {
-                if (nt == 0 && u + kAhead * wps < u1) w.Prefetch(s, (u + kAhead * wps) * kUnit);
-                w.Unit(s, u * kUnit, u + wps < u1 ? (u + wps) * kUnit : -1);
+            for (int round = 0; u < u1; u += wps, ++round) {
+                const int ahead = (u0 + (round + kAhead + 1) * wps) * kUnit;
+                if (nt == 0 && round % wps == wp && ahead < min(u1 * kUnit, e.slots))
+                    w.Prefetch(s, ahead, min(min(ahead + span, u1 * kUnit), e.slots));
+                w.Unit(s, min(u * kUnit, top), u * kUnit, u + wps < u1 ? min((u + wps) * kUnit, top) : -1);
             }
             w.End(s);
 #pragma unroll
@@ -859,7 +951,10 @@ int* Counters(DeviceContext& ctx, size_t n) {
 template <int TYPE, int NB>
 void Launch(DeviceContext& ctx, const TreeArgs& a) {
     // registers per thread bound the warps: fp32 units hold twice the values
-    constexpr int NW = TYPE == MLB_F32 && NB > 2 ? 8 : 12;
+    #ifndef TREE_NW
+#define TREE_NW 12
+#endif
+    constexpr int NW = TYPE == MLB_F32 && NB > 2 ? 8 : TREE_NW;
     TreeSplit sp{};
     sp.rows = a.tokens * a.group;
     sp.wq = sp.rows <= kRows ? 1 : (sp.rows <= 2 * kRows ? 2 : 4);
@@ -871,8 +966,10 @@ void Launch(DeviceContext& ctx, const TreeArgs& a) {
     const int grid = static_cast<int>(std::max(1LL, std::min<long long>(ctx.sm_count, (units + per_cta - 1) / per_cta)));
     const size_t part = size_t(kRows) * sp.wq * (NB * 32 + 2) * sizeof(float);
     sp.parts = static_cast<float*>(Workspace(ctx, 2 * size_t(grid) * part));
+    sp.magic = TYPE == MLB_Q8_0 ? kMagic8 : kMagic4;
     sp.counters = Counters(ctx, size_t(a.batch) * items);
-    constexpr size_t smem = size_t(NW) * kRows * (JoinPitch<NB>() + 2) * sizeof(float);
+    constexpr size_t smem = (size_t(NW) * kRows * (JoinPitch<NB>() + 2) + 4 * kRows) * sizeof(float) +
+                            (TYPE == MLB_F32 ? 0 : 4 * 2 * NB * 32 * sizeof(uint4));
     auto* kernel = TreeMmaKernel<TYPE, NB, NW>;
     if (smem > 48 * 1024)
         CheckCuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem),
@@ -895,6 +992,7 @@ bool LaunchBlocks(DeviceContext& ctx, const TreeArgs& a) {
 }  // namespace
 
 bool LaunchTreeMma(DeviceContext& ctx, const TreeArgs& a) {
+    if (a.c.head_slots < kUnit) return false;  // a unit is 16 slots
     if (a.c.type == MLB_F32) return a.cache_vec && LaunchBlocks<MLB_F32>(ctx, a);
     return a.c.type == MLB_Q8_0 ? LaunchBlocks<MLB_Q8_0>(ctx, a) : LaunchBlocks<MLB_Q4_0>(ctx, a);
 }
