@@ -47,7 +47,13 @@ __device__ __forceinline__ bool SeesDraft(const uint64_t* bits, int t, int j) {
 }
 
 
-// The matrix-instruction kernel (tree_mma.cu); false: the shape is not one of its.
-bool LaunchTreeMma(DeviceContext& ctx, const TreeArgs& a);
+// The matrix-instruction kernels (tree_mma.cuh); false: the shape is not one of
+// theirs.
+bool LaunchTreeF32(DeviceContext& ctx, const TreeArgs& a);
+bool LaunchTreeQ80(DeviceContext& ctx, const TreeArgs& a);
+bool LaunchTreeQ40(DeviceContext& ctx, const TreeArgs& a);
+
+// `n` arrival counters, zero between launches.
+int* TreeCounters(DeviceContext& ctx, size_t n);
 
 }  // namespace mlb

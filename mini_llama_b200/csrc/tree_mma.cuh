@@ -1,0 +1,1088 @@
+// Attention of drafted tokens on the warp-level matrix instructions: few query
+// rows per KV head, the cache read once.
+//
+// The R = tokens x (query heads per KV head) rows that share a KV head are cut
+// into tiles of eight: the N side of mma.m16n8k16.  A warp takes 16 slots of
+// the cache at a time (the M side, S^T = K Q^T) for NT = 1 or 2 tiles of rows:
+//   K      the 16 x head_dim quants as A fragments (the order of the elements
+//          within a block is free, as Q is laid out in the same one), fp16 whole
+//          numbers: exact.  Q is scaled per row by a power of two and split into
+//          fp16 hi + lo (22 bits), so a block's products are exact up to the
+//          fp32 sum; the slot's scale of the block multiplies that sum.
+//   softmax  running maximum and sum per row, the maximum moved only when a
+//          score passes it by 2^2 (a vote): weights are 2^(x - m + 12) <= 2^14,
+//          split into fp16 hi + lo and turned into B fragments by movmatrix.
+//   V      O^T = V^T P^T: quants as exact fp16 A fragments again (byte
+//          transposition in registers); the slot's scale of a block goes into
+//          the weights, P' = hi + lo of p d by one product and two FMAs on half
+//          pairs, relative to a power of two per row that covers the largest d
+//          seen.  Two MMAs per fragment.
+// fp32 caches take the same path with mma.m16n8k8 on tf32 hi + lo pairs (three
+// products; no ranges to mind).  A unit's weighted values are summed in fresh
+// accumulators and added to the running ones in fp32 with rounding to nearest:
+// the matrix unit's own additions truncate, which over a long context would
+// cost several times the fp32 rounding.
+//
+// The units of 16 slots of all (sequence, KV head, row group) items are one
+// list, cut evenly over the CTAs (the lengths are on the device, so every CTA
+// works the cut out from them): sequences of any lengths balance.  A CTA's
+// stretch is dealt out to groups of WQ warps, one tile pair of the item's rows
+// each; a group brings its units into a ring of S stages in shared memory
+// (cp.async, S - 1 units ahead; rows an odd number of 16-byte chunks apart, so
+// every fragment load is free of bank conflicts) and meets at a named barrier
+// once per unit.  The groups join their results in shared memory, and items that
+// are cut between CTAs are joined by the CTA that finishes last (partials in the
+// workspace, one counter per item, added in a fixed order).
+#pragma once
+
+#include <algorithm>
+#include <cmath>
+
+#include "tree_attention.cuh"
+
+namespace mlb {
+
+namespace {
+
+constexpr int kUnit = 16;           // slots of a matrix step
+constexpr int kRows = 8;            // query rows of a tile
+constexpr float kStart = -1.7e38f;  // running maximum before the first score (finite: no inf - inf)
+constexpr float kLag = 2.0f;        // how far scores may pass the running maximum, in powers of two
+constexpr float kOffset = 12.0f;    // weights are relative to 2^12: at most 2^14, and the fp16 pairs resolve
+                                    // 2^-37 of the largest, for slots that weigh little where the heavy ones hold zeros
+constexpr float kLog2e = 1.4426950408889634f;
+
+constexpr int kMaxShared = 225 * 1024;
+constexpr int kMaxStages = 4;
+
+// Warps of a CTA by form (one, two tiles per warp; two tiles and four warps to a
+// group): registers and the ring bound them.
+#ifndef TREE_W1
+#define TREE_W1 12
+#endif
+template <int TYPE, int NB>
+constexpr int kWarps1 = TYPE == MLB_F32 ? (NB > 2 ? 6 : 12) : TREE_W1;
+template <int TYPE, int NB>
+constexpr int kWarps2 = TYPE == MLB_F32 ? (NB > 2 ? 6 : 12) : 12;
+template <int TYPE, int NB>
+constexpr int kWarps4 = TYPE == MLB_F32 && NB > 2 ? 8 : 12;
+
+struct TreeSplit {
+    int groups;    // items of a (sequence, KV head): ceil(R / (8 NT WQ))
+    int rows;      // R
+    float* parts;  // two partial results per CTA
+    int* counters; // per item
+    uint32_t magic;
+};
+
+__device__ __forceinline__ void Mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+        "{%0, %1, %2, %3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ void MmaTf32(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+        "{%0, %1, %2, %3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// The same with a zero accumulator.
+__device__ __forceinline__ void MmaFirst(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+        "{%10, %10, %10, %10};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
+}
+
+__device__ __forceinline__ void MmaTf32First(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+        "{%10, %10, %10, %10};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
+}
+
+__device__ __forceinline__ void AddTo(float (&o)[4], const float (&d)[4]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o[i] += d[i];
+}
+
+__device__ __forceinline__ uint32_t Transpose8x8(uint32_t v) {
+    uint32_t r;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+    return r;
+}
+
+__device__ __forceinline__ float Exp2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+__device__ __forceinline__ uint32_t H2(__half2 v) { return *reinterpret_cast<uint32_t*>(&v); }
+__device__ __forceinline__ __half2 AsHalf2(uint32_t v) { return *reinterpret_cast<__half2*>(&v); }
+
+// (x, y) rounded to halves, and what the rounding left, rounded too.
+__device__ __forceinline__ void SplitHalf(float x, float y, uint32_t& hi, uint32_t& lo) {
+    const __half2 h = __floats2half2_rn(x, y);
+    const float2 f = __half22float2(h);
+    hi = H2(h);
+    lo = H2(__floats2half2_rn(x - f.x, y - f.y));
+}
+
+// x as tf32 (rounded to nearest, halves up) and the rest, whose low 13 bits the
+// matrix unit does not read: together 2^-21 relative at worst.
+__device__ __forceinline__ void SplitTf32(float x, uint32_t& hi, uint32_t& lo) {
+    hi = (__float_as_uint(x) + 0x1000u) & 0xffffe000u;
+    lo = __float_as_uint(x - __uint_as_float(hi));
+}
+
+// int8 in bytes 0 and 2 of w as a half pair: byte ^ 0x80 is q + 128, and the half
+// 0x6400 + u is 1024 + u.  `magic` (kMagic8, kMagic4) comes from the kernel's
+// parameters: as a literal it would not fit the one logic instruction beside the
+// mask.
+constexpr uint32_t kMagic8 = 0x64806480u, kMagic4 = 0x64006400u;
+__device__ __forceinline__ uint32_t EvenBytes(uint32_t w, uint32_t magic) {
+    return H2(__hsub2(AsHalf2((w & 0x00ff00ffu) ^ magic), AsHalf2(kMagic8)));  // - (1024 + 128)
+}
+
+// The nibbles of bytes 0 and 2: low ones n - 8, high ones n - 8.
+__device__ __forceinline__ uint32_t LowNibbles(uint32_t w, uint32_t magic) {
+    return H2(__hsub2(AsHalf2((w & 0x000F000Fu) | magic), AsHalf2(0x64086408u)));  // 1024 + n - 1032
+}
+__device__ __forceinline__ uint32_t HighNibbles(uint32_t w, uint32_t magic) {
+    // (1024 + 16 n) / 16 - 72
+    return H2(__hfma2(AsHalf2((w & 0x00F000F0u) | magic), AsHalf2(0x2C002C00u), AsHalf2(0xD480D480u)));
+}
+
+// The fp16 scales of one slot's blocks in shared memory, two to a word.
+template <int NB>
+__device__ __forceinline__ void LoadScales(const __half* p, uint32_t (&d)[(NB + 1) / 2]) {
+    if constexpr (NB % 4 == 0) {
+#pragma unroll
+        for (int i = 0; i < NB / 4; ++i) {
+            const uint2 w = reinterpret_cast<const uint2*>(p)[i];
+            d[2 * i] = w.x;
+            d[2 * i + 1] = w.y;
+        }
+    } else if constexpr (NB % 2 == 0) {
+#pragma unroll
+        for (int i = 0; i < NB / 2; ++i) d[i] = reinterpret_cast<const uint32_t*>(p)[i];
+    } else {
+        const unsigned short* h = reinterpret_cast<const unsigned short*>(p);
+#pragma unroll
+        for (int i = 0; i < NB / 2; ++i) d[i] = h[2 * i] | (uint32_t(h[2 * i + 1]) << 16);
+        d[NB / 2] = h[NB - 1];
+    }
+}
+
+template <int N>
+__device__ __forceinline__ float ScaleOf(const uint32_t (&d)[N], int b) {
+    return b & 1 ? __high2float(AsHalf2(d[b >> 1])) : __low2float(AsHalf2(d[b >> 1]));
+}
+
+// The rows, lengths and mask that a warp's step needs, common to all forms.
+struct Step {
+    int lane, g, c;  // lane = 4 g + c
+    int slots, len, tokens, words;
+    const uint64_t* mask;  // the batch entry's
+};
+
+__device__ __forceinline__ bool Sees(const Step& s, int t, int slot) {
+    if (slot < s.len) return true;
+    if (slot >= s.slots || t >= s.tokens) return false;
+    return SeesDraft(s.mask ? s.mask + size_t(t) * s.words : nullptr, t, slot - s.len);
+}
+
+// One tile of rows: drafted tokens, running maxima and sums of the thread's two
+// score columns (queries 2c, 2c + 1).
+struct Columns {
+    int t0, t1;
+    float m[2], l[2], cs[2];
+
+    __device__ __forceinline__ void Begin(int t_a, int t_b) {
+        t0 = t_a;
+        t1 = t_b;
+        m[0] = m[1] = kStart;
+        l[0] = l[1] = 0.0f;
+    }
+
+    // Scores (C fragment: rows slot g, g + 8; columns query 2c, 2c + 1) of the
+    // unit at p0, slots from `low` on, to weights 2^(x - m + offset); `rescale`
+    // gets the factors of a moved maximum.
+    template <typename Rescale>
+    __device__ __forceinline__ void Weights(const Step& s, int p0, int low, float (&x)[4], float offset,
+                                            Rescale&& rescale) {
+        if (low + kUnit > s.len) {  // drafted slots, or the end
+            const int a = p0 + s.g, b = a + 8;
+            if (a < low || !Sees(s, t0, a)) x[0] = -INFINITY;
+            if (a < low || !Sees(s, t1, a)) x[1] = -INFINITY;
+            if (b < low || !Sees(s, t0, b)) x[2] = -INFINITY;
+            if (b < low || !Sees(s, t1, b)) x[3] = -INFINITY;
+        }
+        float top0 = fmaxf(x[0], x[2]) * cs[0], top1 = fmaxf(x[1], x[3]) * cs[1];
+        if (__any_sync(0xffffffffu, top0 > m[0] + kLag || top1 > m[1] + kLag)) {
+#pragma unroll
+            for (int o = 4; o < 32; o <<= 1) {
+                top0 = fmaxf(top0, __shfl_xor_sync(0xffffffffu, top0, o));
+                top1 = fmaxf(top1, __shfl_xor_sync(0xffffffffu, top1, o));
+            }
+            const float n0 = fmaxf(m[0], top0), n1 = fmaxf(m[1], top1);
+            const float r0 = Exp2(m[0] - n0), r1 = Exp2(m[1] - n1);
+            m[0] = n0;
+            m[1] = n1;
+            l[0] *= r0;
+            l[1] *= r1;
+            rescale(r0, r1);
+        }
+        const float o0 = offset - m[0], o1 = offset - m[1];
+        x[0] = Exp2(fmaf(x[0], cs[0], o0));
+        x[1] = Exp2(fmaf(x[1], cs[1], o1));
+        x[2] = Exp2(fmaf(x[2], cs[0], o0));
+        x[3] = Exp2(fmaf(x[3], cs[1], o1));
+        l[0] += x[0] + x[2];
+        l[1] += x[1] + x[3];
+    }
+};
+
+// O^T fragments of one tile: [block][row tile][C fragment].
+template <int NB>
+struct Values {
+    float o[NB][2][4];
+
+    __device__ __forceinline__ void Clear() {
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) o[b][i >> 2][i & 3] = 0.0f;
+    }
+    __device__ __forceinline__ void Scale(float r0, float r1) {
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                o[b][j][0] *= r0;
+                o[b][j][1] *= r1;
+                o[b][j][2] *= r0;
+                o[b][j][3] *= r1;
+            }
+    }
+};
+
+// 16 bytes to shared memory, `bytes` (16 or 0) of them read and the rest zeros.
+__device__ __forceinline__ void CopyChunk(uint32_t to, const void* from, int bytes = 16) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
+}
+
+// ---------------------------------------------------------------- quantized caches
+// A warp's running result for NT tiles of rows over Q8_0 / Q4_0 slots.
+template <int TYPE, int NB, int NT>
+struct QuantWarp {
+    static constexpr int kQuantBytes = TYPE == MLB_Q8_0 ? 32 : 16;
+    static constexpr int kChunks = NB * kQuantBytes / 16;  // of a row
+    static constexpr int kPitch = (kChunks | 1) * 16;      // of a row in the ring
+    static constexpr int kPlane = kUnit * kPitch, kScales = kUnit * NB * 2;
+    static constexpr int kStageBytes = 2 * kPlane + 2 * kScales;
+    static constexpr int kFrags = 2 * NB;                  // uint4 per lane and tile: (hi, hi, lo, lo)
+
+    Values<NB> v[NT];
+    Columns col[NT];
+    int e[NT];         // of row g: P' is relative to 2^e
+    float bound[NT];   // 2^e
+    __half2 down[NT];  // 2^-e
+    uint32_t magic;
+    const uint8_t *kp, *vp;  // the head's planes
+    const __half *ksp, *vsp;
+
+    // Output element of a block in o[.][j][0..1] (half 0: row g of the fragment)
+    // or o[.][j][2..3] (half 1: row g + 8).
+    __device__ __forceinline__ static int Dim(int g, int j, int half) {
+        return TYPE == MLB_Q8_0 ? 4 * g + 2 * j + half : 16 * j + 2 * g + half;
+    }
+
+    // Q fragments of one tile (rows q of row g; null: none) and its score factors.
+    __device__ __forceinline__ static void LayOut(const TreeArgs& a, const Step& s, const float* q, uint4* frags,
+                                                  float* undos) {
+        // the thread's elements of its row g in the order of the K fragments: 4c .. 4c + 3 and 16 further
+        float x[NB][8], top = 0.0f;
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                const int d = b * 32 + 16 * half + 4 * s.c;
+                if (a.q_vec) {
+                    const float4 w = q && d < a.c.hd ? __ldg(reinterpret_cast<const float4*>(q + d))
+                                                     : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                    x[b][4 * half] = w.x;
+                    x[b][4 * half + 1] = w.y;
+                    x[b][4 * half + 2] = w.z;
+                    x[b][4 * half + 3] = w.w;
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) x[b][4 * half + i] = q && d + i < a.c.hd ? __ldg(q + d + i) : 0.0f;
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(x[b][i]));
+        }
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        const int up = ScaleExp(top);  // largest |q| into [2^14, 2^15)
+        const float sc = Pow2(up), undo = fmaxf(Pow2(-up) * a.scale * kLog2e, 1e-37f);
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const float* y = &x[b][4 * i];
+                // bytes 0 and 2, then 1 and 3 of a word
+                uint4 f;
+                SplitHalf(y[0] * sc, y[2] * sc, f.x, f.z);
+                SplitHalf(y[1] * sc, y[3] * sc, f.y, f.w);
+                frags[(2 * b + i) * 32 + s.lane] = f;
+            }
+        if (s.c == 0) undos[s.g] = undo;
+    }
+
+    __device__ __forceinline__ void SetPower(int n, int to) {
+        e[n] = to;
+        bound[n] = Pow2(to);
+        down[n] = __float2half2_rn(Pow2(-to));
+    }
+
+    __device__ __forceinline__ void Begin(const TreeArgs& a, const TreeSplit& sp, int seq, int head) {
+        magic = sp.magic;
+        const long long row = a.c.Row(seq, a.layer, head, 0);
+        kp = static_cast<const uint8_t*>(a.c.k) + row * NB * kQuantBytes;
+        vp = static_cast<const uint8_t*>(a.c.v) + row * NB * kQuantBytes;
+        ksp = a.c.ks + row * NB;
+        vsp = a.c.vs + row * NB;
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            v[n].Clear();
+            SetPower(n, -15);
+        }
+    }
+
+    // The unit at p0 into a ring stage, by the `count` threads of a group.
+    template <int COUNT>
+    __device__ __forceinline__ void Copy(uint32_t stage, int p0, int id) const {
+        const uint8_t* k = kp + size_t(p0) * (NB * kQuantBytes);
+        const uint8_t* w = vp + size_t(p0) * (NB * kQuantBytes);
+        constexpr int kAll = kUnit * kChunks;
+#pragma unroll
+        for (int j = 0; j < (kAll + COUNT - 1) / COUNT; ++j) {
+            const int i = id + j * COUNT;
+            if (kAll % COUNT != 0 && i >= kAll) break;
+            const uint32_t to = stage + i / kChunks * kPitch + i % kChunks * 16;
+            CopyChunk(to, k + i * 16);
+            CopyChunk(to + kPlane, w + i * 16);
+        }
+        constexpr int kSc = kScales / 16;  // 2 NB chunks of each
+        if (id < 2 * kSc) {
+            const __half* from = id < kSc ? ksp + size_t(p0) * NB + id * 8 : vsp + size_t(p0) * NB + (id - kSc) * 8;
+            CopyChunk(stage + 2 * kPlane + id * 16, from);
+        }
+    }
+
+    // The staged unit at p0; slots below `low` are another unit's.
+    __device__ __forceinline__ void Unit(const Step& s, const uint8_t* stage, const uint4* frags, int p0, int low) {
+        float x[NT][4];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) x[n][0] = x[n][1] = x[n][2] = x[n][3] = 0.0f;
+        {
+            const __half* sc = reinterpret_cast<const __half*>(stage + 2 * kPlane) + s.g * NB;
+            uint32_t kd[2][(NB + 1) / 2];
+            LoadScales<NB>(sc, kd[0]);
+            LoadScales<NB>(sc + 8 * NB, kd[1]);
+            const uint8_t* row = stage + s.g * kPitch + 4 * s.c;
+#pragma unroll
+            for (int b = 0; b < NB; ++b) {
+                uint32_t f[2][4];
+#pragma unroll
+                for (int r = 0; r < 2; ++r) {
+                    if constexpr (TYPE == MLB_Q8_0) {
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) {
+                            const uint32_t w = *reinterpret_cast<const uint32_t*>(row + 8 * r * kPitch + b * 32 + 16 * i);
+                            f[i][r] = EvenBytes(w, magic);
+                            f[i][2 + r] = EvenBytes(w >> 8, magic);
+                        }
+                    } else {
+                        const uint32_t w = *reinterpret_cast<const uint32_t*>(row + 8 * r * kPitch + b * 16), u = w >> 8;
+                        f[0][r] = LowNibbles(w, magic);
+                        f[0][2 + r] = LowNibbles(u, magic);
+                        f[1][r] = HighNibbles(w, magic);
+                        f[1][2 + r] = HighNibbles(u, magic);
+                    }
+                }
+                const float d0 = ScaleOf(kd[0], b), d1 = ScaleOf(kd[1], b);
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    const uint4 q0 = frags[(n * kFrags + 2 * b) * 32], q1 = frags[(n * kFrags + 2 * b + 1) * 32];
+                    float d[4];
+                    MmaFirst(d, f[0], q0.z, q0.w);
+                    Mma(d, f[1], q1.z, q1.w);
+                    Mma(d, f[0], q0.x, q0.y);
+                    Mma(d, f[1], q1.x, q1.y);
+                    x[n][0] = fmaf(d0, d[0], x[n][0]);
+                    x[n][1] = fmaf(d0, d[1], x[n][1]);
+                    x[n][2] = fmaf(d1, d[2], x[n][2]);
+                    x[n][3] = fmaf(d1, d[3], x[n][3]);
+                }
+            }
+        }
+        // weights as B fragments: row (query) g, slots 2c, 2c + 1 (+ 8)
+        uint32_t ph[NT][2], pl[NT][2];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            col[n].Weights(s, p0, low, x[n], kOffset, [&](float r0, float r1) { v[n].Scale(r0, r1); });
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                SplitHalf(x[n][2 * i], x[n][2 * i + 1], ph[n][i], pl[n][i]);
+                ph[n][i] = Transpose8x8(ph[n][i]);
+                pl[n][i] = Transpose8x8(pl[n][i]);
+            }
+        }
+        uint32_t d[2][NB];  // the scales of slots 2c, 2c + 1 (+ 8) as half pairs
+        {
+            const __half* sc = reinterpret_cast<const __half*>(stage + 2 * kPlane + kScales) + 2 * s.c * NB;
+            uint32_t vd[4][(NB + 1) / 2];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) LoadScales<NB>(sc + ((i & 1) + (i >> 1) * 8) * NB, vd[i]);
+#pragma unroll
+            for (int b = 0; b < NB; ++b)
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+                    d[i][b] = __byte_perm(vd[2 * i][b >> 1], vd[2 * i + 1][b >> 1], b & 1 ? 0x7632 : 0x5410);
+        }
+        const bool edge = low + kUnit > s.len;
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            float top;
+            {
+                uint32_t see[2] = {0xffffffffu, 0xffffffffu};
+                if (edge)  // a slot that is not seen may hold any scale, NaN too
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) see[i] = __hne2_mask(AsHalf2(ph[n][i]), AsHalf2(0u));
+                __half2 big = AsHalf2(0u);
+                if (edge) {
+#pragma unroll
+                    for (int b = 0; b < NB; ++b)
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) big = __hmax2(big, AsHalf2(d[i][b] & see[i]));
+                } else {
+#pragma unroll
+                    for (int b = 0; b < NB; ++b)
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) big = __hmax2(big, AsHalf2(d[i][b]));
+                }
+                top = fmaxf(__low2float(big), __high2float(big));
+            }
+            if (__any_sync(0xffffffffu, top > bound[n])) {
+                float t = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 2));
+                // 2^to > t, `to` within the powers that a half can scale by
+                const int to = max(e[n], min(15, max(-15, static_cast<int>(__float_as_uint(t) >> 23) - 126)));
+                const float f = Pow2(e[n] - to);
+                SetPower(n, to);
+                v[n].Scale(__shfl_sync(0xffffffffu, f, 8 * s.c), __shfl_sync(0xffffffffu, f, 8 * s.c + 4));
+            }
+        }
+        const uint8_t* row = stage + kPlane + 2 * s.c * kPitch + (kQuantBytes / 8) * s.g;
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+            uint32_t f[2][4];
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {  // slots 2c, 2c + 1, then + 8
+                const uint8_t* at = row + 8 * r * kPitch + b * kQuantBytes;
+                if constexpr (TYPE == MLB_Q8_0) {
+                    const uint32_t w0 = *reinterpret_cast<const uint32_t*>(at);
+                    const uint32_t w1 = *reinterpret_cast<const uint32_t*>(at + kPitch);
+                    // bytes of the two slots side by side
+                    const uint32_t low2 = __byte_perm(w0, w1, 0x5410), high2 = __byte_perm(w0, w1, 0x7632);
+                    f[0][2 * r] = EvenBytes(low2, magic);
+                    f[0][2 * r + 1] = EvenBytes(low2 >> 8, magic);
+                    f[1][2 * r] = EvenBytes(high2, magic);
+                    f[1][2 * r + 1] = EvenBytes(high2 >> 8, magic);
+                } else {
+                    const uint32_t w = *reinterpret_cast<const unsigned short*>(at) |
+                                       (uint32_t(*reinterpret_cast<const unsigned short*>(at + kPitch)) << 16);
+                    const uint32_t u = w >> 8;
+                    f[0][2 * r] = LowNibbles(w, magic);
+                    f[0][2 * r + 1] = LowNibbles(u, magic);
+                    f[1][2 * r] = HighNibbles(w, magic);
+                    f[1][2 * r + 1] = HighNibbles(u, magic);
+                }
+            }
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                uint32_t h[2], l[2];
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    uint32_t di = d[i][b];
+                    if (edge) di &= __hne2_mask(AsHalf2(ph[n][i]), AsHalf2(0u));
+                    const __half2 sc = __hmul2(AsHalf2(di), down[n]);
+                    const __half2 p = AsHalf2(ph[n][i]), t = __hmul2(p, sc);
+                    h[i] = H2(t);
+                    l[i] = H2(__hfma2(AsHalf2(pl[n][i]), sc, __hfma2(p, sc, __hneg2(t))));
+                }
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    float t[4];
+                    MmaFirst(t, f[j], l[0], l[1]);
+                    Mma(t, f[j], h[0], h[1]);
+                    AddTo(v[n].o[b][j], t);
+                }
+            }
+        }
+    }
+
+    __device__ __forceinline__ void End(const Step& s) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            const float f = Pow2(e[n]);
+            v[n].Scale(__shfl_sync(0xffffffffu, f, 8 * s.c), __shfl_sync(0xffffffffu, f, 8 * s.c + 4));
+        }
+    }
+};
+
+// ---------------------------------------------------------------- fp32 caches
+template <int NB, int NT>
+struct F32Warp {
+    static constexpr int kChunks = NB * 8;
+    static constexpr int kPitch = (kChunks | 1) * 16;
+    static constexpr int kPlane = kUnit * kPitch;
+    static constexpr int kStageBytes = 2 * kPlane;
+    static constexpr int kFrags = 4 * NB;
+
+    Values<NB> v[NT];
+    Columns col[NT];
+    const float *kp, *vp;
+    int pitch;  // floats between slots
+    int hd;
+
+    __device__ __forceinline__ static int Dim(int g, int j, int half) { return 4 * g + 2 * j + half; }
+
+    __device__ __forceinline__ static void LayOut(const TreeArgs& a, const Step& s, const float* q, uint4* frags,
+                                                  float* undos) {
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {  // elements 2i, 2i + 1 of the thread's eight: k = c, c + 4
+                const int d = b * 32 + 8 * s.c + 2 * i;
+                uint4 f;
+                SplitTf32(q && d < a.c.hd ? __ldg(q + d) : 0.0f, f.x, f.z);
+                SplitTf32(q && d + 1 < a.c.hd ? __ldg(q + d + 1) : 0.0f, f.y, f.w);
+                frags[(4 * b + i) * 32 + s.lane] = f;
+            }
+        if (s.c == 0) undos[s.g] = fmaxf(a.scale * kLog2e, 1e-37f);
+    }
+
+    __device__ __forceinline__ void Begin(const TreeArgs& a, const TreeSplit&, int seq, int head) {
+        const long long row = a.c.Row(seq, a.layer, head, 0);
+        hd = a.c.hd;
+        kp = static_cast<const float*>(a.c.k) + row * hd;
+        vp = static_cast<const float*>(a.c.v) + row * hd;
+        pitch = a.c.n_kv * hd;
+#pragma unroll
+        for (int n = 0; n < NT; ++n) v[n].Clear();
+    }
+
+    template <int COUNT>
+    __device__ __forceinline__ void Copy(uint32_t stage, int p0, int id) const {
+        constexpr int kAll = kUnit * kChunks;
+        for (int j = 0; j < (kAll + COUNT - 1) / COUNT; ++j) {
+            const int i = id + j * COUNT;
+            if (kAll % COUNT != 0 && i >= kAll) break;
+            const int r = i / kChunks, d = i % kChunks * 4, bytes = d < hd ? 16 : 0;
+            const size_t at = size_t(p0 + r) * pitch + (d < hd ? d : 0);
+            const uint32_t to = stage + r * kPitch + d * 4;
+            CopyChunk(to, kp + at, bytes);
+            CopyChunk(to + kPlane, vp + at, bytes);
+        }
+    }
+
+    __device__ __forceinline__ void Unit(const Step& s, const uint8_t* stage, const uint4* frags, int p0, int low) {
+        float x[NT][4], rest[NT][4];
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[n][i] = rest[n][i] = 0.0f;
+        const float* row = reinterpret_cast<const float*>(stage + s.g * kPitch) + 8 * s.c;
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const float4 ra = *reinterpret_cast<const float4*>(row + b * 32 + 4 * h);
+                const float4 rb = *reinterpret_cast<const float4*>(row + 8 * (kPitch / 4) + b * 32 + 4 * h);
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    uint32_t hi[4], lo[4];
+                    SplitTf32(i ? ra.z : ra.x, hi[0], lo[0]);
+                    SplitTf32(i ? rb.z : rb.x, hi[1], lo[1]);
+                    SplitTf32(i ? ra.w : ra.y, hi[2], lo[2]);
+                    SplitTf32(i ? rb.w : rb.y, hi[3], lo[3]);
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) {
+                        const uint4 q = frags[(n * kFrags + 4 * b + 2 * h + i) * 32];
+                        MmaTf32(rest[n], lo, q.x, q.y);
+                        MmaTf32(rest[n], hi, q.z, q.w);
+                        MmaTf32(x[n], hi, q.x, q.y);
+                    }
+                }
+            }
+        // weights as B fragments: query g, slots 2c and 2c + 1 (+ 8)
+        uint32_t ph[NT][4], pl[NT][4];
+        bool odd = false;
+        const float* vrow = reinterpret_cast<const float*>(stage + kPlane + 2 * s.c * kPitch) + 4 * s.g;
+        const bool edge = low + kUnit > s.len;
+        if (edge) {  // a slot that some rows do not see may hold NaN or infinities
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int b = 0; b < NB; ++b) {
+                    const float4 y = *reinterpret_cast<const float4*>(vrow + ((i & 1) + (i >> 1) * 8) * (kPitch / 4) + b * 32);
+                    odd = odd || !(fabsf(y.x) <= 3.4e38f && fabsf(y.y) <= 3.4e38f && fabsf(y.z) <= 3.4e38f &&
+                                   fabsf(y.w) <= 3.4e38f);
+                }
+            odd = __any_sync(0xffffffffu, odd);
+        }
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            AddTo(x[n], rest[n]);
+            col[n].Weights(s, p0, low, x[n], 0.0f, [&](float r0, float r1) { v[n].Scale(r0, r1); });
+            if (odd) {
+                Plainly(s, stage, n, x[n]);
+                continue;
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int src = 4 * (2 * s.c + (i & 1)) + (s.g >> 1);
+                const float even = __shfl_sync(0xffffffffu, x[n][i & 2], src);
+                const float other = __shfl_sync(0xffffffffu, x[n][(i & 2) + 1], src);
+                SplitTf32(s.g & 1 ? other : even, ph[n][i], pl[n][i]);
+            }
+        }
+        if (odd) return;
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+            float4 y[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                y[i] = *reinterpret_cast<const float4*>(vrow + ((i & 1) + (i >> 1) * 8) * (kPitch / 4) + b * 32);
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                float t[NT][4];
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const float4 va = y[2 * i], vb = y[2 * i + 1];
+                    uint32_t hi[4], lo[4];
+                    SplitTf32(j ? va.z : va.x, hi[0], lo[0]);
+                    SplitTf32(j ? va.w : va.y, hi[1], lo[1]);
+                    SplitTf32(j ? vb.z : vb.x, hi[2], lo[2]);
+                    SplitTf32(j ? vb.w : vb.y, hi[3], lo[3]);
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) {
+                        i == 0 ? MmaTf32First(t[n], lo, ph[n][0], ph[n][1]) : MmaTf32(t[n], lo, ph[n][2], ph[n][3]);
+                        MmaTf32(t[n], hi, pl[n][2 * i], pl[n][2 * i + 1]);
+                        MmaTf32(t[n], hi, ph[n][2 * i], ph[n][2 * i + 1]);
+                    }
+                }
+#pragma unroll
+                for (int n = 0; n < NT; ++n) AddTo(v[n].o[b][j], t[n]);
+            }
+        }
+    }
+
+    // The weighted values of one unit slot by slot, those of weight 0 left out.
+    __device__ __forceinline__ void Plainly(const Step& s, const uint8_t* stage, int n, const float (&x)[4]) {
+        const float* row = reinterpret_cast<const float*>(stage + kPlane) + 4 * s.g;
+        for (int i = 0; i < kUnit; ++i) {
+            const int src = 4 * (i & 7) + s.c;
+            const float w0 = __shfl_sync(0xffffffffu, i < 8 ? x[0] : x[2], src);
+            const float w1 = __shfl_sync(0xffffffffu, i < 8 ? x[1] : x[3], src);
+#pragma unroll
+            for (int b = 0; b < NB; ++b) {
+                const float4 y = *reinterpret_cast<const float4*>(row + i * (kPitch / 4) + b * 32);
+                const float e[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+                for (int d = 0; d < 4; ++d) {
+                    float* to = &v[n].o[b][d >> 1][(d & 1) * 2];
+                    if (w0 != 0.0f) to[0] = fmaf(w0, e[d], to[0]);
+                    if (w1 != 0.0f) to[1] = fmaf(w1, e[d], to[1]);
+                }
+            }
+        }
+    }
+
+    __device__ __forceinline__ void End(const Step&) {}
+};
+
+template <int TYPE, int NB, int NT>
+struct WarpOf {
+    using T = QuantWarp<TYPE, NB, NT>;
+};
+template <int NB, int NT>
+struct WarpOf<MLB_F32, NB, NT> {
+    using T = F32Warp<NB, NT>;
+};
+
+__device__ __forceinline__ unsigned WarpSum32(unsigned v) { return __reduce_add_sync(0xffffffffu, v); }
+
+__device__ __forceinline__ unsigned EntryUnits(const TreeArgs& a, int b, unsigned items) {
+    return unsigned((FindEntry(a, b).slots + kUnit - 1) / kUnit) * items;
+}
+
+// Four consecutive elements of an output row.
+__device__ __forceinline__ void StoreOut(const TreeArgs& a, float* row, int d, const float4& v) {
+    if (a.out_vec) {
+        if (d < a.c.hd) *reinterpret_cast<float4*>(row + d) = v;
+        return;
+    }
+    const float e[4] = {v.x, v.y, v.z, v.w};
+    for (int i = 0; i < 4; ++i)
+        if (d + i < a.c.hd) row[d + i] = e[i];
+}
+
+__device__ __forceinline__ float* OutRow(const TreeArgs& a, int b, int head, int r) {
+    return a.out + (size_t(b) * a.tokens + r / a.group) * a.out_stride + size_t(head * a.group + r % a.group) * a.c.hd;
+}
+
+// Sum of partial results: o 2^(m - M) over parts, M their largest maximum.
+struct Joined {
+    float m = kStart, l = 0.0f;
+    float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+
+    __device__ __forceinline__ void Add(float pm, float pl, const float4& po) {
+        const float n = fmaxf(m, pm), a = Exp2(m - n), b = Exp2(pm - n);
+        m = n;
+        l = l * a + pl * b;
+        o.x = o.x * a + po.x * b;
+        o.y = o.y * a + po.y * b;
+        o.z = o.z * a + po.z * b;
+        o.w = o.w * a + po.w * b;
+    }
+    __device__ __forceinline__ float4 Result() const {
+        const float r = l == 0.0f ? 0.0f : 1.0f / l;
+        return make_float4(o.x * r, o.y * r, o.z * r, o.w * r);
+    }
+};
+
+// Even cuts of `total` units over `ctas` CTAs: the first `extra` take one more.
+struct Cut {
+    unsigned each, extra;
+
+    __device__ __forceinline__ Cut(unsigned total, unsigned ctas) : each(total / ctas), extra(total - each * ctas) {}
+    __device__ __forceinline__ unsigned Start(unsigned cta) const { return cta * each + min(cta, extra); }
+    __device__ __forceinline__ unsigned Owner(unsigned unit) const {
+        const unsigned high = extra * (each + 1);
+        return unit < high ? unit / (each + 1) : extra + (unit - high) / each;
+    }
+};
+
+// Shared memory: the ring, which the joining of the groups reuses, the Q
+// fragments and the score factors.
+template <int TYPE, int NB, int NT, int WQ, int NW>
+struct TreeShape {
+    using Warp = typename WarpOf<TYPE, NB, NT>::T;
+    static constexpr int kGroups = NW / WQ;
+    static constexpr int kRowsOf = kRows * NT;        // of a warp
+    static constexpr int kItemRows = kRowsOf * WQ;
+    static constexpr int kPitch = NB * 32 + 4;        // of a row in the join
+    static constexpr int kFragBytes = WQ * NT * Warp::kFrags * 32 * 16;
+    static constexpr int kJoinBytes = NW * kRowsOf * (kPitch + 2) * 4;
+    static constexpr int kUndoBytes = WQ * kRowsOf * 4;
+    static constexpr int kFit = (kMaxShared - kFragBytes - kUndoBytes) / (kGroups * Warp::kStageBytes);
+    static constexpr int kStages = kFit < kMaxStages ? kFit : kMaxStages;
+    static constexpr int kRingBytes = kGroups * kStages * Warp::kStageBytes;
+    static constexpr int kTop = (kRingBytes > kJoinBytes ? kRingBytes : kJoinBytes);
+    static constexpr int kBytes = (kTop + 15) / 16 * 16 + kFragBytes + kUndoBytes;
+    static_assert(kStages >= 2, "a ring has two stages at least");
+    static_assert(kBytes <= kMaxShared + 1024, "shared memory");
+    static_assert(kGroups <= 15, "a named barrier per group");
+};
+
+template <int TYPE, int NB, int NT, int WQ, int NW>
+__global__ void __launch_bounds__(NW * 32, 1) TreeMmaKernel(TreeArgs a, TreeSplit sp) {
+    using Shape = TreeShape<TYPE, NB, NT, WQ, NW>;
+    using Warp = typename Shape::Warp;
+    constexpr int kPitch = Shape::kPitch, kFours = NB * 8, kItemRows = Shape::kItemRows, kStages = Shape::kStages;
+    constexpr unsigned kGroups = Shape::kGroups;
+    extern __shared__ uint4 smem4[];
+    uint8_t* ring = reinterpret_cast<uint8_t*>(smem4);
+    float* so = reinterpret_cast<float*>(smem4);                 // join: [NW][8 NT][kPitch]
+    float* sm = so + NW * Shape::kRowsOf * kPitch;               // [NW][8 NT]
+    float* sl = sm + NW * Shape::kRowsOf;
+    uint4* sq = reinterpret_cast<uint4*>(ring + (Shape::kTop + 15) / 16 * 16);  // [WQ NT][kFrags][32]
+    float* su = reinterpret_cast<float*>(sq + Shape::kFragBytes / 16);          // [WQ NT][8]
+    __shared__ int s_last;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int wq = warp % WQ, group = warp / WQ;
+    const unsigned items = a.c.n_kv * sp.groups;
+
+    // entries with nothing to see
+    for (int b = blockIdx.x; b < a.batch; b += gridDim.x) {
+        if (FindEntry(a, b).slots != 0) continue;
+        for (int t = warp; t < a.tokens; t += NW)
+            for (int i = lane; i < a.n_heads * a.c.hd; i += 32)
+                a.out[(size_t(b) * a.tokens + t) * a.out_stride + i] = 0.0f;
+    }
+
+    // the cut: all units in a row, an even stretch for each CTA
+    unsigned total = 0;
+    for (int b0 = 0; b0 < a.batch; b0 += 32) total += WarpSum32(b0 + lane < a.batch ? EntryUnits(a, b0 + lane, items) : 0);
+    if (total == 0) return;
+    const unsigned ctas = min((total + kGroups - 1) / kGroups, gridDim.x);  // a unit for each group at least
+    if (blockIdx.x >= ctas) return;
+    const Cut cut(total, ctas);
+    unsigned cur = cut.Start(blockIdx.x);
+    const unsigned end = cut.Start(blockIdx.x + 1);
+    // the entry of the first unit
+    int b = 0;
+    unsigned first = 0;
+    for (int b0 = 0; b0 < a.batch; b0 += 32) {
+        const unsigned n = b0 + lane < a.batch ? EntryUnits(a, b0 + lane, items) : 0;
+        const unsigned chunk = WarpSum32(n);
+        if (cur >= first + chunk) {
+            first += chunk;
+            continue;
+        }
+        unsigned incl = n;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const unsigned t = __shfl_up_sync(0xffffffffu, incl, o);
+            if (lane >= o) incl += t;
+        }
+        const int at = __ffs(__ballot_sync(0xffffffffu, first + incl > cur)) - 1;
+        first += __shfl_sync(0xffffffffu, incl - n, at);
+        b = b0 + at;
+        break;
+    }
+
+    Step s;
+    s.lane = lane;
+    s.g = lane >> 2;
+    s.c = lane & 3;
+    s.tokens = a.tokens;
+    s.words = a.words;
+    const int last_unit = a.c.head_slots - kUnit;
+    const uint32_t ring_at = SmemAddr(ring) + group * (kStages * Warp::kStageBytes);
+    const uint8_t* ring_ptr = ring + group * (kStages * Warp::kStageBytes);
+    Warp w;
+    while (cur < end) {
+        const Entry e = FindEntry(a, b);
+        const unsigned units = (e.slots + kUnit - 1) / kUnit;
+        if (cur - first >= units * items) {  // the next entry
+            first += units * items;
+            ++b;
+            continue;
+        }
+        const unsigned item = (cur - first) / units;
+        const int u0 = cur - first - item * units;
+        const int u1 = min(u0 + (end - cur), units);
+        const int head = item / sp.groups, row0 = (item - head * sp.groups) * kItemRows;
+        const int tile = row0 + wq * Shape::kRowsOf;  // the warp's first row
+        s.slots = e.slots;
+        s.len = e.len;
+        s.mask = a.mask ? a.mask + size_t(b) * a.tokens * a.words : nullptr;
+
+        // ---- the ring's first units, then the Q fragments
+        w.Begin(a, sp, e.seq, head);
+        auto copy = [&](int k) {  // unit k of the group
+            const int u = u0 + group + k * int(kGroups);
+            // the last unit of a plane may hold fewer than 16 slots: it starts earlier and leaves the others out
+            if (u < u1)
+                w.template Copy<WQ * 32>(ring_at + (k % kStages) * Warp::kStageBytes, min(u * kUnit, last_unit),
+                                         wq * 32 + lane);
+            asm volatile("cp.async.commit_group;" ::: "memory");
+        };
+#pragma unroll
+        for (int k = 0; k < kStages - 1; ++k) copy(k);
+        for (int n = warp; n < WQ * NT; n += NW) {
+            const int r = row0 + n * kRows + s.g;
+            const float* q = r < sp.rows ? a.q + (size_t(b) * a.tokens + r / a.group) * a.q_stride +
+                                               size_t(head * a.group + r % a.group) * a.c.hd
+                                         : nullptr;
+            Warp::LayOut(a, s, q, sq + n * Warp::kFrags * 32, su + n * kRows);
+        }
+        __syncthreads();
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            const int r = tile + n * kRows + 2 * s.c;
+            const float* undo = su + (wq * NT + n) * kRows + 2 * s.c;
+            w.col[n].Begin(r / a.group, (r + 1) / a.group);
+            w.col[n].cs[0] = undo[0];
+            w.col[n].cs[1] = undo[1];
+        }
+
+        // ---- the group's units
+        const uint4* frags = sq + wq * NT * Warp::kFrags * 32 + lane;
+        int k = 0;
+        for (int u = u0 + group; u < u1; u += kGroups, ++k) {
+            asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
+            // every copy of this unit has landed, and the stage refilled next has been read
+            if (WQ == 1)
+                __syncwarp();
+            else
+                asm volatile("bar.sync %0, %1;" ::"r"(group + 1), "n"(WQ * 32) : "memory");
+            copy(k + kStages - 1);
+            if (tile < sp.rows)
+                w.Unit(s, ring_ptr + (k % kStages) * Warp::kStageBytes, frags, min(u * kUnit, last_unit), u * kUnit);
+        }
+        w.End(s);
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
+        __syncthreads();  // the ring is free for the join
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            Columns& col = w.col[n];
+#pragma unroll
+            for (int o = 4; o < 32; o <<= 1) {
+                col.l[0] += __shfl_xor_sync(0xffffffffu, col.l[0], o);
+                col.l[1] += __shfl_xor_sync(0xffffffffu, col.l[1], o);
+            }
+            const int at = warp * Shape::kRowsOf + n * kRows + 2 * s.c;
+            float* to = so + at * kPitch;
+#pragma unroll
+            for (int i = 0; i < NB; ++i)
+#pragma unroll
+                for (int j = 0; j < 2; ++j)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const int d = i * 32 + w.Dim(s.g, j, h);
+                        to[d] = w.v[n].o[i][j][2 * h];
+                        to[kPitch + d] = w.v[n].o[i][j][2 * h + 1];
+                    }
+            if (s.g == 0) {
+                sm[at] = col.m[0];
+                sm[at + 1] = col.m[1];
+                sl[at] = col.l[0];
+                sl[at + 1] = col.l[1];
+            }
+        }
+        __syncthreads();
+
+        // ---- join the groups
+        const bool whole = u0 == 0 && u1 == int(units);
+        constexpr size_t kPart = size_t(kItemRows) * (NB * 32 + 2);
+        float* part = sp.parts + (2 * size_t(blockIdx.x) + (u0 == 0 ? 1 : 0)) * kPart;
+        const int live_rows = min(kItemRows, sp.rows - row0);
+        for (int i = threadIdx.x; i < live_rows * kFours; i += NW * 32) {
+            const int r = i / kFours, d = (i - r * kFours) * 4;
+            Joined x;
+#pragma unroll 4
+            for (unsigned j = 0; j < kGroups; ++j) {
+                const int at = j * kItemRows + r;  // warp j WQ + its wq
+                x.Add(sm[at], sl[at], *reinterpret_cast<const float4*>(so + at * kPitch + d));
+            }
+            if (whole) {
+                StoreOut(a, OutRow(a, b, head, row0 + r), d, x.Result());
+            } else {
+                __stcg(reinterpret_cast<float4*>(part + r * NB * 32 + d), x.o);
+                if (d == 0) {
+                    __stcg(part + kItemRows * NB * 32 + r, x.m);
+                    __stcg(part + kItemRows * (NB * 32 + 1) + r, x.l);
+                }
+            }
+        }
+
+        // ---- join the CTAs that share the item: the last to arrive adds them up
+        if (!whole) {
+            const unsigned c0 = cut.Owner(cur - u0), c1 = cut.Owner(cur - u0 + units - 1);  // of its first and last unit
+            __threadfence();
+            __syncthreads();
+            if (threadIdx.x == 0) {
+                int* counter = sp.counters + size_t(b) * items + item;
+                s_last = atomicAdd(counter, 1) == int(c1 - c0);
+                if (s_last) *counter = 0;  // every contributor has arrived
+            }
+            __syncthreads();
+            if (s_last) {
+                __threadfence();
+                // a CTA has two parts: of an item that it begins, and of one that it goes on with
+                for (int i = threadIdx.x; i < live_rows * kFours; i += NW * 32) {
+                    const int r = i / kFours, d = (i - r * kFours) * 4;
+                    Joined x;
+                    for (unsigned k0 = c0; k0 <= c1; k0 += 4) {
+                        float pm[4], pl[4];
+                        float4 po[4];
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            if (k0 + j > c1) break;
+                            const float* p = sp.parts + (2 * size_t(k0 + j) + (cut.Start(k0 + j) <= cur - u0 ? 1 : 0)) * kPart;
+                            pm[j] = __ldcg(p + kItemRows * NB * 32 + r);
+                            pl[j] = __ldcg(p + kItemRows * (NB * 32 + 1) + r);
+                            po[j] = __ldcg(reinterpret_cast<const float4*>(p + r * NB * 32 + d));
+                        }
+#pragma unroll
+                        for (int j = 0; j < 4; ++j)
+                            if (k0 + j <= c1) x.Add(pm[j], pl[j], po[j]);
+                    }
+                    StoreOut(a, OutRow(a, b, head, row0 + r), d, x.Result());
+                }
+            }
+        }
+        __syncthreads();
+        cur += u1 - u0;
+    }
+}
+
+template <int TYPE, int NB, int NT, int WQ, int NW>
+bool LaunchShape(DeviceContext& ctx, const TreeArgs& a) {
+    using Shape = TreeShape<TYPE, NB, NT, WQ, NW>;
+    TreeSplit sp{};
+    sp.rows = a.tokens * a.group;
+    sp.groups = static_cast<int>(CeilDiv(sp.rows, Shape::kItemRows));
+    const unsigned long long items = 1ull * a.c.n_kv * sp.groups;
+    // an upper bound of the units, from the caller's bound of the lengths
+    const long long slots = std::min<long long>(1LL * std::min(a.max_len, a.c.max_seq) + a.tokens, a.c.max_seq);
+    const double units = double(a.batch) * double(items) * double(CeilDiv(slots, kUnit));
+    if (units >= 2147483648.0) return false;
+    const int grid = static_cast<int>(
+        std::max(1.0, std::min<double>(ctx.sm_count, std::ceil(units / Shape::kGroups))));
+    sp.parts = static_cast<float*>(
+        Workspace(ctx, 2 * size_t(grid) * Shape::kItemRows * (NB * 32 + 2) * sizeof(float)));
+    sp.counters = TreeCounters(ctx, size_t(a.batch) * items);
+    sp.magic = TYPE == MLB_Q8_0 ? kMagic8 : kMagic4;
+    auto* kernel = TreeMmaKernel<TYPE, NB, NT, WQ, NW>;
+    static int configured[64] = {};
+    if (ctx.device >= 64 || !configured[ctx.device]) {
+        CheckCuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape::kBytes),
+                  "cudaFuncSetAttribute(TreeMmaKernel)");
+        if (ctx.device < 64) configured[ctx.device] = 1;
+    }
+    kernel<<<grid, NW * 32, Shape::kBytes, ctx.stream>>>(a, sp);
+    CheckCuda(cudaGetLastError(), "TreeMmaKernel");
+    return true;
+}
+
+// Rows per KV head choose the tiles: up to 8 one tile per warp; more take two
+// per warp (the quants are converted once for both), up to four warps sharing
+// their slots.
+template <int TYPE, int NB>
+bool LaunchRows(DeviceContext& ctx, const TreeArgs& a) {
+    const long long rows = 1LL * a.tokens * a.group;
+    if (rows <= kRows) return LaunchShape<TYPE, NB, 1, 1, kWarps1<TYPE, NB>>(ctx, a);
+    if (rows <= 2 * kRows) return LaunchShape<TYPE, NB, 2, 1, kWarps2<TYPE, NB>>(ctx, a);
+    if (rows <= 4 * kRows) return LaunchShape<TYPE, NB, 2, 2, kWarps2<TYPE, NB>>(ctx, a);
+    return LaunchShape<TYPE, NB, 2, 4, kWarps4<TYPE, NB>>(ctx, a);
+}
+
+template <int TYPE>
+bool LaunchBlocks(DeviceContext& ctx, const TreeArgs& a) {
+    switch (a.c.blocks) {
+        case 1: return LaunchRows<TYPE, 1>(ctx, a);
+        case 2: return LaunchRows<TYPE, 2>(ctx, a);
+        case 3: return LaunchRows<TYPE, 3>(ctx, a);
+        case 4: return LaunchRows<TYPE, 4>(ctx, a);
+        default: return false;
+    }
+}
+
+}  // namespace
+}  // namespace mlb
