@@ -76,9 +76,6 @@ struct DeviceContext {
     const void* tc_x = nullptr;
     const void* tc_ws = nullptr;
     int tc_m = 0, tc_k = 0, tc_mx = 0, tc_mtiles = 0;
-    // arrival counters of the drafted-token attention, zero between launches
-    int* tree_counters = nullptr;
-    size_t tree_counter_count = 0;
 };
 
 DeviceContext& Ctx(int device);                     // creates on first use, makes device current

@@ -1,7 +1,6 @@
 // Attention of drafted tokens over the KV cache (mlb_attention_tree): `tokens`
 // queries of each sequence against its cached slots, the drafted slots by a bit
 // mask, over fp32, Q8_0 and Q4_0 caches.
-#include <algorithm>
 #include <cmath>
 
 #include "tree_attention.cuh"
@@ -84,28 +83,13 @@ __global__ void __launch_bounds__(kRowWarps * 32) TreeRowKernel(TreeArgs a) {
 }
 
 // Head sizes up to 128 (fp32 caches: rows that allow 16-byte copies) and planes
-// of 16 slots or more.
+// of a unit or more.
 bool LaunchTreeMma(DeviceContext& ctx, const TreeArgs& a) {
-    if (a.c.head_slots < 16) return false;
     if (a.c.type == MLB_F32) return a.cache_vec && LaunchTreeF32(ctx, a);
     return a.c.type == MLB_Q8_0 ? LaunchTreeQ80(ctx, a) : LaunchTreeQ40(ctx, a);
 }
 
 }  // namespace
-
-int* TreeCounters(DeviceContext& ctx, size_t n) {
-    if (n <= ctx.tree_counter_count) return ctx.tree_counters;
-    if (ctx.tree_counters) CheckCuda(cudaFreeAsync(ctx.tree_counters, ctx.stream), "cudaFreeAsync");
-    ctx.tree_counters = nullptr;
-    ctx.tree_counter_count = 0;
-    const size_t want = std::max<size_t>(n, 4096);
-    void* p = nullptr;
-    CheckCuda(cudaMallocFromPoolAsync(&p, want * sizeof(int), ctx.pool, ctx.stream), "cudaMallocFromPoolAsync(counters)");
-    CheckCuda(cudaMemsetAsync(p, 0, want * sizeof(int), ctx.stream), "cudaMemsetAsync(counters)");
-    ctx.tree_counters = static_cast<int*>(p);
-    ctx.tree_counter_count = want;
-    return ctx.tree_counters;
-}
 
 }  // namespace mlb
 

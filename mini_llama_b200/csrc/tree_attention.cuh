@@ -53,7 +53,4 @@ bool LaunchTreeF32(DeviceContext& ctx, const TreeArgs& a);
 bool LaunchTreeQ80(DeviceContext& ctx, const TreeArgs& a);
 bool LaunchTreeQ40(DeviceContext& ctx, const TreeArgs& a);
 
-// `n` arrival counters, zero between launches.
-int* TreeCounters(DeviceContext& ctx, size_t n);
-
 }  // namespace mlb

@@ -30,9 +30,9 @@
 // each; a group brings its units into a ring of S stages in shared memory
 // (cp.async, S - 1 units ahead; rows an odd number of 16-byte chunks apart, so
 // every fragment load is free of bank conflicts) and meets at a named barrier
-// once per unit.  The groups join their results in shared memory, and items that
-// are cut between CTAs are joined by the CTA that finishes last (partials in the
-// workspace, one counter per item, added in a fixed order).
+// once per unit.  The groups join their results in shared memory, and a second
+// kernel joins the items that are cut between CTAs (partials in the workspace,
+// added in the order of the CTAs).
 #pragma once
 
 #include <algorithm>
@@ -44,7 +44,7 @@ namespace mlb {
 
 namespace {
 
-constexpr int kUnit = 16;           // slots of a matrix step
+constexpr int kSlots = 16;          // slots of a matrix step
 constexpr int kRows = 8;            // query rows of a tile
 constexpr float kStart = -1.7e38f;  // running maximum before the first score (finite: no inf - inf)
 constexpr float kLag = 2.0f;        // how far scores may pass the running maximum, in powers of two
@@ -61,7 +61,7 @@ constexpr int kMaxStages = 4;
 #define TREE_W1 12
 #endif
 template <int TYPE, int NB>
-constexpr int kWarps1 = TYPE == MLB_F32 ? (NB > 2 ? 6 : 12) : TREE_W1;
+constexpr int kWarps1 = TYPE == MLB_F32 ? (NB > 2 ? 6 : 12) : (TYPE == MLB_Q8_0 && NB == 4 ? 11 : TREE_W1);
 template <int TYPE, int NB>
 constexpr int kWarps2 = TYPE == MLB_F32 ? (NB > 2 ? 6 : 12) : 12;
 template <int TYPE, int NB>
@@ -71,7 +71,6 @@ struct TreeSplit {
     int groups;    // items of a (sequence, KV head): ceil(R / (8 NT WQ))
     int rows;      // R
     float* parts;  // two partial results per CTA
-    int* counters; // per item
     uint32_t magic;
 };
 
@@ -194,10 +193,11 @@ struct Step {
     const uint64_t* mask;  // the batch entry's
 };
 
+// Without branches, so that the mask words of several slots load together.
 __device__ __forceinline__ bool Sees(const Step& s, int t, int slot) {
-    if (slot < s.len) return true;
-    if (slot >= s.slots || t >= s.tokens) return false;
-    return SeesDraft(s.mask ? s.mask + size_t(t) * s.words : nullptr, t, slot - s.len);
+    const int j = min(max(slot - s.len, 0), s.tokens - 1), row = min(t, s.tokens - 1);
+    const bool draft = s.mask ? (__ldg(s.mask + size_t(row) * s.words + (j >> 6)) >> (j & 63)) & 1 : j <= row;
+    return slot < s.len || (draft && slot < s.slots);
 }
 
 // One tile of rows: drafted tokens, running maxima and sums of the thread's two
@@ -213,20 +213,36 @@ struct Columns {
         l[0] = l[1] = 0.0f;
     }
 
-    // Scores (C fragment: rows slot g, g + 8; columns query 2c, 2c + 1) of the
-    // unit at p0, slots from `low` on, to weights 2^(x - m + offset); `rescale`
-    // gets the factors of a moved maximum.
-    template <typename Rescale>
-    __device__ __forceinline__ void Weights(const Step& s, int p0, int low, float (&x)[4], float offset,
+    // Scores (C fragments: rows slot g, g + 8; columns query 2c, 2c + 1) of the H
+    // steps of a unit at p0, slots from `low` on, to weights 2^(x - m + offset);
+    // `edge`: not every row sees all of it.  `rescale` gets the factors of a
+    // moved maximum.
+    template <int H, typename Rescale>
+    __device__ __forceinline__ void Weights(const Step& s, int p0, int low, bool edge, float (&x)[H][4], float offset,
                                             Rescale&& rescale) {
-        if (low + kUnit > s.len) {  // drafted slots, or the end
-            const int a = p0 + s.g, b = a + 8;
-            if (a < low || !Sees(s, t0, a)) x[0] = -INFINITY;
-            if (a < low || !Sees(s, t1, a)) x[1] = -INFINITY;
-            if (b < low || !Sees(s, t0, b)) x[2] = -INFINITY;
-            if (b < low || !Sees(s, t1, b)) x[3] = -INFINITY;
+        if (edge) {  // drafted slots, or the end
+            bool see[H][4];
+#pragma unroll
+            for (int h = 0; h < H; ++h)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int slot = p0 + h * kSlots + s.g + (i >> 1) * 8;
+                    see[h][i] = slot >= low && Sees(s, i & 1 ? t1 : t0, slot);
+                }
+#pragma unroll
+            for (int h = 0; h < H; ++h)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (!see[h][i]) x[h][i] = -INFINITY;
         }
-        float top0 = fmaxf(x[0], x[2]) * cs[0], top1 = fmaxf(x[1], x[3]) * cs[1];
+        float top0 = fmaxf(x[0][0], x[0][2]), top1 = fmaxf(x[0][1], x[0][3]);
+#pragma unroll
+        for (int h = 1; h < H; ++h) {
+            top0 = fmaxf(top0, fmaxf(x[h][0], x[h][2]));
+            top1 = fmaxf(top1, fmaxf(x[h][1], x[h][3]));
+        }
+        top0 *= cs[0];
+        top1 *= cs[1];
         if (__any_sync(0xffffffffu, top0 > m[0] + kLag || top1 > m[1] + kLag)) {
 #pragma unroll
             for (int o = 4; o < 32; o <<= 1) {
@@ -242,12 +258,15 @@ struct Columns {
             rescale(r0, r1);
         }
         const float o0 = offset - m[0], o1 = offset - m[1];
-        x[0] = Exp2(fmaf(x[0], cs[0], o0));
-        x[1] = Exp2(fmaf(x[1], cs[1], o1));
-        x[2] = Exp2(fmaf(x[2], cs[0], o0));
-        x[3] = Exp2(fmaf(x[3], cs[1], o1));
-        l[0] += x[0] + x[2];
-        l[1] += x[1] + x[3];
+#pragma unroll
+        for (int h = 0; h < H; ++h) {
+            x[h][0] = Exp2(fmaf(x[h][0], cs[0], o0));
+            x[h][1] = Exp2(fmaf(x[h][1], cs[1], o1));
+            x[h][2] = Exp2(fmaf(x[h][2], cs[0], o0));
+            x[h][3] = Exp2(fmaf(x[h][3], cs[1], o1));
+            l[0] += x[h][0] + x[h][2];
+            l[1] += x[h][1] + x[h][3];
+        }
     }
 };
 
@@ -281,9 +300,11 @@ __device__ __forceinline__ void CopyChunk(uint32_t to, const void* from, int byt
 }
 
 // ---------------------------------------------------------------- quantized caches
-// A warp's running result for NT tiles of rows over Q8_0 / Q4_0 slots.
-template <int TYPE, int NB, int NT>
+// A warp's running result for NT tiles of rows over Q8_0 / Q4_0 slots, H steps
+// of 16 slots to a unit.
+template <int TYPE, int NB, int NT, int H>
 struct QuantWarp {
+    static constexpr int kUnit = kSlots * H;
     static constexpr int kQuantBytes = TYPE == MLB_Q8_0 ? 32 : 16;
     static constexpr int kChunks = NB * kQuantBytes / 16;  // of a row
     static constexpr int kPitch = (kChunks | 1) * 16;      // of a row in the ring
@@ -392,98 +413,113 @@ struct QuantWarp {
 
     // The staged unit at p0; slots below `low` are another unit's.
     __device__ __forceinline__ void Unit(const Step& s, const uint8_t* stage, const uint4* frags, int p0, int low) {
-        float x[NT][4];
+        float x[NT][H][4];
 #pragma unroll
-        for (int n = 0; n < NT; ++n) x[n][0] = x[n][1] = x[n][2] = x[n][3] = 0.0f;
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int h = 0; h < H; ++h) x[n][h][0] = x[n][h][1] = x[n][h][2] = x[n][h][3] = 0.0f;
         {
             const __half* sc = reinterpret_cast<const __half*>(stage + 2 * kPlane) + s.g * NB;
-            uint32_t kd[2][(NB + 1) / 2];
-            LoadScales<NB>(sc, kd[0]);
-            LoadScales<NB>(sc + 8 * NB, kd[1]);
+            uint32_t kd[2 * H][(NB + 1) / 2];
+#pragma unroll
+            for (int r = 0; r < 2 * H; ++r) LoadScales<NB>(sc + 8 * r * NB, kd[r]);
             const uint8_t* row = stage + s.g * kPitch + 4 * s.c;
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
-                uint32_t f[2][4];
-#pragma unroll
-                for (int r = 0; r < 2; ++r) {
-                    if constexpr (TYPE == MLB_Q8_0) {
-#pragma unroll
-                        for (int i = 0; i < 2; ++i) {
-                            const uint32_t w = *reinterpret_cast<const uint32_t*>(row + 8 * r * kPitch + b * 32 + 16 * i);
-                            f[i][r] = EvenBytes(w, magic);
-                            f[i][2 + r] = EvenBytes(w >> 8, magic);
-                        }
-                    } else {
-                        const uint32_t w = *reinterpret_cast<const uint32_t*>(row + 8 * r * kPitch + b * 16), u = w >> 8;
-                        f[0][r] = LowNibbles(w, magic);
-                        f[0][2 + r] = LowNibbles(u, magic);
-                        f[1][r] = HighNibbles(w, magic);
-                        f[1][2 + r] = HighNibbles(u, magic);
-                    }
-                }
-                const float d0 = ScaleOf(kd[0], b), d1 = ScaleOf(kd[1], b);
+                uint4 q0[NT], q1[NT];
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
-                    const uint4 q0 = frags[(n * kFrags + 2 * b) * 32], q1 = frags[(n * kFrags + 2 * b + 1) * 32];
-                    float d[4];
-                    MmaFirst(d, f[0], q0.z, q0.w);
-                    Mma(d, f[1], q1.z, q1.w);
-                    Mma(d, f[0], q0.x, q0.y);
-                    Mma(d, f[1], q1.x, q1.y);
-                    x[n][0] = fmaf(d0, d[0], x[n][0]);
-                    x[n][1] = fmaf(d0, d[1], x[n][1]);
-                    x[n][2] = fmaf(d1, d[2], x[n][2]);
-                    x[n][3] = fmaf(d1, d[3], x[n][3]);
+                    q0[n] = frags[(n * kFrags + 2 * b) * 32];
+                    q1[n] = frags[(n * kFrags + 2 * b + 1) * 32];
+                }
+#pragma unroll
+                for (int h = 0; h < H; ++h) {
+                    uint32_t f[2][4];
+#pragma unroll
+                    for (int r = 0; r < 2; ++r) {
+                        const uint8_t* at = row + (8 * r + h * kSlots) * kPitch + b * kQuantBytes;
+                        if constexpr (TYPE == MLB_Q8_0) {
+#pragma unroll
+                            for (int i = 0; i < 2; ++i) {
+                                const uint32_t w = *reinterpret_cast<const uint32_t*>(at + 16 * i);
+                                f[i][r] = EvenBytes(w, magic);
+                                f[i][2 + r] = EvenBytes(w >> 8, magic);
+                            }
+                        } else {
+                            const uint32_t w = *reinterpret_cast<const uint32_t*>(at), u = w >> 8;
+                            f[0][r] = LowNibbles(w, magic);
+                            f[0][2 + r] = LowNibbles(u, magic);
+                            f[1][r] = HighNibbles(w, magic);
+                            f[1][2 + r] = HighNibbles(u, magic);
+                        }
+                    }
+                    const float d0 = ScaleOf(kd[2 * h], b), d1 = ScaleOf(kd[2 * h + 1], b);
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) {
+                        float d[4];
+                        MmaFirst(d, f[0], q0[n].z, q0[n].w);
+                        Mma(d, f[1], q1[n].z, q1[n].w);
+                        Mma(d, f[0], q0[n].x, q0[n].y);
+                        Mma(d, f[1], q1[n].x, q1[n].y);
+                        float(&to)[4] = x[n][h];
+                        to[0] = fmaf(d0, d[0], to[0]);
+                        to[1] = fmaf(d0, d[1], to[1]);
+                        to[2] = fmaf(d1, d[2], to[2]);
+                        to[3] = fmaf(d1, d[3], to[3]);
+                    }
                 }
             }
         }
         // weights as B fragments: row (query) g, slots 2c, 2c + 1 (+ 8)
-        uint32_t ph[NT][2], pl[NT][2];
+        const bool edge = low + kUnit > s.len;
+        uint32_t ph[NT][H][2], pl[NT][H][2];
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-            col[n].Weights(s, p0, low, x[n], kOffset, [&](float r0, float r1) { v[n].Scale(r0, r1); });
+            col[n].Weights(s, p0, low, edge, x[n], kOffset, [&](float r0, float r1) { v[n].Scale(r0, r1); });
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                SplitHalf(x[n][2 * i], x[n][2 * i + 1], ph[n][i], pl[n][i]);
-                ph[n][i] = Transpose8x8(ph[n][i]);
-                pl[n][i] = Transpose8x8(pl[n][i]);
-            }
+            for (int h = 0; h < H; ++h)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    SplitHalf(x[n][h][2 * i], x[n][h][2 * i + 1], ph[n][h][i], pl[n][h][i]);
+                    ph[n][h][i] = Transpose8x8(ph[n][h][i]);
+                    pl[n][h][i] = Transpose8x8(pl[n][h][i]);
+                }
         }
-        uint32_t d[2][NB];  // the scales of slots 2c, 2c + 1 (+ 8) as half pairs
+        uint32_t d[H][2][NB];  // the scales of slots 2c, 2c + 1 (+ 8) as half pairs
         {
             const __half* sc = reinterpret_cast<const __half*>(stage + 2 * kPlane + kScales) + 2 * s.c * NB;
-            uint32_t vd[4][(NB + 1) / 2];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) LoadScales<NB>(sc + ((i & 1) + (i >> 1) * 8) * NB, vd[i]);
+            for (int h = 0; h < H; ++h)
 #pragma unroll
-            for (int b = 0; b < NB; ++b)
+                for (int i = 0; i < 2; ++i) {
+                    uint32_t va[(NB + 1) / 2], vb[(NB + 1) / 2];
+                    LoadScales<NB>(sc + (i * 8 + h * kSlots) * NB, va);
+                    LoadScales<NB>(sc + (i * 8 + h * kSlots + 1) * NB, vb);
 #pragma unroll
-                for (int i = 0; i < 2; ++i)
-                    d[i][b] = __byte_perm(vd[2 * i][b >> 1], vd[2 * i + 1][b >> 1], b & 1 ? 0x7632 : 0x5410);
+                    for (int b = 0; b < NB; ++b)
+                        d[h][i][b] = __byte_perm(va[b >> 1], vb[b >> 1], b & 1 ? 0x7632 : 0x5410);
+                }
         }
-        const bool edge = low + kUnit > s.len;
+        uint32_t all = 0;  // the largest pair where every slot is seen
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-            float top;
-            {
-                uint32_t see[2] = {0xffffffffu, 0xffffffffu};
-                if (edge)  // a slot that is not seen may hold any scale, NaN too
+            __half2 big = AsHalf2(0u);
 #pragma unroll
-                    for (int i = 0; i < 2; ++i) see[i] = __hne2_mask(AsHalf2(ph[n][i]), AsHalf2(0u));
-                __half2 big = AsHalf2(0u);
-                if (edge) {
+            for (int h = 0; h < H; ++h)
 #pragma unroll
-                    for (int b = 0; b < NB; ++b)
+                for (int i = 0; i < 2; ++i) {
+                    if (edge) {  // a slot that is not seen may hold any scale, NaN too
+                        const uint32_t see = __hne2_mask(AsHalf2(ph[n][h][i]), AsHalf2(0u));
 #pragma unroll
-                        for (int i = 0; i < 2; ++i) big = __hmax2(big, AsHalf2(d[i][b] & see[i]));
-                } else {
+                        for (int b = 0; b < NB; ++b) big = __hmax2(big, AsHalf2(d[h][i][b] & see));
+                    } else if (n == 0) {
 #pragma unroll
-                    for (int b = 0; b < NB; ++b)
-#pragma unroll
-                        for (int i = 0; i < 2; ++i) big = __hmax2(big, AsHalf2(d[i][b]));
+                        for (int b = 0; b < NB; ++b) big = __hmax2(big, AsHalf2(d[h][i][b]));
+                    }
                 }
-                top = fmaxf(__low2float(big), __high2float(big));
-            }
+            if (n > 0 && !edge) big = AsHalf2(all);
+            if (n == 0) all = H2(big);
+            const float top = fmaxf(__low2float(big), __high2float(big));
             if (__any_sync(0xffffffffu, top > bound[n])) {
                 float t = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
                 t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 2));
@@ -497,49 +533,55 @@ struct QuantWarp {
         const uint8_t* row = stage + kPlane + 2 * s.c * kPitch + (kQuantBytes / 8) * s.g;
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
-            uint32_t f[2][4];
+            float t[NT][2][4];
 #pragma unroll
-            for (int r = 0; r < 2; ++r) {  // slots 2c, 2c + 1, then + 8
-                const uint8_t* at = row + 8 * r * kPitch + b * kQuantBytes;
-                if constexpr (TYPE == MLB_Q8_0) {
-                    const uint32_t w0 = *reinterpret_cast<const uint32_t*>(at);
-                    const uint32_t w1 = *reinterpret_cast<const uint32_t*>(at + kPitch);
-                    // bytes of the two slots side by side
-                    const uint32_t low2 = __byte_perm(w0, w1, 0x5410), high2 = __byte_perm(w0, w1, 0x7632);
-                    f[0][2 * r] = EvenBytes(low2, magic);
-                    f[0][2 * r + 1] = EvenBytes(low2 >> 8, magic);
-                    f[1][2 * r] = EvenBytes(high2, magic);
-                    f[1][2 * r + 1] = EvenBytes(high2 >> 8, magic);
-                } else {
-                    const uint32_t w = *reinterpret_cast<const unsigned short*>(at) |
-                                       (uint32_t(*reinterpret_cast<const unsigned short*>(at + kPitch)) << 16);
-                    const uint32_t u = w >> 8;
-                    f[0][2 * r] = LowNibbles(w, magic);
-                    f[0][2 * r + 1] = LowNibbles(u, magic);
-                    f[1][2 * r] = HighNibbles(w, magic);
-                    f[1][2 * r + 1] = HighNibbles(u, magic);
+            for (int h = 0; h < H; ++h) {
+                uint32_t f[2][4];
+#pragma unroll
+                for (int r = 0; r < 2; ++r) {  // slots 2c, 2c + 1, then + 8
+                    const uint8_t* at = row + (8 * r + h * kSlots) * kPitch + b * kQuantBytes;
+                    if constexpr (TYPE == MLB_Q8_0) {
+                        const uint32_t w0 = *reinterpret_cast<const uint32_t*>(at);
+                        const uint32_t w1 = *reinterpret_cast<const uint32_t*>(at + kPitch);
+                        // bytes of the two slots side by side
+                        const uint32_t low2 = __byte_perm(w0, w1, 0x5410), high2 = __byte_perm(w0, w1, 0x7632);
+                        f[0][2 * r] = EvenBytes(low2, magic);
+                        f[0][2 * r + 1] = EvenBytes(low2 >> 8, magic);
+                        f[1][2 * r] = EvenBytes(high2, magic);
+                        f[1][2 * r + 1] = EvenBytes(high2 >> 8, magic);
+                    } else {
+                        const uint32_t w = *reinterpret_cast<const unsigned short*>(at) |
+                                           (uint32_t(*reinterpret_cast<const unsigned short*>(at + kPitch)) << 16);
+                        const uint32_t u = w >> 8;
+                        f[0][2 * r] = LowNibbles(w, magic);
+                        f[0][2 * r + 1] = LowNibbles(u, magic);
+                        f[1][2 * r] = HighNibbles(w, magic);
+                        f[1][2 * r + 1] = HighNibbles(u, magic);
+                    }
+                }
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    uint32_t hi[2], lo[2];
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        uint32_t di = d[h][i][b];
+                        if (edge) di &= __hne2_mask(AsHalf2(ph[n][h][i]), AsHalf2(0u));
+                        const __half2 sc = __hmul2(AsHalf2(di), down[n]);
+                        const __half2 p = AsHalf2(ph[n][h][i]), y = __hmul2(p, sc);
+                        hi[i] = H2(y);
+                        lo[i] = H2(__hfma2(AsHalf2(pl[n][h][i]), sc, __hfma2(p, sc, __hneg2(y))));
+                    }
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        h == 0 ? MmaFirst(t[n][j], f[j], lo[0], lo[1]) : Mma(t[n][j], f[j], lo[0], lo[1]);
+                        Mma(t[n][j], f[j], hi[0], hi[1]);
+                    }
                 }
             }
 #pragma unroll
-            for (int n = 0; n < NT; ++n) {
-                uint32_t h[2], l[2];
+            for (int n = 0; n < NT; ++n)
 #pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    uint32_t di = d[i][b];
-                    if (edge) di &= __hne2_mask(AsHalf2(ph[n][i]), AsHalf2(0u));
-                    const __half2 sc = __hmul2(AsHalf2(di), down[n]);
-                    const __half2 p = AsHalf2(ph[n][i]), t = __hmul2(p, sc);
-                    h[i] = H2(t);
-                    l[i] = H2(__hfma2(AsHalf2(pl[n][i]), sc, __hfma2(p, sc, __hneg2(t))));
-                }
-#pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    float t[4];
-                    MmaFirst(t, f[j], l[0], l[1]);
-                    Mma(t, f[j], h[0], h[1]);
-                    AddTo(v[n].o[b][j], t);
-                }
-            }
+                for (int j = 0; j < 2; ++j) AddTo(v[n].o[b][j], t[n][j]);
         }
     }
 
@@ -555,6 +597,7 @@ struct QuantWarp {
 // ---------------------------------------------------------------- fp32 caches
 template <int NB, int NT>
 struct F32Warp {
+    static constexpr int kUnit = kSlots;
     static constexpr int kChunks = NB * 8;
     static constexpr int kPitch = (kChunks | 1) * 16;
     static constexpr int kPlane = kUnit * kPitch;
@@ -609,11 +652,11 @@ struct F32Warp {
     }
 
     __device__ __forceinline__ void Unit(const Step& s, const uint8_t* stage, const uint4* frags, int p0, int low) {
-        float x[NT][4], rest[NT][4];
+        float x[NT][1][4], rest[NT][4];
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) x[n][i] = rest[n][i] = 0.0f;
+            for (int i = 0; i < 4; ++i) x[n][0][i] = rest[n][i] = 0.0f;
         const float* row = reinterpret_cast<const float*>(stage + s.g * kPitch) + 8 * s.c;
 #pragma unroll
         for (int b = 0; b < NB; ++b)
@@ -633,7 +676,7 @@ struct F32Warp {
                         const uint4 q = frags[(n * kFrags + 4 * b + 2 * h + i) * 32];
                         MmaTf32(rest[n], lo, q.x, q.y);
                         MmaTf32(rest[n], hi, q.z, q.w);
-                        MmaTf32(x[n], hi, q.x, q.y);
+                        MmaTf32(x[n][0], hi, q.x, q.y);
                     }
                 }
             }
@@ -655,17 +698,17 @@ struct F32Warp {
         }
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-            AddTo(x[n], rest[n]);
-            col[n].Weights(s, p0, low, x[n], 0.0f, [&](float r0, float r1) { v[n].Scale(r0, r1); });
+            AddTo(x[n][0], rest[n]);
+            col[n].Weights(s, p0, low, edge, x[n], 0.0f, [&](float r0, float r1) { v[n].Scale(r0, r1); });
             if (odd) {
-                Plainly(s, stage, n, x[n]);
+                Plainly(s, stage, n, x[n][0]);
                 continue;
             }
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const int src = 4 * (2 * s.c + (i & 1)) + (s.g >> 1);
-                const float even = __shfl_sync(0xffffffffu, x[n][i & 2], src);
-                const float other = __shfl_sync(0xffffffffu, x[n][(i & 2) + 1], src);
+                const float even = __shfl_sync(0xffffffffu, x[n][0][i & 2], src);
+                const float other = __shfl_sync(0xffffffffu, x[n][0][(i & 2) + 1], src);
                 SplitTf32(s.g & 1 ? other : even, ph[n][i], pl[n][i]);
             }
         }
@@ -724,19 +767,20 @@ struct F32Warp {
     __device__ __forceinline__ void End(const Step&) {}
 };
 
+// One tile per warp leaves registers for two steps to a unit: half the sums of
+// the fresh accumulators, half the loads of Q.
 template <int TYPE, int NB, int NT>
 struct WarpOf {
-    using T = QuantWarp<TYPE, NB, NT>;
+    using T = QuantWarp<TYPE, NB, NT, NT == 1 ? 2 : 1>;
 };
 template <int NB, int NT>
 struct WarpOf<MLB_F32, NB, NT> {
     using T = F32Warp<NB, NT>;
 };
 
-__device__ __forceinline__ unsigned WarpSum32(unsigned v) { return __reduce_add_sync(0xffffffffu, v); }
-
-__device__ __forceinline__ unsigned EntryUnits(const TreeArgs& a, int b, unsigned items) {
-    return unsigned((FindEntry(a, b).slots + kUnit - 1) / kUnit) * items;
+// Units of a batch entry: `unit` slots each, for all its items.
+__device__ __forceinline__ unsigned EntryUnits(const TreeArgs& a, int b, unsigned unit, unsigned items) {
+    return (unsigned(FindEntry(a, b).slots) + unit - 1) / unit * items;
 }
 
 // Four consecutive elements of an output row.
@@ -774,15 +818,52 @@ struct Joined {
     }
 };
 
-// Even cuts of `total` units over `ctas` CTAs: the first `extra` take one more.
+// The list of all units, cut evenly over the CTAs: the first `extra` take one
+// more.  A warp works it out together.
 struct Cut {
-    unsigned each, extra;
+    unsigned total, ctas, each, extra;
 
-    __device__ __forceinline__ Cut(unsigned total, unsigned ctas) : each(total / ctas), extra(total - each * ctas) {}
+    // `groups`: units that a CTA works on at a time.
+    __device__ __forceinline__ Cut(const TreeArgs& a, unsigned unit, unsigned items, unsigned groups, unsigned grid) {
+        const int lane = threadIdx.x & 31;
+        unsigned live = 0;
+        total = 0;
+        for (int b0 = 0; b0 < a.batch; b0 += 32) {
+            const unsigned n = b0 + lane < a.batch ? EntryUnits(a, b0 + lane, unit, items) : 0;
+            total += __reduce_add_sync(0xffffffffu, n);
+            live += __popc(__ballot_sync(0xffffffffu, n != 0));
+        }
+        // a unit for each group, or an item for each CTA, at least
+        ctas = max(1u, min(max((total + groups - 1) / groups, min(live * items, total)), grid));
+        each = total / ctas;
+        extra = total - each * ctas;
+    }
     __device__ __forceinline__ unsigned Start(unsigned cta) const { return cta * each + min(cta, extra); }
-    __device__ __forceinline__ unsigned Owner(unsigned unit) const {
+    __device__ __forceinline__ unsigned Owner(unsigned at) const {
         const unsigned high = extra * (each + 1);
-        return unit < high ? unit / (each + 1) : extra + (unit - high) / each;
+        return at < high ? at / (each + 1) : extra + (at - high) / each;
+    }
+    // The batch entry of unit `at`, and that entry's first unit.
+    __device__ __forceinline__ int Find(const TreeArgs& a, unsigned unit, unsigned items, unsigned at, unsigned& first) const {
+        const int lane = threadIdx.x & 31;
+        first = 0;
+        for (int b0 = 0; b0 < a.batch; b0 += 32) {
+            const unsigned n = b0 + lane < a.batch ? EntryUnits(a, b0 + lane, unit, items) : 0;
+            unsigned incl = n;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const unsigned t = __shfl_up_sync(0xffffffffu, incl, o);
+                if (lane >= o) incl += t;
+            }
+            const unsigned past = __ballot_sync(0xffffffffu, first + incl > at);
+            if (past) {
+                const int to = __ffs(past) - 1;
+                first += __shfl_sync(0xffffffffu, incl - n, to);
+                return b0 + to;
+            }
+            first += __shfl_sync(0xffffffffu, incl, 31);
+        }
+        return a.batch;
     }
 };
 
@@ -813,6 +894,7 @@ __global__ void __launch_bounds__(NW * 32, 1) TreeMmaKernel(TreeArgs a, TreeSpli
     using Shape = TreeShape<TYPE, NB, NT, WQ, NW>;
     using Warp = typename Shape::Warp;
     constexpr int kPitch = Shape::kPitch, kFours = NB * 8, kItemRows = Shape::kItemRows, kStages = Shape::kStages;
+    constexpr int kUnit = Warp::kUnit, kStageBytes = Warp::kStageBytes;
     constexpr unsigned kGroups = Shape::kGroups;
     extern __shared__ uint4 smem4[];
     uint8_t* ring = reinterpret_cast<uint8_t*>(smem4);
@@ -821,7 +903,6 @@ __global__ void __launch_bounds__(NW * 32, 1) TreeMmaKernel(TreeArgs a, TreeSpli
     float* sl = sm + NW * Shape::kRowsOf;
     uint4* sq = reinterpret_cast<uint4*>(ring + (Shape::kTop + 15) / 16 * 16);  // [WQ NT][kFrags][32]
     float* su = reinterpret_cast<float*>(sq + Shape::kFragBytes / 16);          // [WQ NT][8]
-    __shared__ int s_last;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int wq = warp % WQ, group = warp / WQ;
     const unsigned items = a.c.n_kv * sp.groups;
@@ -834,36 +915,13 @@ __global__ void __launch_bounds__(NW * 32, 1) TreeMmaKernel(TreeArgs a, TreeSpli
                 a.out[(size_t(b) * a.tokens + t) * a.out_stride + i] = 0.0f;
     }
 
-    // the cut: all units in a row, an even stretch for each CTA
-    unsigned total = 0;
-    for (int b0 = 0; b0 < a.batch; b0 += 32) total += WarpSum32(b0 + lane < a.batch ? EntryUnits(a, b0 + lane, items) : 0);
-    if (total == 0) return;
-    const unsigned ctas = min((total + kGroups - 1) / kGroups, gridDim.x);  // a unit for each group at least
-    if (blockIdx.x >= ctas) return;
-    const Cut cut(total, ctas);
+    GridDepLaunch();  // the joining kernel may come up as CTAs leave
+    const Cut cut(a, kUnit, items, kGroups, gridDim.x);
+    if (cut.total == 0 || blockIdx.x >= cut.ctas) return;
     unsigned cur = cut.Start(blockIdx.x);
     const unsigned end = cut.Start(blockIdx.x + 1);
-    // the entry of the first unit
-    int b = 0;
-    unsigned first = 0;
-    for (int b0 = 0; b0 < a.batch; b0 += 32) {
-        const unsigned n = b0 + lane < a.batch ? EntryUnits(a, b0 + lane, items) : 0;
-        const unsigned chunk = WarpSum32(n);
-        if (cur >= first + chunk) {
-            first += chunk;
-            continue;
-        }
-        unsigned incl = n;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const unsigned t = __shfl_up_sync(0xffffffffu, incl, o);
-            if (lane >= o) incl += t;
-        }
-        const int at = __ffs(__ballot_sync(0xffffffffu, first + incl > cur)) - 1;
-        first += __shfl_sync(0xffffffffu, incl - n, at);
-        b = b0 + at;
-        break;
-    }
+    unsigned first;
+    int b = cut.Find(a, kUnit, items, cur, first);
 
     Step s;
     s.lane = lane;
@@ -894,16 +952,18 @@ __global__ void __launch_bounds__(NW * 32, 1) TreeMmaKernel(TreeArgs a, TreeSpli
 
         // ---- the ring's first units, then the Q fragments
         w.Begin(a, sp, e.seq, head);
-        auto copy = [&](int k) {  // unit k of the group
-            const int u = u0 + group + k * int(kGroups);
-            // the last unit of a plane may hold fewer than 16 slots: it starts earlier and leaves the others out
-            if (u < u1)
-                w.template Copy<WQ * 32>(ring_at + (k % kStages) * Warp::kStageBytes, min(u * kUnit, last_unit),
-                                         wq * 32 + lane);
+        int from = u0 + group;  // the unit to copy next
+        int into = 0;           // its stage
+        auto copy = [&] {
+            // the last unit of a plane may hold fewer slots: it starts earlier and leaves the others out
+            if (from < u1)
+                w.template Copy<WQ * 32>(ring_at + into, min(from * kUnit, last_unit), wq * 32 + lane);
             asm volatile("cp.async.commit_group;" ::: "memory");
+            from += kGroups;
+            into = into + kStageBytes == kStages * kStageBytes ? 0 : into + kStageBytes;
         };
 #pragma unroll
-        for (int k = 0; k < kStages - 1; ++k) copy(k);
+        for (int k = 0; k < kStages - 1; ++k) copy();
         for (int n = warp; n < WQ * NT; n += NW) {
             const int r = row0 + n * kRows + s.g;
             const float* q = r < sp.rows ? a.q + (size_t(b) * a.tokens + r / a.group) * a.q_stride +
@@ -923,17 +983,17 @@ __global__ void __launch_bounds__(NW * 32, 1) TreeMmaKernel(TreeArgs a, TreeSpli
 
         // ---- the group's units
         const uint4* frags = sq + wq * NT * Warp::kFrags * 32 + lane;
-        int k = 0;
-        for (int u = u0 + group; u < u1; u += kGroups, ++k) {
+        const uint8_t* stage = ring_ptr;
+        for (int u = u0 + group; u < u1; u += kGroups) {
             asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
             // every copy of this unit has landed, and the stage refilled next has been read
             if (WQ == 1)
                 __syncwarp();
             else
                 asm volatile("bar.sync %0, %1;" ::"r"(group + 1), "n"(WQ * 32) : "memory");
-            copy(k + kStages - 1);
-            if (tile < sp.rows)
-                w.Unit(s, ring_ptr + (k % kStages) * Warp::kStageBytes, frags, min(u * kUnit, last_unit), u * kUnit);
+            copy();
+            if (tile < sp.rows) w.Unit(s, stage, frags, min(u * kUnit, last_unit), u * kUnit);
+            stage = stage + kStageBytes == ring_ptr + kStages * kStageBytes ? ring_ptr : stage + kStageBytes;
         }
         w.End(s);
         asm volatile("cp.async.wait_group 0;" ::: "memory");
@@ -991,44 +1051,56 @@ __global__ void __launch_bounds__(NW * 32, 1) TreeMmaKernel(TreeArgs a, TreeSpli
             }
         }
 
-        // ---- join the CTAs that share the item: the last to arrive adds them up
-        if (!whole) {
-            const unsigned c0 = cut.Owner(cur - u0), c1 = cut.Owner(cur - u0 + units - 1);  // of its first and last unit
-            __threadfence();
-            __syncthreads();
-            if (threadIdx.x == 0) {
-                int* counter = sp.counters + size_t(b) * items + item;
-                s_last = atomicAdd(counter, 1) == int(c1 - c0);
-                if (s_last) *counter = 0;  // every contributor has arrived
-            }
-            __syncthreads();
-            if (s_last) {
-                __threadfence();
-                // a CTA has two parts: of an item that it begins, and of one that it goes on with
-                for (int i = threadIdx.x; i < live_rows * kFours; i += NW * 32) {
-                    const int r = i / kFours, d = (i - r * kFours) * 4;
-                    Joined x;
-                    for (unsigned k0 = c0; k0 <= c1; k0 += 4) {
-                        float pm[4], pl[4];
-                        float4 po[4];
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            if (k0 + j > c1) break;
-                            const float* p = sp.parts + (2 * size_t(k0 + j) + (cut.Start(k0 + j) <= cur - u0 ? 1 : 0)) * kPart;
-                            pm[j] = __ldcg(p + kItemRows * NB * 32 + r);
-                            pl[j] = __ldcg(p + kItemRows * (NB * 32 + 1) + r);
-                            po[j] = __ldcg(reinterpret_cast<const float4*>(p + r * NB * 32 + d));
-                        }
-#pragma unroll
-                        for (int j = 0; j < 4; ++j)
-                            if (k0 + j <= c1) x.Add(pm[j], pl[j], po[j]);
-                    }
-                    StoreOut(a, OutRow(a, b, head, row0 + r), d, x.Result());
-                }
-            }
-        }
         __syncthreads();
         cur += u1 - u0;
+    }
+}
+
+// Items that are cut between CTAs: a warp per row adds up their parts, in the
+// order of the CTAs.  blockIdx.x: item, blockIdx.y: rows y, y + gridDim.y, ..
+constexpr int kJoinWarps = 8;
+constexpr int kJoinBatch = 8;  // parts in flight
+
+template <int NB>
+__global__ void __launch_bounds__(kJoinWarps * 32) TreeJoinKernel(TreeArgs a, TreeSplit sp, int unit, int groups,
+                                                                  int item_rows, int grid) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const unsigned items = a.c.n_kv * sp.groups;
+    const int b = blockIdx.x / items;
+    const unsigned item = blockIdx.x - b * items;
+    const Cut cut(a, unit, items, groups, grid);
+    const unsigned units = EntryUnits(a, b, unit, 1);
+    if (units == 0) return;
+    unsigned first = 0;  // of the entry
+    for (int b0 = 0; b0 < b; b0 += 32)
+        first += __reduce_add_sync(0xffffffffu, b0 + lane < b ? EntryUnits(a, b0 + lane, unit, items) : 0);
+    const unsigned u0 = first + item * units;
+    const unsigned c0 = cut.Owner(u0), c1 = cut.Owner(u0 + units - 1);
+    if (c0 == c1) return;
+    GridDepWait();
+    const int head = item / sp.groups, row0 = (item - head * sp.groups) * item_rows;
+    const int rows = min(item_rows, sp.rows - row0);
+    const size_t part = size_t(item_rows) * (NB * 32 + 2);
+    for (int r = blockIdx.y * kJoinWarps + warp; r < rows; r += gridDim.y * kJoinWarps) {
+        const int d = min(lane, NB * 8 - 1) * 4;
+        Joined x;
+        for (unsigned k = c0; k <= c1; k += kJoinBatch) {
+            float pm[kJoinBatch], pl[kJoinBatch];
+            float4 po[kJoinBatch];
+#pragma unroll
+            for (int j = 0; j < kJoinBatch; ++j) {
+                // a CTA has two parts: of the item that it goes on with, and of one that it begins
+                const unsigned cta = min(k + j, c1);
+                const float* p = sp.parts + (2 * size_t(cta) + (cut.Start(cta) <= u0 ? 1 : 0)) * part;
+                pm[j] = __ldcg(p + item_rows * NB * 32 + r);
+                pl[j] = __ldcg(p + item_rows * (NB * 32 + 1) + r);
+                po[j] = __ldcg(reinterpret_cast<const float4*>(p + r * NB * 32 + d));
+            }
+#pragma unroll
+            for (int j = 0; j < kJoinBatch; ++j)
+                if (k + j <= c1) x.Add(pm[j], pl[j], po[j]);
+        }
+        if (lane < NB * 8) StoreOut(a, OutRow(a, b, head, row0 + r), d, x.Result());
     }
 }
 
@@ -1041,13 +1113,12 @@ bool LaunchShape(DeviceContext& ctx, const TreeArgs& a) {
     const unsigned long long items = 1ull * a.c.n_kv * sp.groups;
     // an upper bound of the units, from the caller's bound of the lengths
     const long long slots = std::min<long long>(1LL * std::min(a.max_len, a.c.max_seq) + a.tokens, a.c.max_seq);
-    const double units = double(a.batch) * double(items) * double(CeilDiv(slots, kUnit));
-    if (units >= 2147483648.0) return false;
-    const int grid = static_cast<int>(
-        std::max(1.0, std::min<double>(ctx.sm_count, std::ceil(units / Shape::kGroups))));
+    const double units = double(a.batch) * double(items) * double(CeilDiv(slots, Shape::Warp::kUnit));
+    if (units >= 2147483648.0 || a.c.head_slots < Shape::Warp::kUnit) return false;
+    const int grid = static_cast<int>(std::min<double>(
+        ctx.sm_count, std::max(std::ceil(units / Shape::kGroups), double(a.batch) * double(items))));
     sp.parts = static_cast<float*>(
         Workspace(ctx, 2 * size_t(grid) * Shape::kItemRows * (NB * 32 + 2) * sizeof(float)));
-    sp.counters = TreeCounters(ctx, size_t(a.batch) * items);
     sp.magic = TYPE == MLB_Q8_0 ? kMagic8 : kMagic4;
     auto* kernel = TreeMmaKernel<TYPE, NB, NT, WQ, NW>;
     static int configured[64] = {};
@@ -1058,6 +1129,11 @@ bool LaunchShape(DeviceContext& ctx, const TreeArgs& a) {
     }
     kernel<<<grid, NW * 32, Shape::kBytes, ctx.stream>>>(a, sp);
     CheckCuda(cudaGetLastError(), "TreeMmaKernel");
+    if (grid == 1) return true;  // nothing is cut
+    const int all = a.batch * static_cast<int>(items);
+    const int per_item = std::max(1, std::min(Shape::kItemRows / kJoinWarps, 4 * ctx.sm_count / all));
+    Launch("TreeJoinKernel", TreeJoinKernel<NB>, dim3(all, per_item), dim3(kJoinWarps * 32), 0, ctx.stream, true, a, sp,
+           int(Shape::Warp::kUnit), int(Shape::kGroups), int(Shape::kItemRows), grid);
     return true;
 }
 
