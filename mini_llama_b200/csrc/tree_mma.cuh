@@ -52,20 +52,12 @@ constexpr float kOffset = 12.0f;    // weights are relative to 2^12: at most 2^1
                                     // 2^-37 of the largest, for slots that weigh little where the heavy ones hold zeros
 constexpr float kLog2e = 1.4426950408889634f;
 
-constexpr int kMaxShared = 225 * 1024;
+constexpr int kSmShared = 226 * 1024;  // shared memory of an SM for its CTAs
 constexpr int kMaxStages = 4;
-
-// Warps of a CTA by form (one, two tiles per warp; two tiles and four warps to a
-// group): registers and the ring bound them.
-#ifndef TREE_W1
-#define TREE_W1 12
+#ifndef TREE_NW4
+#define TREE_NW4 4
+#define TREE_PER4 3
 #endif
-template <int TYPE, int NB>
-constexpr int kWarps1 = TYPE == MLB_F32 ? (NB > 2 ? 6 : 12) : (TYPE == MLB_Q8_0 && NB == 4 ? 11 : TREE_W1);
-template <int TYPE, int NB>
-constexpr int kWarps2 = TYPE == MLB_F32 ? (NB > 2 ? 6 : 12) : 12;
-template <int TYPE, int NB>
-constexpr int kWarps4 = TYPE == MLB_F32 && NB > 2 ? 8 : 12;
 
 struct TreeSplit {
     int groups;    // items of a (sequence, KV head): ceil(R / (8 NT WQ))
@@ -307,9 +299,12 @@ struct QuantWarp {
     static constexpr int kUnit = kSlots * H;
     static constexpr int kQuantBytes = TYPE == MLB_Q8_0 ? 32 : 16;
     static constexpr int kChunks = NB * kQuantBytes / 16;  // of a row
-    static constexpr int kPitch = (kChunks | 1) * 16;      // of a row in the ring
+    // Rows of eight chunks are stored with chunk j at j ^ (row % 8), others an odd number of chunks apart: either
+    // way the rows that a fragment load touches lie in different banks.
+    static constexpr bool kXor = kChunks == 8;
+    static constexpr int kPitch = kXor ? 128 : (kChunks | 1) * 16;
     static constexpr int kPlane = kUnit * kPitch, kScales = kUnit * NB * 2;
-    static constexpr int kStageBytes = 2 * kPlane + 2 * kScales;
+    static constexpr int kStageBytes = kPlane + kScales;   // of K, and of V
     static constexpr int kFrags = 2 * NB;                  // uint4 per lane and tile: (hi, hi, lo, lo)
 
     Values<NB> v[NT];
@@ -317,6 +312,9 @@ struct QuantWarp {
     int e[NT];         // of row g: P' is relative to 2^e
     float bound[NT];   // 2^e
     __half2 down[NT];  // 2^-e
+    // weights of the unit as B fragments: row (query) g, slots 2c, 2c + 1 (+ 8), hi and lo
+    uint32_t ph[NT][H][2], pl[NT][H][2];
+    bool edge;         // not every row sees all of the unit
     uint32_t magic;
     const uint8_t *kp, *vp;  // the head's planes
     const __half *ksp, *vsp;
@@ -390,36 +388,41 @@ struct QuantWarp {
         }
     }
 
-    // The unit at p0 into a ring stage, by the `count` threads of a group.
+    // K (or V) of the unit at p0 into a ring stage, by the COUNT threads of a group.
     template <int COUNT>
-    __device__ __forceinline__ void Copy(uint32_t stage, int p0, int id) const {
-        const uint8_t* k = kp + size_t(p0) * (NB * kQuantBytes);
-        const uint8_t* w = vp + size_t(p0) * (NB * kQuantBytes);
+    __device__ __forceinline__ static void Copy(const uint8_t* plane, const __half* scales, uint32_t stage, int p0, int id) {
+        const uint8_t* from = plane + size_t(p0) * (NB * kQuantBytes);
         constexpr int kAll = kUnit * kChunks;
 #pragma unroll
         for (int j = 0; j < (kAll + COUNT - 1) / COUNT; ++j) {
             const int i = id + j * COUNT;
             if (kAll % COUNT != 0 && i >= kAll) break;
-            const uint32_t to = stage + i / kChunks * kPitch + i % kChunks * 16;
-            CopyChunk(to, k + i * 16);
-            CopyChunk(to + kPlane, w + i * 16);
+            const int row = i / kChunks, chunk = i % kChunks;
+            CopyChunk(stage + row * kPitch + (kXor ? chunk ^ (row & 7) : chunk) * 16, from + i * 16);
         }
-        constexpr int kSc = kScales / 16;  // 2 NB chunks of each
-        if (id < 2 * kSc) {
-            const __half* from = id < kSc ? ksp + size_t(p0) * NB + id * 8 : vsp + size_t(p0) * NB + (id - kSc) * 8;
-            CopyChunk(stage + 2 * kPlane + id * 16, from);
-        }
+        constexpr int kSc = kScales / 16;  // at most 16
+        if (id < kSc) CopyChunk(stage + kPlane + id * 16, scales + size_t(p0) * NB + id * 8);
+    }
+    template <int COUNT>
+    __device__ __forceinline__ void CopyK(uint32_t stage, int p0, int id) const {
+        Copy<COUNT>(kp, ksp, stage, p0, id);
+    }
+    template <int COUNT>
+    __device__ __forceinline__ void CopyV(uint32_t stage, int p0, int id) const {
+        Copy<COUNT>(vp, vsp, stage, p0, id);
     }
 
-    // The staged unit at p0; slots below `low` are another unit's.
-    __device__ __forceinline__ void Unit(const Step& s, const uint8_t* stage, const uint4* frags, int p0, int low) {
+    // Scores and weights of the unit at p0, its K staged; slots below `low` are
+    // another unit's.
+    __device__ __forceinline__ void Keys(const Step& s, const uint8_t* stage, const uint4* frags, int p0, int low) {
+        edge = low + kUnit > s.len;
         float x[NT][H][4];
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
             for (int h = 0; h < H; ++h) x[n][h][0] = x[n][h][1] = x[n][h][2] = x[n][h][3] = 0.0f;
         {
-            const __half* sc = reinterpret_cast<const __half*>(stage + 2 * kPlane) + s.g * NB;
+            const __half* sc = reinterpret_cast<const __half*>(stage + kPlane) + s.g * NB;
             uint32_t kd[2 * H][(NB + 1) / 2];
 #pragma unroll
             for (int r = 0; r < 2 * H; ++r) LoadScales<NB>(sc + 8 * r * NB, kd[r]);
@@ -437,16 +440,17 @@ struct QuantWarp {
                     uint32_t f[2][4];
 #pragma unroll
                     for (int r = 0; r < 2; ++r) {
-                        const uint8_t* at = row + (8 * r + h * kSlots) * kPitch + b * kQuantBytes;
+                        const uint8_t* at = row + (8 * r + h * kSlots) * kPitch;
                         if constexpr (TYPE == MLB_Q8_0) {
 #pragma unroll
                             for (int i = 0; i < 2; ++i) {
-                                const uint32_t w = *reinterpret_cast<const uint32_t*>(at + 16 * i);
+                                const int chunk = kXor ? ((2 * b + i) ^ s.g) * 16 : (2 * b + i) * 16;
+                                const uint32_t w = *reinterpret_cast<const uint32_t*>(at + chunk);
                                 f[i][r] = EvenBytes(w, magic);
                                 f[i][2 + r] = EvenBytes(w >> 8, magic);
                             }
                         } else {
-                            const uint32_t w = *reinterpret_cast<const uint32_t*>(at), u = w >> 8;
+                            const uint32_t w = *reinterpret_cast<const uint32_t*>(at + b * 16), u = w >> 8;
                             f[0][r] = LowNibbles(w, magic);
                             f[0][2 + r] = LowNibbles(u, magic);
                             f[1][r] = HighNibbles(w, magic);
@@ -470,9 +474,6 @@ struct QuantWarp {
                 }
             }
         }
-        // weights as B fragments: row (query) g, slots 2c, 2c + 1 (+ 8)
-        const bool edge = low + kUnit > s.len;
-        uint32_t ph[NT][H][2], pl[NT][H][2];
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
             col[n].Weights(s, p0, low, edge, x[n], kOffset, [&](float r0, float r1) { v[n].Scale(r0, r1); });
@@ -485,9 +486,13 @@ struct QuantWarp {
                     pl[n][h][i] = Transpose8x8(pl[n][h][i]);
                 }
         }
+    }
+
+    // The weighted values of the unit, its V staged.
+    __device__ __forceinline__ void Sum(const Step& s, const uint8_t* stage) {
         uint32_t d[H][2][NB];  // the scales of slots 2c, 2c + 1 (+ 8) as half pairs
         {
-            const __half* sc = reinterpret_cast<const __half*>(stage + 2 * kPlane + kScales) + 2 * s.c * NB;
+            const __half* sc = reinterpret_cast<const __half*>(stage + kPlane) + 2 * s.c * NB;
 #pragma unroll
             for (int h = 0; h < H; ++h)
 #pragma unroll
@@ -530,7 +535,8 @@ struct QuantWarp {
                 v[n].Scale(__shfl_sync(0xffffffffu, f, 8 * s.c), __shfl_sync(0xffffffffu, f, 8 * s.c + 4));
             }
         }
-        const uint8_t* row = stage + kPlane + 2 * s.c * kPitch + (kQuantBytes / 8) * s.g;
+        const uint8_t* row = stage + 2 * s.c * kPitch + (kXor ? 4 * (s.g & 3) : (kQuantBytes / 8) * s.g);
+        const int turn = ((s.g >> 2) ^ (2 * s.c)) * 16;  // chunk of the first slot in block 0
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
             float t[NT][2][4];
@@ -539,10 +545,11 @@ struct QuantWarp {
                 uint32_t f[2][4];
 #pragma unroll
                 for (int r = 0; r < 2; ++r) {  // slots 2c, 2c + 1, then + 8
-                    const uint8_t* at = row + (8 * r + h * kSlots) * kPitch + b * kQuantBytes;
+                    const uint8_t* at = row + (8 * r + h * kSlots) * kPitch + (kXor ? 0 : b * kQuantBytes);
                     if constexpr (TYPE == MLB_Q8_0) {
-                        const uint32_t w0 = *reinterpret_cast<const uint32_t*>(at);
-                        const uint32_t w1 = *reinterpret_cast<const uint32_t*>(at + kPitch);
+                        const int o0 = kXor ? turn ^ (32 * b) : 0, o1 = kXor ? turn ^ (32 * b + 16) : 0;
+                        const uint32_t w0 = *reinterpret_cast<const uint32_t*>(at + o0);
+                        const uint32_t w1 = *reinterpret_cast<const uint32_t*>(at + kPitch + o1);
                         // bytes of the two slots side by side
                         const uint32_t low2 = __byte_perm(w0, w1, 0x5410), high2 = __byte_perm(w0, w1, 0x7632);
                         f[0][2 * r] = EvenBytes(low2, magic);
@@ -600,12 +607,13 @@ struct F32Warp {
     static constexpr int kUnit = kSlots;
     static constexpr int kChunks = NB * 8;
     static constexpr int kPitch = (kChunks | 1) * 16;
-    static constexpr int kPlane = kUnit * kPitch;
-    static constexpr int kStageBytes = 2 * kPlane;
+    static constexpr int kStageBytes = kUnit * kPitch;  // of K, and of V
     static constexpr int kFrags = 4 * NB;
 
     Values<NB> v[NT];
     Columns col[NT];
+    float p[NT][4];  // weights of the unit, as the scores' C fragments
+    bool edge;       // not every row sees all of the unit
     const float *kp, *vp;
     int pitch;  // floats between slots
     int hd;
@@ -638,20 +646,27 @@ struct F32Warp {
     }
 
     template <int COUNT>
-    __device__ __forceinline__ void Copy(uint32_t stage, int p0, int id) const {
+    __device__ __forceinline__ void Copy(const float* plane, uint32_t stage, int p0, int id) const {
         constexpr int kAll = kUnit * kChunks;
+#pragma unroll 4
         for (int j = 0; j < (kAll + COUNT - 1) / COUNT; ++j) {
             const int i = id + j * COUNT;
             if (kAll % COUNT != 0 && i >= kAll) break;
             const int r = i / kChunks, d = i % kChunks * 4, bytes = d < hd ? 16 : 0;
-            const size_t at = size_t(p0 + r) * pitch + (d < hd ? d : 0);
-            const uint32_t to = stage + r * kPitch + d * 4;
-            CopyChunk(to, kp + at, bytes);
-            CopyChunk(to + kPlane, vp + at, bytes);
+            CopyChunk(stage + r * kPitch + d * 4, plane + size_t(p0 + r) * pitch + (d < hd ? d : 0), bytes);
         }
     }
+    template <int COUNT>
+    __device__ __forceinline__ void CopyK(uint32_t stage, int p0, int id) const {
+        Copy<COUNT>(kp, stage, p0, id);
+    }
+    template <int COUNT>
+    __device__ __forceinline__ void CopyV(uint32_t stage, int p0, int id) const {
+        Copy<COUNT>(vp, stage, p0, id);
+    }
 
-    __device__ __forceinline__ void Unit(const Step& s, const uint8_t* stage, const uint4* frags, int p0, int low) {
+    __device__ __forceinline__ void Keys(const Step& s, const uint8_t* stage, const uint4* frags, int p0, int low) {
+        edge = low + kUnit > s.len;
         float x[NT][1][4], rest[NT][4];
 #pragma unroll
         for (int n = 0; n < NT; ++n)
@@ -680,12 +695,19 @@ struct F32Warp {
                     }
                 }
             }
-        // weights as B fragments: query g, slots 2c and 2c + 1 (+ 8)
-        uint32_t ph[NT][4], pl[NT][4];
-        bool odd = false;
-        const float* vrow = reinterpret_cast<const float*>(stage + kPlane + 2 * s.c * kPitch) + 4 * s.g;
-        const bool edge = low + kUnit > s.len;
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            AddTo(x[n][0], rest[n]);
+            col[n].Weights(s, p0, low, edge, x[n], 0.0f, [&](float r0, float r1) { v[n].Scale(r0, r1); });
+#pragma unroll
+            for (int i = 0; i < 4; ++i) p[n][i] = x[n][0][i];
+        }
+    }
+
+    __device__ __forceinline__ void Sum(const Step& s, const uint8_t* stage) {
+        const float* vrow = reinterpret_cast<const float*>(stage + 2 * s.c * kPitch) + 4 * s.g;
         if (edge) {  // a slot that some rows do not see may hold NaN or infinities
+            bool odd = false;
 #pragma unroll
             for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -694,25 +716,23 @@ struct F32Warp {
                     odd = odd || !(fabsf(y.x) <= 3.4e38f && fabsf(y.y) <= 3.4e38f && fabsf(y.z) <= 3.4e38f &&
                                    fabsf(y.w) <= 3.4e38f);
                 }
-            odd = __any_sync(0xffffffffu, odd);
-        }
+            if (__any_sync(0xffffffffu, odd)) {
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-            AddTo(x[n][0], rest[n]);
-            col[n].Weights(s, p0, low, edge, x[n], 0.0f, [&](float r0, float r1) { v[n].Scale(r0, r1); });
-            if (odd) {
-                Plainly(s, stage, n, x[n][0]);
-                continue;
+                for (int n = 0; n < NT; ++n) Plainly(s, stage, n);
+                return;
             }
+        }
+        // weights as B fragments: query g, slots 2c and 2c + 1 (+ 8)
+        uint32_t ph[NT][4], pl[NT][4];
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const int src = 4 * (2 * s.c + (i & 1)) + (s.g >> 1);
-                const float even = __shfl_sync(0xffffffffu, x[n][0][i & 2], src);
-                const float other = __shfl_sync(0xffffffffu, x[n][0][(i & 2) + 1], src);
+                const float even = __shfl_sync(0xffffffffu, p[n][i & 2], src);
+                const float other = __shfl_sync(0xffffffffu, p[n][(i & 2) + 1], src);
                 SplitTf32(s.g & 1 ? other : even, ph[n][i], pl[n][i]);
             }
-        }
-        if (odd) return;
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
             float4 y[4];
@@ -744,8 +764,9 @@ struct F32Warp {
     }
 
     // The weighted values of one unit slot by slot, those of weight 0 left out.
-    __device__ __forceinline__ void Plainly(const Step& s, const uint8_t* stage, int n, const float (&x)[4]) {
-        const float* row = reinterpret_cast<const float*>(stage + kPlane) + 4 * s.g;
+    __device__ __forceinline__ void Plainly(const Step& s, const uint8_t* stage, int n) {
+        const float(&x)[4] = p[n];
+        const float* row = reinterpret_cast<const float*>(stage) + 4 * s.g;
         for (int i = 0; i < kUnit; ++i) {
             const int src = 4 * (i & 7) + s.c;
             const float w0 = __shfl_sync(0xffffffffu, i < 8 ? x[0] : x[2], src);
@@ -867,9 +888,10 @@ struct Cut {
     }
 };
 
-// Shared memory: the ring, which the joining of the groups reuses, the Q
-// fragments and the score factors.
-template <int TYPE, int NB, int NT, int WQ, int NW>
+// Shared memory: the ring of every group (S stages of K, then S of V), which the
+// joining of the groups reuses, the Q fragments and the score factors.  PER_SM
+// CTAs share an SM, so that one joins or starts while another computes.
+template <int TYPE, int NB, int NT, int WQ, int NW, int PER_SM>
 struct TreeShape {
     using Warp = typename WarpOf<TYPE, NB, NT>::T;
     static constexpr int kGroups = NW / WQ;
@@ -879,19 +901,20 @@ struct TreeShape {
     static constexpr int kFragBytes = WQ * NT * Warp::kFrags * 32 * 16;
     static constexpr int kJoinBytes = NW * kRowsOf * (kPitch + 2) * 4;
     static constexpr int kUndoBytes = WQ * kRowsOf * 4;
-    static constexpr int kFit = (kMaxShared - kFragBytes - kUndoBytes) / (kGroups * Warp::kStageBytes);
+    static constexpr int kMaxShared = kSmShared / PER_SM - 1024;
+    static constexpr int kFit = (kMaxShared - kFragBytes - kUndoBytes) / (kGroups * 2 * Warp::kStageBytes);
     static constexpr int kStages = kFit < kMaxStages ? kFit : kMaxStages;
-    static constexpr int kRingBytes = kGroups * kStages * Warp::kStageBytes;
-    static constexpr int kTop = (kRingBytes > kJoinBytes ? kRingBytes : kJoinBytes);
+    static constexpr int kRingBytes = kStages * 2 * Warp::kStageBytes;  // of a group
+    static constexpr int kTop = (kGroups * kRingBytes > kJoinBytes ? kGroups * kRingBytes : kJoinBytes);
     static constexpr int kBytes = (kTop + 15) / 16 * 16 + kFragBytes + kUndoBytes;
     static_assert(kStages >= 2, "a ring has two stages at least");
-    static_assert(kBytes <= kMaxShared + 1024, "shared memory");
+    static_assert(kBytes <= kMaxShared, "shared memory");
     static_assert(kGroups <= 15, "a named barrier per group");
 };
 
-template <int TYPE, int NB, int NT, int WQ, int NW>
-__global__ void __launch_bounds__(NW * 32, 1) TreeMmaKernel(TreeArgs a, TreeSplit sp) {
-    using Shape = TreeShape<TYPE, NB, NT, WQ, NW>;
+template <int TYPE, int NB, int NT, int WQ, int NW, int PER_SM>
+__global__ void __launch_bounds__(NW * 32, PER_SM) TreeMmaKernel(TreeArgs a, TreeSplit sp) {
+    using Shape = TreeShape<TYPE, NB, NT, WQ, NW, PER_SM>;
     using Warp = typename Shape::Warp;
     constexpr int kPitch = Shape::kPitch, kFours = NB * 8, kItemRows = Shape::kItemRows, kStages = Shape::kStages;
     constexpr int kUnit = Warp::kUnit, kStageBytes = Warp::kStageBytes;
@@ -930,8 +953,9 @@ __global__ void __launch_bounds__(NW * 32, 1) TreeMmaKernel(TreeArgs a, TreeSpli
     s.tokens = a.tokens;
     s.words = a.words;
     const int last_unit = a.c.head_slots - kUnit;
-    const uint32_t ring_at = SmemAddr(ring) + group * (kStages * Warp::kStageBytes);
-    const uint8_t* ring_ptr = ring + group * (kStages * Warp::kStageBytes);
+    constexpr int kRing = kStages * kStageBytes;  // of K, then of V
+    const uint8_t* ring_ptr = ring + group * Shape::kRingBytes;
+    const uint32_t ring_at = SmemAddr(ring_ptr);
     Warp w;
     while (cur < end) {
         const Entry e = FindEntry(a, b);
@@ -952,18 +976,29 @@ __global__ void __launch_bounds__(NW * 32, 1) TreeMmaKernel(TreeArgs a, TreeSpli
 
         // ---- the ring's first units, then the Q fragments
         w.Begin(a, sp, e.seq, head);
-        int from = u0 + group;  // the unit to copy next
-        int into = 0;           // its stage
-        auto copy = [&] {
-            // the last unit of a plane may hold fewer slots: it starts earlier and leaves the others out
-            if (from < u1)
-                w.template Copy<WQ * 32>(ring_at + into, min(from * kUnit, last_unit), wq * 32 + lane);
+        // K runs half a unit ahead of V: its stage is free again once the scores are done
+        int k_from = u0 + group, v_from = k_from;  // the units to copy next
+        int k_into = 0, v_into = 0;                // their stages
+        const int id = wq * 32 + lane;
+        // the last unit of a plane may hold fewer slots: it starts earlier and leaves the others out
+        auto copy_k = [&] {
+            if (k_from < u1) w.template CopyK<WQ * 32>(ring_at + k_into, min(k_from * kUnit, last_unit), id);
             asm volatile("cp.async.commit_group;" ::: "memory");
-            from += kGroups;
-            into = into + kStageBytes == kStages * kStageBytes ? 0 : into + kStageBytes;
+            k_from += kGroups;
+            k_into = k_into + kStageBytes == kRing ? 0 : k_into + kStageBytes;
+        };
+        auto copy_v = [&] {
+            if (v_from < u1) w.template CopyV<WQ * 32>(ring_at + kRing + v_into, min(v_from * kUnit, last_unit), id);
+            asm volatile("cp.async.commit_group;" ::: "memory");
+            v_from += kGroups;
+            v_into = v_into + kStageBytes == kRing ? 0 : v_into + kStageBytes;
         };
 #pragma unroll
-        for (int k = 0; k < kStages - 1; ++k) copy();
+        for (int k = 0; k < kStages - 1; ++k) {
+            copy_k();
+            copy_v();
+        }
+        copy_k();
         for (int n = warp; n < WQ * NT; n += NW) {
             const int r = row0 + n * kRows + s.g;
             const float* q = r < sp.rows ? a.q + (size_t(b) * a.tokens + r / a.group) * a.q_stride +
@@ -983,17 +1018,23 @@ __global__ void __launch_bounds__(NW * 32, 1) TreeMmaKernel(TreeArgs a, TreeSpli
 
         // ---- the group's units
         const uint4* frags = sq + wq * NT * Warp::kFrags * 32 + lane;
-        const uint8_t* stage = ring_ptr;
-        for (int u = u0 + group; u < u1; u += kGroups) {
-            asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
-            // every copy of this unit has landed, and the stage refilled next has been read
+        // all copies but the 2 (S - 1) latest have landed, and every warp of the group is here
+        auto meet = [&] {
+            asm volatile("cp.async.wait_group %0;" ::"n"(2 * (kStages - 1)) : "memory");
             if (WQ == 1)
                 __syncwarp();
             else
                 asm volatile("bar.sync %0, %1;" ::"r"(group + 1), "n"(WQ * 32) : "memory");
-            copy();
-            if (tile < sp.rows) w.Unit(s, stage, frags, min(u * kUnit, last_unit), u * kUnit);
-            stage = stage + kStageBytes == ring_ptr + kStages * kStageBytes ? ring_ptr : stage + kStageBytes;
+        };
+        int stage = 0;
+        for (int u = u0 + group; u < u1; u += kGroups) {
+            meet();  // this unit's K is there, the last unit's V has been read
+            copy_v();
+            if (tile < sp.rows) w.Keys(s, ring_ptr + stage, frags, min(u * kUnit, last_unit), u * kUnit);
+            meet();  // its V is there, its K has been read
+            copy_k();
+            if (tile < sp.rows) w.Sum(s, ring_ptr + kRing + stage);
+            stage = stage + kStageBytes == kRing ? 0 : stage + kStageBytes;
         }
         w.End(s);
         asm volatile("cp.async.wait_group 0;" ::: "memory");
@@ -1104,9 +1145,9 @@ __global__ void __launch_bounds__(kJoinWarps * 32) TreeJoinKernel(TreeArgs a, Tr
     }
 }
 
-template <int TYPE, int NB, int NT, int WQ, int NW>
+template <int TYPE, int NB, int NT, int WQ, int NW, int PER_SM>
 bool LaunchShape(DeviceContext& ctx, const TreeArgs& a) {
-    using Shape = TreeShape<TYPE, NB, NT, WQ, NW>;
+    using Shape = TreeShape<TYPE, NB, NT, WQ, NW, PER_SM>;
     TreeSplit sp{};
     sp.rows = a.tokens * a.group;
     sp.groups = static_cast<int>(CeilDiv(sp.rows, Shape::kItemRows));
@@ -1116,11 +1157,11 @@ bool LaunchShape(DeviceContext& ctx, const TreeArgs& a) {
     const double units = double(a.batch) * double(items) * double(CeilDiv(slots, Shape::Warp::kUnit));
     if (units >= 2147483648.0 || a.c.head_slots < Shape::Warp::kUnit) return false;
     const int grid = static_cast<int>(std::min<double>(
-        ctx.sm_count, std::max(std::ceil(units / Shape::kGroups), double(a.batch) * double(items))));
+        PER_SM * ctx.sm_count, std::max(std::ceil(units / Shape::kGroups), double(a.batch) * double(items))));
     sp.parts = static_cast<float*>(
         Workspace(ctx, 2 * size_t(grid) * Shape::kItemRows * (NB * 32 + 2) * sizeof(float)));
     sp.magic = TYPE == MLB_Q8_0 ? kMagic8 : kMagic4;
-    auto* kernel = TreeMmaKernel<TYPE, NB, NT, WQ, NW>;
+    auto* kernel = TreeMmaKernel<TYPE, NB, NT, WQ, NW, PER_SM>;
     static int configured[64] = {};
     if (ctx.device >= 64 || !configured[ctx.device]) {
         CheckCuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape::kBytes),
@@ -1139,14 +1180,21 @@ bool LaunchShape(DeviceContext& ctx, const TreeArgs& a) {
 
 // Rows per KV head choose the tiles: up to 8 one tile per warp; more take two
 // per warp (the quants are converted once for both), up to four warps sharing
-// their slots.
+// their slots.  fp32 heads above 64 elements: one tile per warp, the registers
+// and the ring hold no more.
 template <int TYPE, int NB>
 bool LaunchRows(DeviceContext& ctx, const TreeArgs& a) {
     const long long rows = 1LL * a.tokens * a.group;
-    if (rows <= kRows) return LaunchShape<TYPE, NB, 1, 1, kWarps1<TYPE, NB>>(ctx, a);
-    if (rows <= 2 * kRows) return LaunchShape<TYPE, NB, 2, 1, kWarps2<TYPE, NB>>(ctx, a);
-    if (rows <= 4 * kRows) return LaunchShape<TYPE, NB, 2, 2, kWarps2<TYPE, NB>>(ctx, a);
-    return LaunchShape<TYPE, NB, 2, 4, kWarps4<TYPE, NB>>(ctx, a);
+    if constexpr (TYPE == MLB_F32 && NB > 2) {
+        if (rows <= kRows) return LaunchShape<TYPE, NB, 1, 1, 3, 2>(ctx, a);
+        if (rows <= 2 * kRows) return LaunchShape<TYPE, NB, 1, 2, 4, 2>(ctx, a);
+        return LaunchShape<TYPE, NB, 1, 4, 4, 2>(ctx, a);
+    } else {
+        if (rows <= kRows) return LaunchShape<TYPE, NB, 1, 1, 6, 2>(ctx, a);
+        if (rows <= 2 * kRows) return LaunchShape<TYPE, NB, 2, 1, 6, 2>(ctx, a);
+        if (rows <= 4 * kRows) return LaunchShape<TYPE, NB, 2, 2, 6, 2>(ctx, a);
+        return LaunchShape<TYPE, NB, 2, 4, TREE_NW4, TREE_PER4>(ctx, a);
+    }
 }
 
 template <int TYPE>
