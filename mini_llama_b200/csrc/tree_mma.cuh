@@ -291,6 +291,18 @@ __device__ __forceinline__ void CopyChunk(uint32_t to, const void* from, int byt
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
 }
 
+// Shared-memory loads by 32-bit address; volatile: they stay behind the waits.
+__device__ __forceinline__ uint32_t LoadWord(uint32_t at, int more) {
+    uint32_t v;
+    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(at + more));
+    return v;
+}
+__device__ __forceinline__ uint32_t LoadHalf(uint32_t at, int more) {
+    uint16_t v;
+    asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(at + more));
+    return v;
+}
+
 // ---------------------------------------------------------------- quantized caches
 // A warp's running result for NT tiles of rows over Q8_0 / Q4_0 slots, H steps
 // of 16 slots to a unit.
@@ -305,6 +317,7 @@ struct QuantWarp {
     static constexpr int kPitch = kXor ? 128 : (kChunks | 1) * 16;
     static constexpr int kPlane = kUnit * kPitch, kScales = kUnit * NB * 2;
     static constexpr int kStageBytes = kPlane + kScales;   // of K, and of V
+    static_assert(!kXor || kStageBytes % 128 == 0, "the chunk bits of a stage's address are free");
     static constexpr int kFrags = 2 * NB;                  // uint4 per lane and tile: (hi, hi, lo, lo)
 
     Values<NB> v[NT];
@@ -426,7 +439,8 @@ struct QuantWarp {
             uint32_t kd[2 * H][(NB + 1) / 2];
 #pragma unroll
             for (int r = 0; r < 2 * H; ++r) LoadScales<NB>(sc + 8 * r * NB, kd[r]);
-            const uint8_t* row = stage + s.g * kPitch + 4 * s.c;
+            // (with kXor the address bits of the chunk hold g, and chunk j is one exclusive or away)
+            const uint32_t row = SmemAddr(stage) + s.g * kPitch + 4 * s.c + (kXor ? s.g * 16 : 0);
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
                 uint4 q0[NT], q1[NT];
@@ -440,17 +454,17 @@ struct QuantWarp {
                     uint32_t f[2][4];
 #pragma unroll
                     for (int r = 0; r < 2; ++r) {
-                        const uint8_t* at = row + (8 * r + h * kSlots) * kPitch;
+                        const int step = (8 * r + h * kSlots) * kPitch;
                         if constexpr (TYPE == MLB_Q8_0) {
 #pragma unroll
                             for (int i = 0; i < 2; ++i) {
-                                const int chunk = kXor ? ((2 * b + i) ^ s.g) * 16 : (2 * b + i) * 16;
-                                const uint32_t w = *reinterpret_cast<const uint32_t*>(at + chunk);
+                                const int chunk = (2 * b + i) * 16;
+                                const uint32_t w = kXor ? LoadWord(row ^ chunk, step) : LoadWord(row, step + chunk);
                                 f[i][r] = EvenBytes(w, magic);
                                 f[i][2 + r] = EvenBytes(w >> 8, magic);
                             }
                         } else {
-                            const uint32_t w = *reinterpret_cast<const uint32_t*>(at + b * 16), u = w >> 8;
+                            const uint32_t w = LoadWord(row, step + b * 16), u = w >> 8;
                             f[0][r] = LowNibbles(w, magic);
                             f[0][2 + r] = LowNibbles(u, magic);
                             f[1][r] = HighNibbles(w, magic);
@@ -535,8 +549,8 @@ struct QuantWarp {
                 v[n].Scale(__shfl_sync(0xffffffffu, f, 8 * s.c), __shfl_sync(0xffffffffu, f, 8 * s.c + 4));
             }
         }
-        const uint8_t* row = stage + 2 * s.c * kPitch + (kXor ? 4 * (s.g & 3) : (kQuantBytes / 8) * s.g);
-        const int turn = ((s.g >> 2) ^ (2 * s.c)) * 16;  // chunk of the first slot in block 0
+        const uint32_t row = SmemAddr(stage) + 2 * s.c * kPitch +
+                             (kXor ? ((s.g >> 2) ^ (2 * s.c)) * 16 + 4 * (s.g & 3) : (kQuantBytes / 8) * s.g);
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
             float t[NT][2][4];
@@ -545,11 +559,11 @@ struct QuantWarp {
                 uint32_t f[2][4];
 #pragma unroll
                 for (int r = 0; r < 2; ++r) {  // slots 2c, 2c + 1, then + 8
-                    const uint8_t* at = row + (8 * r + h * kSlots) * kPitch + (kXor ? 0 : b * kQuantBytes);
+                    const int step = (8 * r + h * kSlots) * kPitch, chunk = b * kQuantBytes;
                     if constexpr (TYPE == MLB_Q8_0) {
-                        const int o0 = kXor ? turn ^ (32 * b) : 0, o1 = kXor ? turn ^ (32 * b + 16) : 0;
-                        const uint32_t w0 = *reinterpret_cast<const uint32_t*>(at + o0);
-                        const uint32_t w1 = *reinterpret_cast<const uint32_t*>(at + kPitch + o1);
+                        const uint32_t w0 = kXor ? LoadWord(row ^ chunk, step) : LoadWord(row, step + chunk);
+                        const uint32_t w1 = kXor ? LoadWord(row ^ (chunk + 16), step + kPitch)
+                                                 : LoadWord(row, step + chunk + kPitch);
                         // bytes of the two slots side by side
                         const uint32_t low2 = __byte_perm(w0, w1, 0x5410), high2 = __byte_perm(w0, w1, 0x7632);
                         f[0][2 * r] = EvenBytes(low2, magic);
@@ -557,8 +571,7 @@ struct QuantWarp {
                         f[1][2 * r] = EvenBytes(high2, magic);
                         f[1][2 * r + 1] = EvenBytes(high2 >> 8, magic);
                     } else {
-                        const uint32_t w = *reinterpret_cast<const unsigned short*>(at) |
-                                           (uint32_t(*reinterpret_cast<const unsigned short*>(at + kPitch)) << 16);
+                        const uint32_t w = LoadHalf(row, step + chunk) | (LoadHalf(row, step + chunk + kPitch) << 16);
                         const uint32_t u = w >> 8;
                         f[0][2 * r] = LowNibbles(w, magic);
                         f[0][2 * r + 1] = LowNibbles(u, magic);
@@ -919,7 +932,7 @@ __global__ void __launch_bounds__(NW * 32, PER_SM) TreeMmaKernel(TreeArgs a, Tre
     constexpr int kPitch = Shape::kPitch, kFours = NB * 8, kItemRows = Shape::kItemRows, kStages = Shape::kStages;
     constexpr int kUnit = Warp::kUnit, kStageBytes = Warp::kStageBytes;
     constexpr unsigned kGroups = Shape::kGroups;
-    extern __shared__ uint4 smem4[];
+    extern __shared__ __align__(128) uint4 smem4[];
     uint8_t* ring = reinterpret_cast<uint8_t*>(smem4);
     float* so = reinterpret_cast<float*>(smem4);                 // join: [NW][8 NT][kPitch]
     float* sm = so + NW * Shape::kRowsOf * kPitch;               // [NW][8 NT]
