@@ -86,6 +86,7 @@ __global__ void __launch_bounds__(kRowWarps * 32) TreeRowKernel(TreeArgs a) {
 // of a unit or more.
 bool LaunchTreeMma(DeviceContext& ctx, const TreeArgs& a) {
     if (a.c.type == MLB_F32) return a.cache_vec && LaunchTreeF32(ctx, a);
+    if (1LL * a.tokens * a.group > 32 && LaunchTreeTc(ctx, a)) return true;
     return a.c.type == MLB_Q8_0 ? LaunchTreeQ80(ctx, a) : LaunchTreeQ40(ctx, a);
 }
 

@@ -52,5 +52,7 @@ __device__ __forceinline__ bool SeesDraft(const uint64_t* bits, int t, int j) {
 bool LaunchTreeF32(DeviceContext& ctx, const TreeArgs& a);
 bool LaunchTreeQ80(DeviceContext& ctx, const TreeArgs& a);
 bool LaunchTreeQ40(DeviceContext& ctx, const TreeArgs& a);
+// The tensor-memory kernel (tree_tc.cu) for many rows over quantized caches.
+bool LaunchTreeTc(DeviceContext& ctx, const TreeArgs& a);
 
 }  // namespace mlb

@@ -530,10 +530,10 @@ struct QuantWarp {
                     if (edge) {  // a slot that is not seen may hold any scale, NaN too
                         const uint32_t see = __hne2_mask(AsHalf2(ph[n][h][i]), AsHalf2(0u));
 #pragma unroll
-                        for (int b = 0; b < NB; ++b) big = __hmax2(big, AsHalf2(d[h][i][b] & see));
+                        for (int b = 0; b < NB; ++b) big = __hmax2(big, __habs2(AsHalf2(d[h][i][b] & see)));
                     } else if (n == 0) {
 #pragma unroll
-                        for (int b = 0; b < NB; ++b) big = __hmax2(big, AsHalf2(d[h][i][b]));
+                        for (int b = 0; b < NB; ++b) big = __hmax2(big, __habs2(AsHalf2(d[h][i][b])));
                     }
                 }
             if (n > 0 && !edge) big = AsHalf2(all);

@@ -1,0 +1,686 @@
+// Attention of many drafted rows over a quantized cache on the 5th-generation
+// tensor cores (tcgen05): more than 32 rows per KV head, where the matrix work
+// of the warp-level kernel (tree_mma.cuh) outgrows the cache's bytes.
+//
+// An item is 128 query rows (tokens x query heads of one KV head, zeros past
+// their end) against a stretch of the cache, 128 slots to a tile:
+//   S = Q K^T     128 x 128, three MMA products: K = d q is exact as fp16 hi + lo
+//                 (19 bits: hi = rn(d q), lo = fma(d, q, -hi); fp16(d) is a
+//                 multiple of 2^-24, so subnormal scales too), Q is scaled per row
+//                 by a power of two and split into hi + lo (22 bits), the lo lo
+//                 product is dropped (2^-22)
+//   softmax       a row's running maximum m, moved when a score passes it by 2^2;
+//                 weights 2^(x - m + 12) <= 2^14 as fp16 hi + lo, written over the
+//                 scores in tensor memory
+//   O = P V       128 x head_dim, A from tensor memory, V = hi + lo as K, stored as it
+//                 lies in the cache (the N side contiguous); a fresh accumulator per
+//                 tile, added to the running rows in registers in fp32 (the matrix
+//                 unit's own sums truncate)
+// A tile with a scale of 2^8 or more (|value| could pass fp16's range) is taken
+// times 2^-9, undone in fp32.  Slots that only some rows see may hold any bytes:
+// K touches its own column only; a V scale that is not finite in a drafted slot
+// becomes 0 and the rows that see it NaN in that block.
+//
+// Bound: the MMAs, 6 x 128 x 128 x head_dim multiply-adds a tile.  Four
+// warpgroups, one CTA per SM, launched with 128 registers a thread and split
+// 168 + 168 + 104 + 72 between them; roles by warp:
+//   0-7    softmax and accumulation: row = lane of tensor memory, two threads to a
+//          row (64 slots, half of head_dim each)
+//   8-11   producers: thread = slot; the row's quants in registers a tile ahead,
+//          converted into the operand images (no swizzle: 16-byte chunks of eight
+//          elements, chunk c of row r at 2048 c + 16 r)
+//   12     tensor memory (13-15 idle); one lane issues all MMAs: QK(i + 1) before PV(i), so that
+//          the tensor pipe works while the softmax of tile i + 1 and the conversion of
+//          the next tiles run
+// Scores have three buffers in tensor memory (PV(i) still reads its weights when
+// QK(i + 2) starts), O one.  The cut of the items over the CTAs and the joining
+// of cut items are those of tree_mma.cuh.  Every wait is bounded; an expired one
+// sets the device status word, every role leaves, and issued MMAs are waited for
+// before tensor memory is freed.
+#include "tree_mma.cuh"
+
+namespace mlb {
+
+namespace {
+
+constexpr int kTile = 128;       // slots of a tile and rows of an item
+constexpr int kSoftWarps = 8;    // softmax warps
+constexpr int kProdWarps = 4;    // producer warps
+constexpr int kTcWarps = kSoftWarps + kProdWarps + 4;  // the last warpgroup: one warp issues the MMAs
+constexpr int kMmaWarp = kSoftWarps + kProdWarps;
+constexpr int kScoreBufs = 3;
+constexpr int kOCol = kScoreBufs * kTile;  // tensor-memory column of O
+constexpr uint64_t kTcWait = 2000000000ull;
+constexpr int kInfoBufs = 4;     // tiles whose flags are kept
+
+struct TcTreeShared {
+    uint64_t q_full, k_full, k_empty, v_full, v_empty, o_full, o_empty, drain;
+    uint64_t soft, prod;  // meetings of the softmax and of the producer threads
+    uint64_t s_full[kScoreBufs], p_full[kScoreBufs];
+    uint32_t tmem;
+    int abort;
+    float top[2][2][kTile];  // [parity][half][row]: the largest scores of a tile
+    float sum[2][kTile];     // the largest |q|
+    float last[2][kTile];    // sums of the weights
+    uint32_t flag[2][kProdWarps];
+    int k_big[kInfoBufs], v_big[kInfoBufs], v_odd[kInfoBufs];
+    uint32_t v_bad[kInfoBufs][4][kTile / 32];  // [tile][block][slots]: scales that are not finite, drafted slots
+};
+constexpr int kTcHeaderBytes = 7168;
+static_assert(sizeof(TcTreeShared) <= kTcHeaderBytes, "header");
+
+__device__ __forceinline__ void Fail(TcTreeShared& sh, int* status) {
+    atomicCAS(status, 0, MLB_ERR_DEVICE_TIMEOUT);
+    *reinterpret_cast<volatile int*>(&sh.abort) = 1;
+}
+
+// Waits for a phase; false (status set, abort raised) when it gave up.  One
+// thread's wait, and a whole warp's, which gives all its lanes the same answer.
+__device__ __forceinline__ bool WaitOne(TcTreeShared& sh, uint64_t* bar, uint32_t parity, int* status) {
+    const volatile int* abort = &sh.abort;
+    if (MbarWaitFor(bar, parity, kTcWait, abort)) return true;
+    if (!*abort) Fail(sh, status);
+    return false;
+}
+__device__ __forceinline__ bool Wait(TcTreeShared& sh, uint64_t* bar, uint32_t parity, int* status) {
+    return __all_sync(0xffffffffu, WaitOne(sh, bar, parity, status));
+}
+
+__device__ __forceinline__ void Arrive(uint64_t* bar) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(SmemAddr(bar)) : "memory");
+}
+__device__ __forceinline__ void Commit(uint64_t* bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(SmemAddr(bar))
+                 : "memory");
+}
+__device__ __forceinline__ void FenceBefore() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void FenceAfter() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void FenceAsync() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+// A meeting of a role's warps: bounded, as every wait, so that nobody is left
+// behind when one of them gives up.
+__device__ __forceinline__ bool Meet(TcTreeShared& sh, uint64_t* bar, uint32_t& phase, int* status) {
+    Arrive(bar);
+    return Wait(sh, bar, phase++ & 1, status);
+}
+
+// Shared-memory descriptor, no swizzle: lead = bytes between the two 8-element
+// chunks of K (K-major) or between groups of 8 K (MN-major), stride = bytes
+// between groups of 8 rows (K-major) or of 8 N (MN-major).
+__device__ __forceinline__ uint64_t Descriptor(uint32_t addr, uint32_t lead, uint32_t stride) {
+    return static_cast<uint64_t>((addr >> 4) & 0x3FFFu) | (static_cast<uint64_t>((lead >> 4) & 0x3FFFu) << 16) |
+           (static_cast<uint64_t>((stride >> 4) & 0x3FFFu) << 32) | (1ull << 46);
+}
+// kind::f16, fp16 operands, fp32 accumulators, M = 128; bit 16: B is MN-major.
+__device__ __forceinline__ uint32_t Instruction(int n, bool b_mn) {
+    return (1u << 4) | (b_mn ? 1u << 16 : 0u) | (static_cast<uint32_t>(n >> 3) << 17) | (8u << 24);
+}
+
+__device__ __forceinline__ void MmaShared(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %5, %5, %5}, p;\n\t}\n" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(0));
+}
+__device__ __forceinline__ void MmaTensor(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %5, %5, %5}, p;\n\t}\n" ::"r"(d),
+        "r"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(0));
+}
+
+// 16 columns of the warp's 32 lanes.
+__device__ __forceinline__ void Load16(uint32_t at, float* v) {
+    uint32_t r[16];
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, "
+        "[%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(at));
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
+}
+__device__ __forceinline__ void Store8(uint32_t at, const uint32_t (&r)[8]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(at), "r"(r[0]),
+                 "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]));
+}
+__device__ __forceinline__ void WaitLoad() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void WaitStore() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// The items of a CTA, one after the other; every role walks them alike.
+struct Walk {
+    unsigned cur, end, first;
+    int b;
+    // of the current item
+    Entry e;
+    unsigned units;
+    int u0, u1, head, row0;
+
+    __device__ __forceinline__ bool Next(const TreeArgs& a, const TreeSplit& sp, unsigned items) {
+        while (cur < end) {
+            e = FindEntry(a, b);
+            units = (e.slots + kTile - 1) / kTile;
+            if (cur - first >= units * items) {
+                first += units * items;
+                ++b;
+                continue;
+            }
+            const unsigned item = (cur - first) / units;
+            u0 = cur - first - item * units;
+            u1 = min(u0 + (end - cur), units);
+            head = item / sp.groups;
+            row0 = (item - head * sp.groups) * kTile;
+            cur += u1 - u0;
+            return true;
+        }
+        return false;
+    }
+};
+
+// Which of the 32 slots from s0 row t sees, of `slots` slots, `len` of them committed.
+__device__ __forceinline__ uint32_t SeenBits(const uint64_t* mask, int words, int tokens, int t, int s0, int len, int slots) {
+    const int n = min(max(len - s0, 0), 32);           // committed ones
+    uint32_t seen = n == 32 ? 0xffffffffu : (1u << n) - 1;
+    const int live = min(max(slots - s0, 0), 32);      // drafted or committed
+    if (n < live && t < tokens) {
+        const int j0 = s0 + n - len;  // the first drafted token here
+        uint64_t bits;
+        if (mask) {
+            const uint64_t* row = mask + size_t(t) * words + (j0 >> 6);
+            bits = __ldg(row) >> (j0 & 63);
+            if ((j0 & 63) != 0 && (j0 >> 6) + 1 < words) bits |= __ldg(row + 1) << (64 - (j0 & 63));
+        } else {
+            bits = t >= j0 ? (t - j0 >= 63 ? ~0ull : (2ull << (t - j0)) - 1) : 0;
+        }
+        const uint32_t in = live == 32 ? 0xffffffffu : (1u << live) - 1;
+        seen |= (static_cast<uint32_t>(bits) << n) & in;
+    }
+    return seen;
+}
+
+template <int TYPE, int NB>
+struct RawRow {
+    static constexpr int kChunks = NB * (TYPE == MLB_Q8_0 ? 2 : 1);
+    uint4 q[kChunks];
+    uint32_t d[(NB + 1) / 2];
+
+    __device__ __forceinline__ void Load(const uint8_t* plane, const __half* scales, int row) {
+        const uint4* p = reinterpret_cast<const uint4*>(plane + size_t(row) * kChunks * 16);
+#pragma unroll
+        for (int i = 0; i < kChunks; ++i) q[i] = __ldg(p + i);
+        const unsigned short* h = reinterpret_cast<const unsigned short*>(scales + size_t(row) * NB);
+#pragma unroll
+        for (int i = 0; i < NB; ++i) {
+            const uint32_t v = __ldg(h + i);
+            d[i >> 1] = i & 1 ? d[i >> 1] | (v << 16) : v;
+        }
+    }
+    __device__ __forceinline__ uint32_t Scale(int b) const { return (b & 1 ? d[b >> 1] >> 16 : d[b >> 1]) & 0xffffu; }
+    __device__ __forceinline__ void Clear(int b) { d[b >> 1] &= b & 1 ? 0x0000ffffu : 0xffff0000u; }
+};
+
+// hi and lo of d times a half pair, into two words.
+__device__ __forceinline__ void Product(uint32_t pair, __half2 d, uint32_t& hi, uint32_t& lo) {
+    const __half2 h = __hmul2(AsHalf2(pair), d);
+    hi = H2(h);
+    lo = H2(__hfma2(AsHalf2(pair), d, __hneg2(h)));
+}
+
+// A row's images: within each group of four elements in the order 0, 2, 1, 3.
+template <int TYPE, int NB>
+__device__ __forceinline__ void Convert(const RawRow<TYPE, NB>& r, uint8_t* image, int slot, bool big, uint32_t magic) {
+    constexpr int kLo = NB * 32 * kTile * 2;  // of the lo image
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+        __half2 d = __half2half2(__ushort_as_half(static_cast<unsigned short>(r.Scale(b))));
+        if (big) d = __hmul2(d, AsHalf2(0x18001800u));  // 2^-9
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {  // eight elements each
+            uint32_t p[4];
+            if constexpr (TYPE == MLB_Q8_0) {
+                const uint4 q = r.q[2 * b + (c >> 1)];
+                const uint32_t w0 = c & 1 ? q.z : q.x, w1 = c & 1 ? q.w : q.y;
+                p[0] = EvenBytes(w0, magic);
+                p[1] = EvenBytes(w0 >> 8, magic);
+                p[2] = EvenBytes(w1, magic);
+                p[3] = EvenBytes(w1 >> 8, magic);
+            } else {
+                const uint4 q = r.q[b];
+                const uint32_t w0 = c & 1 ? q.z : q.x, w1 = c & 1 ? q.w : q.y;
+                p[0] = c < 2 ? LowNibbles(w0, magic) : HighNibbles(w0, magic);
+                p[1] = c < 2 ? LowNibbles(w0 >> 8, magic) : HighNibbles(w0 >> 8, magic);
+                p[2] = c < 2 ? LowNibbles(w1, magic) : HighNibbles(w1, magic);
+                p[3] = c < 2 ? LowNibbles(w1 >> 8, magic) : HighNibbles(w1 >> 8, magic);
+            }
+            uint4 hi, lo;
+            Product(p[0], d, hi.x, lo.x);
+            Product(p[1], d, hi.y, lo.y);
+            Product(p[2], d, hi.z, lo.z);
+            Product(p[3], d, hi.w, lo.w);
+            uint8_t* to = image + (4 * b + c) * 2048 + slot * 16;
+            *reinterpret_cast<uint4*>(to) = hi;
+            *reinterpret_cast<uint4*>(to + kLo) = lo;
+        }
+    }
+}
+
+template <int TYPE, int NB>
+__global__ void __launch_bounds__(kTcWarps * 32, 1) TreeTcKernel(TreeArgs a, TreeSplit sp, int* status) {
+    constexpr int HD = NB * 32, kImage = HD * kTile * 2;  // one fp16 image
+    constexpr int kHalf = HD / 2;                         // head_dim of a softmax thread
+    extern __shared__ __align__(1024) uint8_t tc_smem[];
+    TcTreeShared& sh = *reinterpret_cast<TcTreeShared*>(tc_smem);
+    uint8_t* qi = tc_smem + kTcHeaderBytes;  // hi, lo
+    uint8_t* ki = qi + 2 * kImage;
+    uint8_t* vi = ki + 2 * kImage;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const unsigned items = a.c.n_kv * sp.groups;
+
+    // entries with nothing to see
+    for (int b = blockIdx.x; b < a.batch; b += gridDim.x) {
+        if (FindEntry(a, b).slots != 0) continue;
+        for (int t = warp; t < a.tokens; t += kTcWarps)
+            for (int i = lane; i < a.n_heads * a.c.hd; i += 32)
+                a.out[(size_t(b) * a.tokens + t) * a.out_stride + i] = 0.0f;
+    }
+    GridDepLaunch();  // the joining kernel may come up as CTAs leave
+    const Cut cut(a, kTile, items, 1, gridDim.x);
+    if (cut.total == 0 || blockIdx.x >= cut.ctas) return;
+    Walk walk;
+    walk.cur = cut.Start(blockIdx.x);
+    walk.end = cut.Start(blockIdx.x + 1);
+    walk.b = cut.Find(a, kTile, items, walk.cur, walk.first);
+
+    if (threadIdx.x == 0) {
+        MbarInit(&sh.q_full, kSoftWarps * 32);
+        MbarInit(&sh.k_full, kProdWarps * 32);
+        MbarInit(&sh.v_full, kProdWarps * 32);
+        MbarInit(&sh.k_empty, 1);
+        MbarInit(&sh.v_empty, 1);
+        MbarInit(&sh.o_full, 1);
+        MbarInit(&sh.o_empty, kSoftWarps * 32);
+        MbarInit(&sh.drain, 1);
+        MbarInit(&sh.soft, kSoftWarps * 32);
+        MbarInit(&sh.prod, kProdWarps * 32);
+        for (int i = 0; i < kScoreBufs; ++i) {
+            MbarInit(&sh.s_full[i], 1);
+            MbarInit(&sh.p_full[i], kSoftWarps * 32);
+        }
+        FenceMbarInit();
+        sh.abort = 0;
+    }
+    if (warp == kMmaWarp) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(SmemAddr(&sh.tmem)));
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::);
+    }
+    FenceBefore();
+    __syncthreads();
+    FenceAfter();
+    const uint32_t tmem = sh.tmem;
+
+    if (warp < kSoftWarps) {
+        // ------------------------------------------------ softmax and accumulation
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 168;");
+        const int half = warp >> 2, row = (warp & 3) * 32 + lane;
+        const uint32_t lanes = tmem + ((static_cast<uint32_t>(warp & 3) * 32) << 16);
+        int it = 0;  // tiles so far
+        uint32_t met = 0;
+        bool ok = true;
+        while (ok && walk.Next(a, sp, items)) {
+            const int r = walk.row0 + row;
+            const bool live = r < sp.rows;
+            const int t = r / a.group;
+            float cs;
+            {  // this thread's half of the row of Q
+                const float* q = live ? a.q + (size_t(walk.b) * a.tokens + t) * a.q_stride +
+                                            size_t(walk.head * a.group + r % a.group) * a.c.hd
+                                      : nullptr;
+                float x[kHalf], top = 0.0f;
+#pragma unroll
+                for (int i = 0; i < kHalf; i += 4) {
+                    const int d = half * kHalf + i;
+                    if (a.q_vec) {
+                        const float4 w = q && d < a.c.hd ? __ldg(reinterpret_cast<const float4*>(q + d))
+                                                         : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                        x[i] = w.x;
+                        x[i + 1] = w.y;
+                        x[i + 2] = w.z;
+                        x[i + 3] = w.w;
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) x[i + j] = q && d + j < a.c.hd ? __ldg(q + d + j) : 0.0f;
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < kHalf; ++i) top = fmaxf(top, fabsf(x[i]));
+                // (its own words: the tiles' maxima of the last item may still be read)
+                sh.sum[half][row] = top;
+                if (!(ok = Meet(sh, &sh.soft, met, status))) break;
+                top = fmaxf(sh.sum[0][row], sh.sum[1][row]);
+                const int up = ScaleExp(top);
+                const float sc = Pow2(up);
+                cs = fmaxf(Pow2(-up) * a.scale * kLog2e, 1e-37f);
+#pragma unroll
+                for (int i = 0; i < kHalf; i += 8) {
+                    uint4 hi, lo;
+                    SplitHalf(x[i] * sc, x[i + 2] * sc, hi.x, lo.x);
+                    SplitHalf(x[i + 1] * sc, x[i + 3] * sc, hi.y, lo.y);
+                    SplitHalf(x[i + 4] * sc, x[i + 6] * sc, hi.z, lo.z);
+                    SplitHalf(x[i + 5] * sc, x[i + 7] * sc, hi.w, lo.w);
+                    uint8_t* to = qi + (half * kHalf + i) / 8 * 2048 + row * 16;
+                    *reinterpret_cast<uint4*>(to) = hi;
+                    *reinterpret_cast<uint4*>(to + kImage) = lo;
+                }
+                FenceAsync();
+                Arrive(&sh.q_full);
+            }
+            float o[kHalf], m = kStart, l = 0.0f, m_of_o = kStart, m_last = kStart;
+            uint32_t poison = 0;
+#pragma unroll
+            for (int i = 0; i < kHalf; ++i) o[i] = 0.0f;
+            const uint64_t* mask = a.mask ? a.mask + size_t(walk.b) * a.tokens * a.words : nullptr;
+
+            // adds O of the item's tile u (running number n) to the row
+            auto add = [&](int u, int n) {
+                if (!Wait(sh, &sh.o_full, n & 1, status)) return false;
+                FenceAfter();
+                const float keep = Exp2(m_of_o - m_last);
+                m_of_o = m_last;
+                const float times = sh.v_big[n % kInfoBufs] ? 512.0f : 1.0f;
+#pragma unroll
+                for (int i = 0; i < kHalf; i += 16) {
+                    float d[16];
+                    Load16(lanes + kOCol + half * kHalf + i, d);
+                    WaitLoad();
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) o[i + j] = fmaf(o[i + j], keep, d[j] * times);
+                }
+                if (sh.v_odd[n % kInfoBufs]) {
+#pragma unroll
+                    for (int k = 0; k < kTile / 32; ++k) {
+                        const uint32_t seen = SeenBits(mask, a.words, a.tokens, t, u * kTile + 32 * k, walk.e.len, walk.e.slots);
+                        for (int b = 0; b < NB; ++b)
+                            if (seen & sh.v_bad[n % kInfoBufs][b][k]) poison |= 1u << b;
+                    }
+                }
+                FenceBefore();
+                Arrive(&sh.o_empty);
+                return true;
+            };
+
+            for (int u = walk.u0; u < walk.u1; ++u, ++it) {
+                const uint32_t buf = lanes + (it % kScoreBufs) * kTile;
+                if (!(ok = Wait(sh, &sh.s_full[it % kScoreBufs], (it / kScoreBufs) & 1, status))) break;
+                FenceAfter();
+                float x[64];
+#pragma unroll
+                for (int i = 0; i < 64; i += 16) Load16(buf + half * 64 + i, x + i);
+                WaitLoad();
+                const float c = sh.k_big[it % kInfoBufs] ? cs * 512.0f : cs;
+                if ((u + 1) * kTile > walk.e.len) {
+#pragma unroll
+                    for (int k = 0; k < 2; ++k) {
+                        const uint32_t seen = SeenBits(mask, a.words, a.tokens, t, u * kTile + half * 64 + 32 * k, walk.e.len,
+                                                       walk.e.slots);
+#pragma unroll
+                        for (int i = 0; i < 32; ++i)
+                            if (!((seen >> i) & 1)) x[32 * k + i] = -INFINITY;
+                    }
+                }
+                float top = x[0];
+#pragma unroll
+                for (int i = 1; i < 64; ++i) top = fmaxf(top, x[i]);
+                sh.top[it & 1][half][row] = top;
+                FenceBefore();
+                // both halves of the row are in registers: their columns are free for the weights
+                if (!(ok = Meet(sh, &sh.soft, met, status))) break;
+                FenceAfter();
+                top = fmaxf(top, sh.top[it & 1][half ^ 1][row]) * c;
+                if (top > m + kLag) {
+                    l *= Exp2(m - top);
+                    m = top;
+                }
+                const float off = kOffset - m;
+#pragma unroll
+                for (int i = 0; i < 64; i += 16) {
+                    uint32_t hi[8], lo[8];
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        const float p0 = Exp2(fmaf(x[i + 2 * j], c, off)), p1 = Exp2(fmaf(x[i + 2 * j + 1], c, off));
+                        l += p0 + p1;
+                        SplitHalf(p0, p1, hi[j], lo[j]);
+                    }
+                    Store8(buf + half * 32 + i / 2, hi);
+                    Store8(buf + 64 + half * 32 + i / 2, lo);
+                }
+                WaitStore();
+                FenceBefore();
+                Arrive(&sh.p_full[it % kScoreBufs]);
+                if (u > walk.u0 && !(ok = add(u - 1, it - 1))) break;
+                m_last = m;
+            }
+            ok = ok && add(walk.u1 - 1, it - 1);
+            if (!ok) break;
+            // ---- the row's result, or its part of it
+            sh.last[half][row] = l;
+            if (!(ok = Meet(sh, &sh.soft, met, status))) break;
+            l = sh.last[0][row] + sh.last[1][row];
+            if (live) {
+#pragma unroll
+                for (int i = 0; i < kHalf; ++i)
+                    if ((poison >> ((half * kHalf + i) / 32)) & 1) o[i] = NAN;
+                if (walk.u0 == 0 && walk.u1 == int(walk.units)) {
+                    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+                    float* out = OutRow(a, walk.b, walk.head, r);
+#pragma unroll
+                    for (int i = 0; i < kHalf; i += 4)  // back from the order 0, 2, 1, 3
+                        StoreOut(a, out, half * kHalf + i, make_float4(o[i] * inv, o[i + 2] * inv, o[i + 1] * inv, o[i + 3] * inv));
+                } else {
+                    float* part = sp.parts + (2 * size_t(blockIdx.x) + (walk.u0 == 0 ? 1 : 0)) * (size_t(kTile) * (HD + 2));
+#pragma unroll
+                    for (int i = 0; i < kHalf; i += 4)
+                        __stcg(reinterpret_cast<float4*>(part + row * HD + half * kHalf + i),
+                               make_float4(o[i], o[i + 2], o[i + 1], o[i + 3]));
+                    if (half == 0) {
+                        __stcg(part + kTile * HD + row, m);
+                        __stcg(part + kTile * (HD + 1) + row, l);
+                    }
+                }
+            }
+            __syncwarp();
+        }
+    } else if (warp < kSoftWarps + kProdWarps) {
+        // ------------------------------------------------ producers
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
+        const int slot = threadIdx.x - kSoftWarps * 32;
+        int kt = 0, vt = 0;  // tiles of K and V so far
+        uint32_t met = 0;
+        bool ok = true;
+        // what the producers' `bits` hold together
+        auto together = [&](uint32_t bits) {
+            bits = __reduce_or_sync(0xffffffffu, bits);
+            const uint32_t side = met & 1;
+            if (lane == 0) sh.flag[side][slot / 32] = bits;
+            ok = Meet(sh, &sh.prod, met, status);
+            return sh.flag[side][0] | sh.flag[side][1] | sh.flag[side][2] | sh.flag[side][3];
+        };
+        while (ok && walk.Next(a, sp, items)) {
+            const long long base = a.c.Row(walk.e.seq, a.layer, walk.head, 0);
+            constexpr int kRowBytes = RawRow<TYPE, NB>::kChunks * 16;
+            const uint8_t* kp = static_cast<const uint8_t*>(a.c.k) + base * kRowBytes;
+            const uint8_t* vp = static_cast<const uint8_t*>(a.c.v) + base * kRowBytes;
+            const __half *ks = a.c.ks + base * NB, *vs = a.c.vs + base * NB;
+            RawRow<TYPE, NB> rk, rv;
+            auto load = [&](RawRow<TYPE, NB>& r, const uint8_t* plane, const __half* scales, int u) {
+                const int at = u * kTile + slot;
+                r.Load(plane, scales, min(at, a.c.head_slots - 1));
+                if (at >= walk.e.slots)
+#pragma unroll
+                    for (int i = 0; i < (NB + 1) / 2; ++i) r.d[i] = 0;
+            };
+            auto big_scale = [&](const RawRow<TYPE, NB>& r) {
+                bool big = false;
+#pragma unroll
+                for (int b = 0; b < NB; ++b) big = big || (r.Scale(b) & 0x7fffu) >= 0x5C00u;  // 2^8, infinity, NaN
+                return big;
+            };
+            auto put_k = [&](int u) {
+                const bool big = together(big_scale(rk)) != 0;
+                if (!ok) return;
+                if (kt > 0 && !(ok = Wait(sh, &sh.k_empty, (kt - 1) & 1, status))) return;
+                if (slot == 0) sh.k_big[kt % kInfoBufs] = big;
+                Convert<TYPE, NB>(rk, ki, slot, big, sp.magic);
+                FenceAsync();
+                Arrive(&sh.k_full);
+                ++kt;
+                if (u + 1 < walk.u1) load(rk, kp, ks, u + 1);
+            };
+            auto put_v = [&](int u) {
+                // a drafted slot's scale that is not finite is taken out and noted
+                uint32_t odd = 0;
+#pragma unroll
+                for (int b = 0; b < NB; ++b)
+                    if ((rv.Scale(b) & 0x7C00u) == 0x7C00u && u * kTile + slot >= walk.e.len) {
+                        odd |= 1u << b;
+                        rv.Clear(b);
+                    }
+                const uint32_t flags = together((big_scale(rv) ? 1u : 0u) | (odd ? 2u : 0u));
+                if (!ok) return;
+                const bool big = flags & 1, any = flags & 2;
+                if (vt > 0 && !(ok = Wait(sh, &sh.v_empty, (vt - 1) & 1, status))) return;
+                if (any)
+                    for (int b = 0; b < NB; ++b) {
+                        const uint32_t bits = __ballot_sync(0xffffffffu, (odd >> b) & 1);
+                        if (lane == 0) sh.v_bad[vt % kInfoBufs][b][slot / 32] = bits;
+                    }
+                if (slot == 0) {
+                    sh.v_big[vt % kInfoBufs] = big;
+                    sh.v_odd[vt % kInfoBufs] = any;
+                }
+                Convert<TYPE, NB>(rv, vi, slot, big, sp.magic);
+                FenceAsync();
+                Arrive(&sh.v_full);
+                ++vt;
+                if (u + 1 < walk.u1) load(rv, vp, vs, u + 1);
+            };
+            load(rk, kp, ks, walk.u0);
+            load(rv, vp, vs, walk.u0);
+            put_k(walk.u0);
+            for (int u = walk.u0; ok && u < walk.u1; ++u) {
+                if (u + 1 < walk.u1) put_k(u + 1);
+                if (ok) put_v(u);
+            }
+        }
+    } else {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+    }
+    if (warp == kMmaWarp && lane == 0) {
+        // ------------------------------------------------ MMA issue
+        const uint32_t qk = Instruction(kTile, false), pv = Instruction(HD, true);
+        // K-major images: chunks of K 2048 bytes apart, groups of 8 rows 128
+        const uint64_t qd = Descriptor(SmemAddr(qi), 2048, 128), kd = Descriptor(SmemAddr(ki), 2048, 128);
+        // V: groups of 8 slots 128 bytes apart, groups of 8 of head_dim 2048
+        const uint64_t vd = Descriptor(SmemAddr(vi), 128, 2048);
+        constexpr uint64_t kLoStep = kImage >> 4, kKStep = 4096 >> 4, kVStep = 256 >> 4;
+        int it = 0, item = 0;
+        bool ok = true;
+        auto values = [&](int n) {  // PV of running tile n
+            if (!WaitOne(sh, &sh.v_full, n & 1, status) || !WaitOne(sh, &sh.p_full[n % kScoreBufs], (n / kScoreBufs) & 1, status))
+                return false;
+            // the last O has been read (so its weights' buffer, two scores back, is free too)
+            if (n > 0 && !WaitOne(sh, &sh.o_empty, (n - 1) & 1, status)) return false;
+            FenceAfter();
+            const uint32_t p = tmem + (n % kScoreBufs) * kTile;
+#pragma unroll
+            for (int s = 0; s < kTile / 16; ++s) MmaTensor(tmem + kOCol, p + 64 + 8 * s, vd + s * kVStep, pv, s != 0);
+#pragma unroll
+            for (int s = 0; s < kTile / 16; ++s) MmaTensor(tmem + kOCol, p + 8 * s, vd + kLoStep + s * kVStep, pv, 1);
+#pragma unroll
+            for (int s = 0; s < kTile / 16; ++s) MmaTensor(tmem + kOCol, p + 8 * s, vd + s * kVStep, pv, 1);
+            Commit(&sh.v_empty);
+            Commit(&sh.o_full);
+            return true;
+        };
+        while (ok && walk.Next(a, sp, items)) {
+            if (!(ok = WaitOne(sh, &sh.q_full, item & 1, status))) break;
+            ++item;
+            for (int u = walk.u0; u < walk.u1; ++u, ++it) {
+                if (!(ok = WaitOne(sh, &sh.k_full, it & 1, status))) break;
+                FenceAfter();
+                const uint32_t d = tmem + (it % kScoreBufs) * kTile;
+#pragma unroll
+                for (int s = 0; s < HD / 16; ++s) MmaShared(d, qd + kLoStep + s * kKStep, kd + s * kKStep, qk, s != 0);
+#pragma unroll
+                for (int s = 0; s < HD / 16; ++s) MmaShared(d, qd + s * kKStep, kd + kLoStep + s * kKStep, qk, 1);
+#pragma unroll
+                for (int s = 0; s < HD / 16; ++s) MmaShared(d, qd + s * kKStep, kd + s * kKStep, qk, 1);
+                Commit(&sh.k_empty);
+                Commit(&sh.s_full[it % kScoreBufs]);
+                if (u > walk.u0 && !(ok = values(it - 1))) {
+                    ++it;
+                    break;
+                }
+            }
+            if (ok) ok = values(it - 1);
+        }
+        // every MMA issued has finished before tensor memory is freed
+        Commit(&sh.drain);
+        if (!MbarWaitFor(&sh.drain, 0, kTcWait, nullptr)) Fail(sh, status);
+    }
+    FenceBefore();
+    __syncthreads();
+    if (warp == kMmaWarp) {
+        FenceAfter();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
+    }
+}
+
+template <int TYPE, int NB>
+bool LaunchTc(DeviceContext& ctx, const TreeArgs& a) {
+    TreeSplit sp{};
+    sp.rows = a.tokens * a.group;
+    sp.groups = static_cast<int>(CeilDiv(sp.rows, kTile));
+    const unsigned long long items = 1ull * a.c.n_kv * sp.groups;
+    const long long slots = std::min<long long>(1LL * std::min(a.max_len, a.c.max_seq) + a.tokens, a.c.max_seq);
+    const double units = double(a.batch) * double(items) * double(CeilDiv(slots, kTile));
+    if (units >= 2147483648.0) return false;
+    const int grid = static_cast<int>(std::min<double>(ctx.sm_count, units));
+    sp.parts = static_cast<float*>(Workspace(ctx, 2 * size_t(grid) * kTile * (NB * 32 + 2) * sizeof(float)));
+    sp.magic = TYPE == MLB_Q8_0 ? kMagic8 : kMagic4;
+    constexpr int kBytes = kTcHeaderBytes + 6 * NB * 32 * kTile * 2;
+    auto* kernel = TreeTcKernel<TYPE, NB>;
+    static int configured[64] = {};
+    if (ctx.device >= 64 || !configured[ctx.device]) {
+        CheckCuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kBytes),
+                  "cudaFuncSetAttribute(TreeTcKernel)");
+        if (ctx.device < 64) configured[ctx.device] = 1;
+    }
+    kernel<<<grid, kTcWarps * 32, kBytes, ctx.stream>>>(a, sp, ctx.status);
+    CheckCuda(cudaGetLastError(), "TreeTcKernel");
+    if (grid == 1) return true;  // nothing is cut
+    const int all = a.batch * static_cast<int>(items);
+    const int per_item = std::max(1, std::min(kTile / kJoinWarps, 4 * ctx.sm_count / all));
+    Launch("TreeJoinKernel", TreeJoinKernel<NB>, dim3(all, per_item), dim3(kJoinWarps * 32), 0, ctx.stream, true, a, sp,
+           int(kTile), 1, int(kTile), grid);
+    return true;
+}
+
+template <int TYPE>
+bool LaunchTcBlocks(DeviceContext& ctx, const TreeArgs& a) {
+    switch (a.c.blocks) {
+        case 1: return LaunchTc<TYPE, 1>(ctx, a);
+        case 2: return LaunchTc<TYPE, 2>(ctx, a);
+        case 3: return LaunchTc<TYPE, 3>(ctx, a);
+        case 4: return LaunchTc<TYPE, 4>(ctx, a);
+        default: return false;
+    }
+}
+
+}  // namespace
+
+bool LaunchTreeTc(DeviceContext& ctx, const TreeArgs& a) {
+    if (a.c.type == MLB_F32) return false;
+    return a.c.type == MLB_Q8_0 ? LaunchTcBlocks<MLB_Q8_0>(ctx, a) : LaunchTcBlocks<MLB_Q4_0>(ctx, a);
+}
+
+}  // namespace mlb
