@@ -10,8 +10,7 @@
 //                 by a power of two and split into hi + lo (22 bits), the lo lo
 //                 product is dropped (2^-22)
 //   softmax       a row's running maximum m, moved when a score passes it by 2^2;
-//                 weights 2^(x - m + 12) <= 2^14 as fp16 hi + lo, written over the
-//                 scores in tensor memory
+//                 weights 2^(x - m + 12) <= 2^14 as fp16 hi + lo, into tensor memory
 //   O = P V       128 x head_dim, A from tensor memory, V = hi + lo as K, stored as it
 //                 lies in the cache (the N side contiguous); a fresh accumulator per
 //                 tile, added to the running rows in registers in fp32 (the matrix
@@ -21,22 +20,23 @@
 // K touches its own column only; a V scale that is not finite in a drafted slot
 // becomes 0 and the rows that see it NaN in that block.
 //
-// Bound: the MMAs, 6 x 128 x 128 x head_dim multiply-adds a tile.  Four
-// warpgroups, one CTA per SM, launched with 128 registers a thread and split
-// 168 + 168 + 104 + 72 between them; roles by warp:
+// Bound: the MMAs, 6 x 128 x 128 x head_dim multiply-adds a tile (64 cycles for
+// 128 x 128 x 16), and the shared memory that they, the images' stores and the
+// other loads share.  One CTA per SM, roles by warp:
 //   0-7    softmax and accumulation: row = lane of tensor memory, two threads to a
-//          row (64 slots, half of head_dim each)
+//          row (64 slots, half of head_dim each); scores are read twice, for the
+//          maximum and for the weights, so that a thread holds 16 at a time
 //   8-11   producers: thread = slot; the row's quants in registers a tile ahead,
 //          converted into the operand images (no swizzle: 16-byte chunks of eight
 //          elements, chunk c of row r at 2048 c + 16 r)
-//   12     tensor memory (13-15 idle); one lane issues all MMAs: QK(i + 1) before PV(i), so that
-//          the tensor pipe works while the softmax of tile i + 1 and the conversion of
-//          the next tiles run
-// Scores have three buffers in tensor memory (PV(i) still reads its weights when
-// QK(i + 2) starts), O one.  The cut of the items over the CTAs and the joining
-// of cut items are those of tree_mma.cuh.  Every wait is bounded; an expired one
-// sets the device status word, every role leaves, and issued MMAs are waited for
-// before tensor memory is freed.
+//   12     tensor memory; one lane issues all MMAs: QK(i + 1) before PV(i), so that
+//          the tensor pipe works while the weights of tile i + 1 and the images of
+//          the next tiles are made
+// Tensor memory: two buffers of scores, one of weights (free again when its PV is
+// done) and one O.  The cut of the items over the CTAs and the joining of cut
+// items are those of tree_mma.cuh.  Every wait is bounded; an expired one sets the
+// device status word, every role leaves, and issued MMAs are waited for before
+// tensor memory is freed.
 #include "tree_mma.cuh"
 
 namespace mlb {
@@ -46,17 +46,16 @@ namespace {
 constexpr int kTile = 128;       // slots of a tile and rows of an item
 constexpr int kSoftWarps = 8;    // softmax warps
 constexpr int kProdWarps = 4;    // producer warps
-constexpr int kTcWarps = kSoftWarps + kProdWarps + 4;  // the last warpgroup: one warp issues the MMAs
 constexpr int kMmaWarp = kSoftWarps + kProdWarps;
-constexpr int kScoreBufs = 3;
-constexpr int kOCol = kScoreBufs * kTile;  // tensor-memory column of O
+constexpr int kTcWarps = kMmaWarp + 1;
+constexpr int kPCol = 2 * kTile, kOCol = 3 * kTile;  // tensor-memory columns of the weights and of O
 constexpr uint64_t kTcWait = 2000000000ull;
 constexpr int kInfoBufs = 4;     // tiles whose flags are kept
 
 struct TcTreeShared {
     uint64_t q_full, k_full, k_empty, v_full, v_empty, o_full, o_empty, drain;
     uint64_t soft, prod;  // meetings of the softmax and of the producer threads
-    uint64_t s_full[kScoreBufs], p_full[kScoreBufs];
+    uint64_t p_full, s_full[2], s_empty[2];
     uint32_t tmem;
     int abort;
     float top[2][2][kTile];  // [parity][half][row]: the largest scores of a tile
@@ -302,9 +301,10 @@ __global__ void __launch_bounds__(kTcWarps * 32, 1) TreeTcKernel(TreeArgs a, Tre
         MbarInit(&sh.drain, 1);
         MbarInit(&sh.soft, kSoftWarps * 32);
         MbarInit(&sh.prod, kProdWarps * 32);
-        for (int i = 0; i < kScoreBufs; ++i) {
+        MbarInit(&sh.p_full, kSoftWarps * 32);
+        for (int i = 0; i < 2; ++i) {
             MbarInit(&sh.s_full[i], 1);
-            MbarInit(&sh.p_full[i], kSoftWarps * 32);
+            MbarInit(&sh.s_empty[i], kSoftWarps * 32);
         }
         FenceMbarInit();
         sh.abort = 0;
@@ -320,7 +320,6 @@ __global__ void __launch_bounds__(kTcWarps * 32, 1) TreeTcKernel(TreeArgs a, Tre
 
     if (warp < kSoftWarps) {
         // ------------------------------------------------ softmax and accumulation
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 168;");
         const int half = warp >> 2, row = (warp & 3) * 32 + lane;
         const uint32_t lanes = tmem + ((static_cast<uint32_t>(warp & 3) * 32) << 16);
         int it = 0;  // tiles so far
@@ -380,23 +379,24 @@ __global__ void __launch_bounds__(kTcWarps * 32, 1) TreeTcKernel(TreeArgs a, Tre
             for (int i = 0; i < kHalf; ++i) o[i] = 0.0f;
             const uint64_t* mask = a.mask ? a.mask + size_t(walk.b) * a.tokens * a.words : nullptr;
 
-            // adds O of the item's tile u (running number n) to the row
+            // adds O of the item's tile u (running number n, complete) to the row
             auto add = [&](int u, int n) {
-                if (!Wait(sh, &sh.o_full, n & 1, status)) return false;
-                FenceAfter();
                 const float keep = Exp2(m_of_o - m_last);
                 m_of_o = m_last;
-                const float times = sh.v_big[n % kInfoBufs] ? 512.0f : 1.0f;
+                const bool big = sh.v_big[n % kInfoBufs];
 #pragma unroll
                 for (int i = 0; i < kHalf; i += 16) {
                     float d[16];
                     Load16(lanes + kOCol + half * kHalf + i, d);
                     WaitLoad();
+                    if (big)
 #pragma unroll
-                    for (int j = 0; j < 16; ++j) o[i + j] = fmaf(o[i + j], keep, d[j] * times);
+                        for (int j = 0; j < 16; ++j) d[j] *= 512.0f;
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) o[i + j] = fmaf(o[i + j], keep, d[j]);
                 }
                 if (sh.v_odd[n % kInfoBufs]) {
-#pragma unroll
+#pragma unroll 1
                     for (int k = 0; k < kTile / 32; ++k) {
                         const uint32_t seen = SeenBits(mask, a.words, a.tokens, t, u * kTile + 32 * k, walk.e.len, walk.e.slots);
                         for (int b = 0; b < NB; ++b)
@@ -405,62 +405,73 @@ __global__ void __launch_bounds__(kTcWarps * 32, 1) TreeTcKernel(TreeArgs a, Tre
                 }
                 FenceBefore();
                 Arrive(&sh.o_empty);
-                return true;
             };
 
             for (int u = walk.u0; u < walk.u1; ++u, ++it) {
-                const uint32_t buf = lanes + (it % kScoreBufs) * kTile;
-                if (!(ok = Wait(sh, &sh.s_full[it % kScoreBufs], (it / kScoreBufs) & 1, status))) break;
+                const uint32_t scores = lanes + (it & 1) * kTile + half * 64;
+                if (!(ok = Wait(sh, &sh.s_full[it & 1], (it >> 1) & 1, status))) break;
                 FenceAfter();
-                float x[64];
+                uint32_t seen[2] = {0xffffffffu, 0xffffffffu};
+                const bool edge = (u + 1) * kTile > walk.e.len;
+                if (edge)
 #pragma unroll
-                for (int i = 0; i < 64; i += 16) Load16(buf + half * 64 + i, x + i);
-                WaitLoad();
-                const float c = sh.k_big[it % kInfoBufs] ? cs * 512.0f : cs;
-                if ((u + 1) * kTile > walk.e.len) {
+                    for (int k = 0; k < 2; ++k)
+                        seen[k] = SeenBits(mask, a.words, a.tokens, t, u * kTile + half * 64 + 32 * k, walk.e.len, walk.e.slots);
+                auto hide = [&](float (&x)[16], int i) {
+                    if (edge)
 #pragma unroll
-                    for (int k = 0; k < 2; ++k) {
-                        const uint32_t seen = SeenBits(mask, a.words, a.tokens, t, u * kTile + half * 64 + 32 * k, walk.e.len,
-                                                       walk.e.slots);
+                        for (int j = 0; j < 16; ++j)
+                            if (!((seen[i >> 5] >> ((i & 31) + j)) & 1)) x[j] = -INFINITY;
+                };
+                float top = -INFINITY;
 #pragma unroll
-                        for (int i = 0; i < 32; ++i)
-                            if (!((seen >> i) & 1)) x[32 * k + i] = -INFINITY;
-                    }
+                for (int i = 0; i < 64; i += 16) {
+                    float x[16];
+                    Load16(scores + i, x);
+                    WaitLoad();
+                    hide(x, i);
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) top = fmaxf(top, x[j]);
                 }
-                float top = x[0];
-#pragma unroll
-                for (int i = 1; i < 64; ++i) top = fmaxf(top, x[i]);
                 sh.top[it & 1][half][row] = top;
-                FenceBefore();
-                // both halves of the row are in registers: their columns are free for the weights
                 if (!(ok = Meet(sh, &sh.soft, met, status))) break;
-                FenceAfter();
+                const float c = sh.k_big[it % kInfoBufs] ? cs * 512.0f : cs;
                 top = fmaxf(top, sh.top[it & 1][half ^ 1][row]) * c;
                 if (top > m + kLag) {
                     l *= Exp2(m - top);
                     m = top;
                 }
+                // the last PV is done: its weights may be replaced, its O read
+                if (it > 0 && !(ok = Wait(sh, &sh.o_full, (it - 1) & 1, status))) break;
+                FenceAfter();
                 const float off = kOffset - m;
 #pragma unroll
                 for (int i = 0; i < 64; i += 16) {
+                    float x[16];
+                    Load16(scores + i, x);
+                    WaitLoad();
+                    hide(x, i);
                     uint32_t hi[8], lo[8];
 #pragma unroll
                     for (int j = 0; j < 8; ++j) {
-                        const float p0 = Exp2(fmaf(x[i + 2 * j], c, off)), p1 = Exp2(fmaf(x[i + 2 * j + 1], c, off));
+                        const float p0 = Exp2(fmaf(x[2 * j], c, off)), p1 = Exp2(fmaf(x[2 * j + 1], c, off));
                         l += p0 + p1;
                         SplitHalf(p0, p1, hi[j], lo[j]);
                     }
-                    Store8(buf + half * 32 + i / 2, hi);
-                    Store8(buf + 64 + half * 32 + i / 2, lo);
+                    Store8(lanes + kPCol + half * 32 + i / 2, hi);
+                    Store8(lanes + kPCol + 64 + half * 32 + i / 2, lo);
                 }
                 WaitStore();
                 FenceBefore();
-                Arrive(&sh.p_full[it % kScoreBufs]);
-                if (u > walk.u0 && !(ok = add(u - 1, it - 1))) break;
+                Arrive(&sh.s_empty[it & 1]);
+                Arrive(&sh.p_full);
+                if (u > walk.u0) add(u - 1, it - 1);
                 m_last = m;
             }
-            ok = ok && add(walk.u1 - 1, it - 1);
+            ok = ok && Wait(sh, &sh.o_full, (it - 1) & 1, status);
             if (!ok) break;
+            FenceAfter();
+            add(walk.u1 - 1, it - 1);
             // ---- the row's result, or its part of it
             sh.last[half][row] = l;
             if (!(ok = Meet(sh, &sh.soft, met, status))) break;
@@ -491,7 +502,6 @@ __global__ void __launch_bounds__(kTcWarps * 32, 1) TreeTcKernel(TreeArgs a, Tre
         }
     } else if (warp < kSoftWarps + kProdWarps) {
         // ------------------------------------------------ producers
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
         const int slot = threadIdx.x - kSoftWarps * 32;
         int kt = 0, vt = 0;  // tiles of K and V so far
         uint32_t met = 0;
@@ -571,10 +581,7 @@ __global__ void __launch_bounds__(kTcWarps * 32, 1) TreeTcKernel(TreeArgs a, Tre
                 if (ok) put_v(u);
             }
         }
-    } else {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
-    }
-    if (warp == kMmaWarp && lane == 0) {
+    } else if (lane == 0) {
         // ------------------------------------------------ MMA issue
         const uint32_t qk = Instruction(kTile, false), pv = Instruction(HD, true);
         // K-major images: chunks of K 2048 bytes apart, groups of 8 rows 128
@@ -585,12 +592,10 @@ __global__ void __launch_bounds__(kTcWarps * 32, 1) TreeTcKernel(TreeArgs a, Tre
         int it = 0, item = 0;
         bool ok = true;
         auto values = [&](int n) {  // PV of running tile n
-            if (!WaitOne(sh, &sh.v_full, n & 1, status) || !WaitOne(sh, &sh.p_full[n % kScoreBufs], (n / kScoreBufs) & 1, status))
-                return false;
-            // the last O has been read (so its weights' buffer, two scores back, is free too)
-            if (n > 0 && !WaitOne(sh, &sh.o_empty, (n - 1) & 1, status)) return false;
+            if (!WaitOne(sh, &sh.v_full, n & 1, status) || !WaitOne(sh, &sh.p_full, n & 1, status)) return false;
+            if (n > 0 && !WaitOne(sh, &sh.o_empty, (n - 1) & 1, status)) return false;  // the last O has been read
             FenceAfter();
-            const uint32_t p = tmem + (n % kScoreBufs) * kTile;
+            const uint32_t p = tmem + kPCol;
 #pragma unroll
             for (int s = 0; s < kTile / 16; ++s) MmaTensor(tmem + kOCol, p + 64 + 8 * s, vd + s * kVStep, pv, s != 0);
 #pragma unroll
@@ -606,8 +611,9 @@ __global__ void __launch_bounds__(kTcWarps * 32, 1) TreeTcKernel(TreeArgs a, Tre
             ++item;
             for (int u = walk.u0; u < walk.u1; ++u, ++it) {
                 if (!(ok = WaitOne(sh, &sh.k_full, it & 1, status))) break;
+                if (it > 1 && !(ok = WaitOne(sh, &sh.s_empty[it & 1], ((it >> 1) - 1) & 1, status))) break;
                 FenceAfter();
-                const uint32_t d = tmem + (it % kScoreBufs) * kTile;
+                const uint32_t d = tmem + (it & 1) * kTile;
 #pragma unroll
                 for (int s = 0; s < HD / 16; ++s) MmaShared(d, qd + kLoStep + s * kKStep, kd + s * kKStep, qk, s != 0);
 #pragma unroll
@@ -615,7 +621,7 @@ __global__ void __launch_bounds__(kTcWarps * 32, 1) TreeTcKernel(TreeArgs a, Tre
 #pragma unroll
                 for (int s = 0; s < HD / 16; ++s) MmaShared(d, qd + s * kKStep, kd + s * kKStep, qk, 1);
                 Commit(&sh.k_empty);
-                Commit(&sh.s_full[it % kScoreBufs]);
+                Commit(&sh.s_full[it & 1]);
                 if (u > walk.u0 && !(ok = values(it - 1))) {
                     ++it;
                     break;
