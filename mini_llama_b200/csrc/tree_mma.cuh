@@ -1158,6 +1158,17 @@ __global__ void __launch_bounds__(kJoinWarps * 32) TreeJoinKernel(TreeArgs a, Tr
     }
 }
 
+// Comes up while the main kernel's last CTAs run.
+template <int NB>
+void LaunchJoin(DeviceContext& ctx, const TreeArgs& a, const TreeSplit& sp, int unit, int groups, int item_rows, int grid) {
+    const int all = a.batch * a.c.n_kv * sp.groups;
+    // a row for each warp, as long as that is not many more CTAs than the device holds
+    const int rows = std::min(item_rows, sp.rows);
+    const int per_item = std::max(1, std::min<int>(CeilDiv(rows, kJoinWarps), 16 * ctx.sm_count / all));
+    Launch("TreeJoinKernel", TreeJoinKernel<NB>, dim3(all, per_item), dim3(kJoinWarps * 32), 0, ctx.stream, true, a, sp, unit,
+           groups, item_rows, grid);
+}
+
 template <int TYPE, int NB, int NT, int WQ, int NW, int PER_SM>
 bool LaunchShape(DeviceContext& ctx, const TreeArgs& a) {
     using Shape = TreeShape<TYPE, NB, NT, WQ, NW, PER_SM>;
@@ -1184,10 +1195,7 @@ bool LaunchShape(DeviceContext& ctx, const TreeArgs& a) {
     kernel<<<grid, NW * 32, Shape::kBytes, ctx.stream>>>(a, sp);
     CheckCuda(cudaGetLastError(), "TreeMmaKernel");
     if (grid == 1) return true;  // nothing is cut
-    const int all = a.batch * static_cast<int>(items);
-    const int per_item = std::max(1, std::min(Shape::kItemRows / kJoinWarps, 4 * ctx.sm_count / all));
-    Launch("TreeJoinKernel", TreeJoinKernel<NB>, dim3(all, per_item), dim3(kJoinWarps * 32), 0, ctx.stream, true, a, sp,
-           int(Shape::Warp::kUnit), int(Shape::kGroups), int(Shape::kItemRows), grid);
+    LaunchJoin<NB>(ctx, a, sp, Shape::Warp::kUnit, Shape::kGroups, Shape::kItemRows, grid);
     return true;
 }
 

@@ -10,7 +10,8 @@
 //                 by a power of two and split into hi + lo (22 bits), the lo lo
 //                 product is dropped (2^-22)
 //   softmax       a row's running maximum m, moved when a score passes it by 2^2;
-//                 weights 2^(x - m + 12) <= 2^14 as fp16 hi + lo, into tensor memory
+//                 weights 2^(x - m + 12) <= 2^14 as fp16 hi + lo, written over the
+//                 scores: 16 columns become 8 of hi and 8 of lo
 //   O = P V       128 x head_dim, A from tensor memory, V = hi + lo as K, stored as it
 //                 lies in the cache (the N side contiguous); a fresh accumulator per
 //                 tile, added to the running rows in registers in fp32 (the matrix
@@ -25,15 +26,17 @@
 // other loads share.  One CTA per SM, roles by warp:
 //   0-7    softmax and accumulation: row = lane of tensor memory, two threads to a
 //          row (64 slots, half of head_dim each); scores are read twice, for the
-//          maximum and for the weights, so that a thread holds 16 at a time
-//   8-11   producers: thread = slot; the row's quants in registers a tile ahead,
+//          maximum and for the weights, so that a thread holds 16 at a time.  Q goes
+//          into tensor memory once per item: as an A operand there it leaves half of
+//          shared memory's bandwidth to the producers
+//   8-11   producers: quants in registers a tile ahead of the images,
 //          converted into the operand images (no swizzle: 16-byte chunks of eight
-//          elements, chunk c of row r at 2048 c + 16 r)
+//          elements, chunk c of row r at 2064 c + 16 r)
 //   12     tensor memory; one lane issues all MMAs: QK(i + 1) before PV(i), so that
 //          the tensor pipe works while the weights of tile i + 1 and the images of
 //          the next tiles are made
-// Tensor memory: two buffers of scores, one of weights (free again when its PV is
-// done) and one O.  The cut of the items over the CTAs and the joining of cut
+// Tensor memory: two buffers of scores and weights, Q, one O.  Shared memory: two
+// images of K, one of V.  The cut of the items over the CTAs and the joining of cut
 // items are those of tree_mma.cuh.  Every wait is bounded; an expired one sets the
 // device status word, every role leaves, and issued MMAs are waited for before
 // tensor memory is freed.
@@ -48,14 +51,15 @@ constexpr int kSoftWarps = 8;    // softmax warps
 constexpr int kProdWarps = 4;    // producer warps
 constexpr int kMmaWarp = kSoftWarps + kProdWarps;
 constexpr int kTcWarps = kMmaWarp + 1;
-constexpr int kPCol = 2 * kTile, kOCol = 3 * kTile;  // tensor-memory columns of the weights and of O
+constexpr int kQCol = 2 * kTile, kOCol = 3 * kTile;  // tensor-memory columns of Q and of O
+constexpr int kChunkPitch = 16 * kTile + 16;  // bytes between the chunks of eight elements in an image
 constexpr uint64_t kTcWait = 2000000000ull;
 constexpr int kInfoBufs = 4;     // tiles whose flags are kept
 
 struct TcTreeShared {
-    uint64_t q_full, k_full, k_empty, v_full, v_empty, o_full, o_empty, drain;
+    uint64_t q_full, v_full, v_empty, o_full, o_empty, drain;
     uint64_t soft, prod;  // meetings of the softmax and of the producer threads
-    uint64_t p_full, s_full[2], s_empty[2];
+    uint64_t s_full[2], p_full[2], k_full[2], k_empty[2];
     uint32_t tmem;
     int abort;
     float top[2][2][kTile];  // [parity][half][row]: the largest scores of a tile
@@ -114,12 +118,7 @@ __device__ __forceinline__ uint32_t Instruction(int n, bool b_mn) {
     return (1u << 4) | (b_mn ? 1u << 16 : 0u) | (static_cast<uint32_t>(n >> 3) << 17) | (8u << 24);
 }
 
-__device__ __forceinline__ void MmaShared(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %5, %5, %5}, p;\n\t}\n" ::"r"(d),
-        "l"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(0));
-}
+// A from tensor memory, B from shared memory.
 __device__ __forceinline__ void MmaTensor(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
     asm volatile(
         "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
@@ -197,27 +196,6 @@ __device__ __forceinline__ uint32_t SeenBits(const uint64_t* mask, int words, in
     return seen;
 }
 
-template <int TYPE, int NB>
-struct RawRow {
-    static constexpr int kChunks = NB * (TYPE == MLB_Q8_0 ? 2 : 1);
-    uint4 q[kChunks];
-    uint32_t d[(NB + 1) / 2];
-
-    __device__ __forceinline__ void Load(const uint8_t* plane, const __half* scales, int row) {
-        const uint4* p = reinterpret_cast<const uint4*>(plane + size_t(row) * kChunks * 16);
-#pragma unroll
-        for (int i = 0; i < kChunks; ++i) q[i] = __ldg(p + i);
-        const unsigned short* h = reinterpret_cast<const unsigned short*>(scales + size_t(row) * NB);
-#pragma unroll
-        for (int i = 0; i < NB; ++i) {
-            const uint32_t v = __ldg(h + i);
-            d[i >> 1] = i & 1 ? d[i >> 1] | (v << 16) : v;
-        }
-    }
-    __device__ __forceinline__ uint32_t Scale(int b) const { return (b & 1 ? d[b >> 1] >> 16 : d[b >> 1]) & 0xffffu; }
-    __device__ __forceinline__ void Clear(int b) { d[b >> 1] &= b & 1 ? 0x0000ffffu : 0xffff0000u; }
-};
-
 // hi and lo of d times a half pair, into two words.
 __device__ __forceinline__ void Product(uint32_t pair, __half2 d, uint32_t& hi, uint32_t& lo) {
     const __half2 h = __hmul2(AsHalf2(pair), d);
@@ -225,53 +203,95 @@ __device__ __forceinline__ void Product(uint32_t pair, __half2 d, uint32_t& hi, 
     lo = H2(__hfma2(AsHalf2(pair), d, __hneg2(h)));
 }
 
-// A row's images: within each group of four elements in the order 0, 2, 1, 3.
+// A producer's share of a tile of K or V: one 16-byte piece of quants in each of
+// kPieces places.  Eight neighbouring threads take kSide pieces of 8 / kSide
+// rows, so that loads are whole sectors and the images' stores hit eight
+// different groups of banks.
 template <int TYPE, int NB>
-__device__ __forceinline__ void Convert(const RawRow<TYPE, NB>& r, uint8_t* image, int slot, bool big, uint32_t magic) {
-    constexpr int kLo = NB * 32 * kTile * 2;  // of the lo image
+struct Share {
+    static constexpr int kPieces = NB * (TYPE == MLB_Q8_0 ? 2 : 1);  // of a row
+    static constexpr int kMost = TYPE == MLB_Q8_0 ? 4 : 2;
+    static constexpr int kSide = kPieces % kMost == 0 ? kMost : (kPieces % 2 == 0 ? 2 : 1);
+    static constexpr int kAcross = kPieces / kSide;        // places next to one another
+    static constexpr int kRowsAt = kTile / kSide;          // rows of a place
+    uint4 q[kPieces];
+    unsigned short d[kPieces];
+
+    __device__ __forceinline__ static int Row(int j, int id) { return j / kAcross * kRowsAt + id / kSide; }
+    __device__ __forceinline__ static int Piece(int j, int id) { return j % kAcross * kSide + id % kSide; }
+    __device__ __forceinline__ static int Block(int piece) { return TYPE == MLB_Q8_0 ? piece >> 1 : piece; }
+
+    // Rows of the tile at p0; those from `slots` on count as zeros.
+    __device__ __forceinline__ void Load(const uint8_t* plane, const __half* scales, int p0, int slots, int last, int id) {
 #pragma unroll
-    for (int b = 0; b < NB; ++b) {
-        __half2 d = __half2half2(__ushort_as_half(static_cast<unsigned short>(r.Scale(b))));
-        if (big) d = __hmul2(d, AsHalf2(0x18001800u));  // 2^-9
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {  // eight elements each
-            uint32_t p[4];
-            if constexpr (TYPE == MLB_Q8_0) {
-                const uint4 q = r.q[2 * b + (c >> 1)];
-                const uint32_t w0 = c & 1 ? q.z : q.x, w1 = c & 1 ? q.w : q.y;
-                p[0] = EvenBytes(w0, magic);
-                p[1] = EvenBytes(w0 >> 8, magic);
-                p[2] = EvenBytes(w1, magic);
-                p[3] = EvenBytes(w1 >> 8, magic);
-            } else {
-                const uint4 q = r.q[b];
-                const uint32_t w0 = c & 1 ? q.z : q.x, w1 = c & 1 ? q.w : q.y;
-                p[0] = c < 2 ? LowNibbles(w0, magic) : HighNibbles(w0, magic);
-                p[1] = c < 2 ? LowNibbles(w0 >> 8, magic) : HighNibbles(w0 >> 8, magic);
-                p[2] = c < 2 ? LowNibbles(w1, magic) : HighNibbles(w1, magic);
-                p[3] = c < 2 ? LowNibbles(w1 >> 8, magic) : HighNibbles(w1 >> 8, magic);
-            }
-            uint4 hi, lo;
-            Product(p[0], d, hi.x, lo.x);
-            Product(p[1], d, hi.y, lo.y);
-            Product(p[2], d, hi.z, lo.z);
-            Product(p[3], d, hi.w, lo.w);
-            uint8_t* to = image + (4 * b + c) * 2048 + slot * 16;
-            *reinterpret_cast<uint4*>(to) = hi;
-            *reinterpret_cast<uint4*>(to + kLo) = lo;
+        for (int j = 0; j < kPieces; ++j) {
+            const int at = p0 + Row(j, id), row = min(at, last), piece = Piece(j, id);
+            q[j] = __ldg(reinterpret_cast<const uint4*>(plane + size_t(row) * (kPieces * 16)) + piece);
+            d[j] = __ldg(reinterpret_cast<const unsigned short*>(scales + size_t(row) * NB + Block(piece)));
+            if (at >= slots) d[j] = 0;
         }
     }
-}
+    __device__ __forceinline__ bool Big() const {
+        bool big = false;
+#pragma unroll
+        for (int j = 0; j < kPieces; ++j) big = big || (d[j] & 0x7fffu) >= 0x5C00u;  // 2^8, infinity, NaN
+        return big;
+    }
+    // Takes out the scales that are not finite of rows from `from` on; whether there was one.
+    __device__ __forceinline__ bool TakeOdd(int from, int id) {
+        bool odd = false;
+#pragma unroll
+        for (int j = 0; j < kPieces; ++j)
+            if ((d[j] & 0x7C00u) == 0x7C00u && Row(j, id) >= from) {
+                odd = true;
+                d[j] = 0;
+            }
+        return odd;
+    }
+    // Into the images: within each group of four elements in the order 0, 2, 1, 3.
+    __device__ __forceinline__ void Convert(uint8_t* image, int id, bool big, uint32_t magic) const {
+        constexpr int kLo = NB * 4 * kChunkPitch;  // of the lo image
+#pragma unroll
+        for (int j = 0; j < kPieces; ++j) {
+            __half2 s = __half2half2(__ushort_as_half(d[j]));
+            if (big) s = __hmul2(s, AsHalf2(0x18001800u));  // 2^-9
+            uint8_t* to = image + Piece(j, id) * ((TYPE == MLB_Q8_0 ? 2 : 4) * kChunkPitch) + Row(j, id) * 16;
+            const uint32_t w[4] = {q[j].x, q[j].y, q[j].z, q[j].w};
+#pragma unroll
+            for (int c = 0; c < (TYPE == MLB_Q8_0 ? 2 : 4); ++c) {  // eight elements each
+                const uint32_t w0 = w[2 * (c & 1)], w1 = w[2 * (c & 1) + 1];
+                uint32_t p[4];
+                if constexpr (TYPE == MLB_Q8_0) {
+                    p[0] = EvenBytes(w0, magic);
+                    p[1] = EvenBytes(w0 >> 8, magic);
+                    p[2] = EvenBytes(w1, magic);
+                    p[3] = EvenBytes(w1 >> 8, magic);
+                } else {
+                    p[0] = c < 2 ? LowNibbles(w0, magic) : HighNibbles(w0, magic);
+                    p[1] = c < 2 ? LowNibbles(w0 >> 8, magic) : HighNibbles(w0 >> 8, magic);
+                    p[2] = c < 2 ? LowNibbles(w1, magic) : HighNibbles(w1, magic);
+                    p[3] = c < 2 ? LowNibbles(w1 >> 8, magic) : HighNibbles(w1 >> 8, magic);
+                }
+                uint4 hi, lo;
+                Product(p[0], s, hi.x, lo.x);
+                Product(p[1], s, hi.y, lo.y);
+                Product(p[2], s, hi.z, lo.z);
+                Product(p[3], s, hi.w, lo.w);
+                *reinterpret_cast<uint4*>(to + c * kChunkPitch) = hi;
+                *reinterpret_cast<uint4*>(to + c * kChunkPitch + kLo) = lo;
+            }
+        }
+    }
+};
 
 template <int TYPE, int NB>
 __global__ void __launch_bounds__(kTcWarps * 32, 1) TreeTcKernel(TreeArgs a, TreeSplit sp, int* status) {
-    constexpr int HD = NB * 32, kImage = HD * kTile * 2;  // one fp16 image
+    constexpr int HD = NB * 32, kImage = NB * 4 * kChunkPitch;  // one fp16 image
     constexpr int kHalf = HD / 2;                         // head_dim of a softmax thread
     extern __shared__ __align__(1024) uint8_t tc_smem[];
     TcTreeShared& sh = *reinterpret_cast<TcTreeShared*>(tc_smem);
-    uint8_t* qi = tc_smem + kTcHeaderBytes;  // hi, lo
-    uint8_t* ki = qi + 2 * kImage;
-    uint8_t* vi = ki + 2 * kImage;
+    uint8_t* ki = tc_smem + kTcHeaderBytes;  // two buffers of hi, lo
+    uint8_t* vi = ki + 4 * kImage;           // hi, lo
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const unsigned items = a.c.n_kv * sp.groups;
 
@@ -292,19 +312,18 @@ __global__ void __launch_bounds__(kTcWarps * 32, 1) TreeTcKernel(TreeArgs a, Tre
 
     if (threadIdx.x == 0) {
         MbarInit(&sh.q_full, kSoftWarps * 32);
-        MbarInit(&sh.k_full, kProdWarps * 32);
         MbarInit(&sh.v_full, kProdWarps * 32);
-        MbarInit(&sh.k_empty, 1);
         MbarInit(&sh.v_empty, 1);
         MbarInit(&sh.o_full, 1);
         MbarInit(&sh.o_empty, kSoftWarps * 32);
         MbarInit(&sh.drain, 1);
         MbarInit(&sh.soft, kSoftWarps * 32);
         MbarInit(&sh.prod, kProdWarps * 32);
-        MbarInit(&sh.p_full, kSoftWarps * 32);
         for (int i = 0; i < 2; ++i) {
+            MbarInit(&sh.p_full[i], kSoftWarps * 32);
             MbarInit(&sh.s_full[i], 1);
-            MbarInit(&sh.s_empty[i], kSoftWarps * 32);
+            MbarInit(&sh.k_full[i], kProdWarps * 32);
+            MbarInit(&sh.k_empty[i], 1);
         }
         FenceMbarInit();
         sh.abort = 0;
@@ -360,17 +379,19 @@ __global__ void __launch_bounds__(kTcWarps * 32, 1) TreeTcKernel(TreeArgs a, Tre
                 const float sc = Pow2(up);
                 cs = fmaxf(Pow2(-up) * a.scale * kLog2e, 1e-37f);
 #pragma unroll
-                for (int i = 0; i < kHalf; i += 8) {
-                    uint4 hi, lo;
-                    SplitHalf(x[i] * sc, x[i + 2] * sc, hi.x, lo.x);
-                    SplitHalf(x[i + 1] * sc, x[i + 3] * sc, hi.y, lo.y);
-                    SplitHalf(x[i + 4] * sc, x[i + 6] * sc, hi.z, lo.z);
-                    SplitHalf(x[i + 5] * sc, x[i + 7] * sc, hi.w, lo.w);
-                    uint8_t* to = qi + (half * kHalf + i) / 8 * 2048 + row * 16;
-                    *reinterpret_cast<uint4*>(to) = hi;
-                    *reinterpret_cast<uint4*>(to + kImage) = lo;
+                for (int i = 0; i < kHalf; i += 16) {  // a k step: 8 columns of hi, 8 of lo
+                    uint32_t hi[8], lo[8];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {  // the images' order 0, 2, 1, 3
+                        const float* y = x + i + 4 * j;
+                        SplitHalf(y[0] * sc, y[2] * sc, hi[2 * j], lo[2 * j]);
+                        SplitHalf(y[1] * sc, y[3] * sc, hi[2 * j + 1], lo[2 * j + 1]);
+                    }
+                    Store8(lanes + kQCol + half * kHalf + i, hi);
+                    Store8(lanes + kQCol + half * kHalf + i + 8, lo);
                 }
-                FenceAsync();
+                WaitStore();
+                FenceBefore();
                 Arrive(&sh.q_full);
             }
             float o[kHalf], m = kStart, l = 0.0f, m_of_o = kStart, m_last = kStart;
@@ -441,9 +462,6 @@ __global__ void __launch_bounds__(kTcWarps * 32, 1) TreeTcKernel(TreeArgs a, Tre
                     l *= Exp2(m - top);
                     m = top;
                 }
-                // the last PV is done: its weights may be replaced, its O read
-                if (it > 0 && !(ok = Wait(sh, &sh.o_full, (it - 1) & 1, status))) break;
-                FenceAfter();
                 const float off = kOffset - m;
 #pragma unroll
                 for (int i = 0; i < 64; i += 16) {
@@ -458,14 +476,17 @@ __global__ void __launch_bounds__(kTcWarps * 32, 1) TreeTcKernel(TreeArgs a, Tre
                         l += p0 + p1;
                         SplitHalf(p0, p1, hi[j], lo[j]);
                     }
-                    Store8(lanes + kPCol + half * 32 + i / 2, hi);
-                    Store8(lanes + kPCol + 64 + half * 32 + i / 2, lo);
+                    Store8(scores + i, hi);
+                    Store8(scores + i + 8, lo);
                 }
                 WaitStore();
                 FenceBefore();
-                Arrive(&sh.s_empty[it & 1]);
-                Arrive(&sh.p_full);
-                if (u > walk.u0) add(u - 1, it - 1);
+                Arrive(&sh.p_full[it & 1]);
+                if (u > walk.u0) {
+                    if (!(ok = Wait(sh, &sh.o_full, (it - 1) & 1, status))) break;
+                    FenceAfter();
+                    add(u - 1, it - 1);
+                }
                 m_last = m;
             }
             ok = ok && Wait(sh, &sh.o_full, (it - 1) & 1, status);
@@ -502,7 +523,7 @@ __global__ void __launch_bounds__(kTcWarps * 32, 1) TreeTcKernel(TreeArgs a, Tre
         }
     } else if (warp < kSoftWarps + kProdWarps) {
         // ------------------------------------------------ producers
-        const int slot = threadIdx.x - kSoftWarps * 32;
+        const int id = threadIdx.x - kSoftWarps * 32;
         int kt = 0, vt = 0;  // tiles of K and V so far
         uint32_t met = 0;
         bool ok = true;
@@ -510,64 +531,53 @@ __global__ void __launch_bounds__(kTcWarps * 32, 1) TreeTcKernel(TreeArgs a, Tre
         auto together = [&](uint32_t bits) {
             bits = __reduce_or_sync(0xffffffffu, bits);
             const uint32_t side = met & 1;
-            if (lane == 0) sh.flag[side][slot / 32] = bits;
+            if (lane == 0) sh.flag[side][id / 32] = bits;
             ok = Meet(sh, &sh.prod, met, status);
             return sh.flag[side][0] | sh.flag[side][1] | sh.flag[side][2] | sh.flag[side][3];
         };
         while (ok && walk.Next(a, sp, items)) {
             const long long base = a.c.Row(walk.e.seq, a.layer, walk.head, 0);
-            constexpr int kRowBytes = RawRow<TYPE, NB>::kChunks * 16;
+            constexpr int kRowBytes = Share<TYPE, NB>::kPieces * 16;
             const uint8_t* kp = static_cast<const uint8_t*>(a.c.k) + base * kRowBytes;
             const uint8_t* vp = static_cast<const uint8_t*>(a.c.v) + base * kRowBytes;
             const __half *ks = a.c.ks + base * NB, *vs = a.c.vs + base * NB;
-            RawRow<TYPE, NB> rk, rv;
-            auto load = [&](RawRow<TYPE, NB>& r, const uint8_t* plane, const __half* scales, int u) {
-                const int at = u * kTile + slot;
-                r.Load(plane, scales, min(at, a.c.head_slots - 1));
-                if (at >= walk.e.slots)
-#pragma unroll
-                    for (int i = 0; i < (NB + 1) / 2; ++i) r.d[i] = 0;
-            };
-            auto big_scale = [&](const RawRow<TYPE, NB>& r) {
-                bool big = false;
-#pragma unroll
-                for (int b = 0; b < NB; ++b) big = big || (r.Scale(b) & 0x7fffu) >= 0x5C00u;  // 2^8, infinity, NaN
-                return big;
+            Share<TYPE, NB> rk, rv;
+            auto load = [&](Share<TYPE, NB>& r, const uint8_t* plane, const __half* scales, int u) {
+                r.Load(plane, scales, u * kTile, walk.e.slots, a.c.head_slots - 1, id);
             };
             auto put_k = [&](int u) {
-                const bool big = together(big_scale(rk)) != 0;
+                const bool big = together(rk.Big()) != 0;
                 if (!ok) return;
-                if (kt > 0 && !(ok = Wait(sh, &sh.k_empty, (kt - 1) & 1, status))) return;
-                if (slot == 0) sh.k_big[kt % kInfoBufs] = big;
-                Convert<TYPE, NB>(rk, ki, slot, big, sp.magic);
+                if (kt > 1 && !(ok = Wait(sh, &sh.k_empty[kt & 1], ((kt >> 1) - 1) & 1, status))) return;
+                if (id == 0) sh.k_big[kt % kInfoBufs] = big;
+                rk.Convert(ki + (kt & 1) * 2 * kImage, id, big, sp.magic);
                 FenceAsync();
-                Arrive(&sh.k_full);
+                Arrive(&sh.k_full[kt & 1]);
                 ++kt;
                 if (u + 1 < walk.u1) load(rk, kp, ks, u + 1);
             };
             auto put_v = [&](int u) {
                 // a drafted slot's scale that is not finite is taken out and noted
-                uint32_t odd = 0;
-#pragma unroll
-                for (int b = 0; b < NB; ++b)
-                    if ((rv.Scale(b) & 0x7C00u) == 0x7C00u && u * kTile + slot >= walk.e.len) {
-                        odd |= 1u << b;
-                        rv.Clear(b);
-                    }
-                const uint32_t flags = together((big_scale(rv) ? 1u : 0u) | (odd ? 2u : 0u));
+                const bool odd = rv.TakeOdd(walk.e.len - u * kTile, id);
+                const uint32_t flags = together((rv.Big() ? 1u : 0u) | (odd ? 2u : 0u));
                 if (!ok) return;
                 const bool big = flags & 1, any = flags & 2;
                 if (vt > 0 && !(ok = Wait(sh, &sh.v_empty, (vt - 1) & 1, status))) return;
-                if (any)
+                if (any) {  // a row for each thread
+                    const int at = u * kTile + id;
                     for (int b = 0; b < NB; ++b) {
-                        const uint32_t bits = __ballot_sync(0xffffffffu, (odd >> b) & 1);
-                        if (lane == 0) sh.v_bad[vt % kInfoBufs][b][slot / 32] = bits;
+                        const unsigned short d =
+                            __ldg(reinterpret_cast<const unsigned short*>(vs + size_t(min(at, a.c.head_slots - 1)) * NB + b));
+                        const bool bad = (d & 0x7C00u) == 0x7C00u && at >= walk.e.len && at < walk.e.slots;
+                        const uint32_t bits = __ballot_sync(0xffffffffu, bad);
+                        if (lane == 0) sh.v_bad[vt % kInfoBufs][b][id / 32] = bits;
                     }
-                if (slot == 0) {
+                }
+                if (id == 0) {
                     sh.v_big[vt % kInfoBufs] = big;
                     sh.v_odd[vt % kInfoBufs] = any;
                 }
-                Convert<TYPE, NB>(rv, vi, slot, big, sp.magic);
+                rv.Convert(vi, id, big, sp.magic);
                 FenceAsync();
                 Arrive(&sh.v_full);
                 ++vt;
@@ -584,24 +594,24 @@ __global__ void __launch_bounds__(kTcWarps * 32, 1) TreeTcKernel(TreeArgs a, Tre
     } else if (lane == 0) {
         // ------------------------------------------------ MMA issue
         const uint32_t qk = Instruction(kTile, false), pv = Instruction(HD, true);
-        // K-major images: chunks of K 2048 bytes apart, groups of 8 rows 128
-        const uint64_t qd = Descriptor(SmemAddr(qi), 2048, 128), kd = Descriptor(SmemAddr(ki), 2048, 128);
-        // V: groups of 8 slots 128 bytes apart, groups of 8 of head_dim 2048
-        const uint64_t vd = Descriptor(SmemAddr(vi), 128, 2048);
-        constexpr uint64_t kLoStep = kImage >> 4, kKStep = 4096 >> 4, kVStep = 256 >> 4;
+        // K-major images: chunks of K kChunkPitch bytes apart, groups of 8 rows 128
+        const uint64_t kd = Descriptor(SmemAddr(ki), kChunkPitch, 128);
+        // V: groups of 8 slots 128 bytes apart, groups of 8 of head_dim kChunkPitch
+        const uint64_t vd = Descriptor(SmemAddr(vi), 128, kChunkPitch);
+        constexpr uint64_t kLoStep = kImage >> 4, kKStep = (2 * kChunkPitch) >> 4, kVStep = 256 >> 4;
         int it = 0, item = 0;
         bool ok = true;
         auto values = [&](int n) {  // PV of running tile n
-            if (!WaitOne(sh, &sh.v_full, n & 1, status) || !WaitOne(sh, &sh.p_full, n & 1, status)) return false;
+            if (!WaitOne(sh, &sh.v_full, n & 1, status) || !WaitOne(sh, &sh.p_full[n & 1], (n >> 1) & 1, status)) return false;
             if (n > 0 && !WaitOne(sh, &sh.o_empty, (n - 1) & 1, status)) return false;  // the last O has been read
             FenceAfter();
-            const uint32_t p = tmem + kPCol;
+            const uint32_t p = tmem + (n & 1) * kTile;
 #pragma unroll
-            for (int s = 0; s < kTile / 16; ++s) MmaTensor(tmem + kOCol, p + 64 + 8 * s, vd + s * kVStep, pv, s != 0);
+            for (int s = 0; s < kTile / 16; ++s) MmaTensor(tmem + kOCol, p + 16 * s + 8, vd + s * kVStep, pv, s != 0);
 #pragma unroll
-            for (int s = 0; s < kTile / 16; ++s) MmaTensor(tmem + kOCol, p + 8 * s, vd + kLoStep + s * kVStep, pv, 1);
+            for (int s = 0; s < kTile / 16; ++s) MmaTensor(tmem + kOCol, p + 16 * s, vd + kLoStep + s * kVStep, pv, 1);
 #pragma unroll
-            for (int s = 0; s < kTile / 16; ++s) MmaTensor(tmem + kOCol, p + 8 * s, vd + s * kVStep, pv, 1);
+            for (int s = 0; s < kTile / 16; ++s) MmaTensor(tmem + kOCol, p + 16 * s, vd + s * kVStep, pv, 1);
             Commit(&sh.v_empty);
             Commit(&sh.o_full);
             return true;
@@ -610,17 +620,20 @@ __global__ void __launch_bounds__(kTcWarps * 32, 1) TreeTcKernel(TreeArgs a, Tre
             if (!(ok = WaitOne(sh, &sh.q_full, item & 1, status))) break;
             ++item;
             for (int u = walk.u0; u < walk.u1; ++u, ++it) {
-                if (!(ok = WaitOne(sh, &sh.k_full, it & 1, status))) break;
-                if (it > 1 && !(ok = WaitOne(sh, &sh.s_empty[it & 1], ((it >> 1) - 1) & 1, status))) break;
+                if (!(ok = WaitOne(sh, &sh.k_full[it & 1], (it >> 1) & 1, status))) break;
+                // The weights that lay in this buffer, of tile it - 2, have been multiplied: its PV is the one issued
+                // last, but at the start of an item, where PV(it - 1) has been issued after O(it - 2) was read.
+                if (it > 1 && u > walk.u0 && !(ok = WaitOne(sh, &sh.o_full, it & 1, status))) break;
                 FenceAfter();
-                const uint32_t d = tmem + (it & 1) * kTile;
+                const uint32_t d = tmem + (it & 1) * kTile, q = tmem + kQCol;
+                const uint64_t k = kd + (it & 1) * 2 * kLoStep;
 #pragma unroll
-                for (int s = 0; s < HD / 16; ++s) MmaShared(d, qd + kLoStep + s * kKStep, kd + s * kKStep, qk, s != 0);
+                for (int s = 0; s < HD / 16; ++s) MmaTensor(d, q + 16 * s + 8, k + s * kKStep, qk, s != 0);
 #pragma unroll
-                for (int s = 0; s < HD / 16; ++s) MmaShared(d, qd + s * kKStep, kd + kLoStep + s * kKStep, qk, 1);
+                for (int s = 0; s < HD / 16; ++s) MmaTensor(d, q + 16 * s, k + kLoStep + s * kKStep, qk, 1);
 #pragma unroll
-                for (int s = 0; s < HD / 16; ++s) MmaShared(d, qd + s * kKStep, kd + s * kKStep, qk, 1);
-                Commit(&sh.k_empty);
+                for (int s = 0; s < HD / 16; ++s) MmaTensor(d, q + 16 * s, k + s * kKStep, qk, 1);
+                Commit(&sh.k_empty[it & 1]);
                 Commit(&sh.s_full[it & 1]);
                 if (u > walk.u0 && !(ok = values(it - 1))) {
                     ++it;
@@ -653,7 +666,7 @@ bool LaunchTc(DeviceContext& ctx, const TreeArgs& a) {
     const int grid = static_cast<int>(std::min<double>(ctx.sm_count, units));
     sp.parts = static_cast<float*>(Workspace(ctx, 2 * size_t(grid) * kTile * (NB * 32 + 2) * sizeof(float)));
     sp.magic = TYPE == MLB_Q8_0 ? kMagic8 : kMagic4;
-    constexpr int kBytes = kTcHeaderBytes + 6 * NB * 32 * kTile * 2;
+    constexpr int kBytes = kTcHeaderBytes + 6 * NB * 4 * kChunkPitch;
     auto* kernel = TreeTcKernel<TYPE, NB>;
     static int configured[64] = {};
     if (ctx.device >= 64 || !configured[ctx.device]) {
@@ -664,10 +677,7 @@ bool LaunchTc(DeviceContext& ctx, const TreeArgs& a) {
     kernel<<<grid, kTcWarps * 32, kBytes, ctx.stream>>>(a, sp, ctx.status);
     CheckCuda(cudaGetLastError(), "TreeTcKernel");
     if (grid == 1) return true;  // nothing is cut
-    const int all = a.batch * static_cast<int>(items);
-    const int per_item = std::max(1, std::min(kTile / kJoinWarps, 4 * ctx.sm_count / all));
-    Launch("TreeJoinKernel", TreeJoinKernel<NB>, dim3(all, per_item), dim3(kJoinWarps * 32), 0, ctx.stream, true, a, sp,
-           int(kTile), 1, int(kTile), grid);
+    LaunchJoin<NB>(ctx, a, sp, kTile, 1, kTile, grid);
     return true;
 }
 
