@@ -29,10 +29,10 @@
 //          maximum and for the weights, so that a thread holds 16 at a time.  Q goes
 //          into tensor memory once per item: as an A operand there it leaves half of
 //          shared memory's bandwidth to the producers
-//   8-11   producers: quants in registers a tile ahead of the images,
+//   8-15   producers: quants in registers a tile ahead of the images,
 //          converted into the operand images (no swizzle: 16-byte chunks of eight
 //          elements, chunk c of row r at 2064 c + 16 r)
-//   12     tensor memory; one lane issues all MMAs: QK(i + 1) before PV(i), so that
+//   16     tensor memory (17-19 idle); one lane issues all MMAs: QK(i + 1) before PV(i), so that
 //          the tensor pipe works while the weights of tile i + 1 and the images of
 //          the next tiles are made
 // Tensor memory: two buffers of scores and weights, Q, one O.  Shared memory: two
@@ -48,9 +48,14 @@ namespace {
 
 constexpr int kTile = 128;       // slots of a tile and rows of an item
 constexpr int kSoftWarps = 8;    // softmax warps
-constexpr int kProdWarps = 4;    // producer warps
+constexpr int kProdWarps = 8;    // producer warps
 constexpr int kMmaWarp = kSoftWarps + kProdWarps;
-constexpr int kTcWarps = kMmaWarp + 1;
+constexpr int kTcWarps = kMmaWarp + 4;  // a whole warpgroup, for the register split
+// Registers of a softmax, a producer and an MMA thread: five warpgroups launched
+// with 96 each, 2 x 144 + 2 x 72 + 40 of their 5 x 96.
+constexpr int kSoftRegs = 144, kProdRegs = 72, kMmaRegs = 40;
+static_assert(2 * kSoftRegs + 2 * kProdRegs + kMmaRegs <= 5 * 96, "setmaxnreg draws on the launch's registers");
+constexpr int kProducers = kProdWarps * 32;
 constexpr int kQCol = 2 * kTile, kOCol = 3 * kTile;  // tensor-memory columns of Q and of O
 constexpr int kChunkPitch = 16 * kTile + 16;  // bytes between the chunks of eight elements in an image
 constexpr uint64_t kTcWait = 2000000000ull;
@@ -203,28 +208,33 @@ __device__ __forceinline__ void Product(uint32_t pair, __half2 d, uint32_t& hi, 
     lo = H2(__hfma2(AsHalf2(pair), d, __hneg2(h)));
 }
 
-// A producer's share of a tile of K or V: one 16-byte piece of quants in each of
-// kPieces places.  Eight neighbouring threads take kSide pieces of 8 / kSide
-// rows, so that loads are whole sectors and the images' stores hit eight
-// different groups of banks.
+// A producer's share of a tile of K or V: 16-byte pieces of quants.  Eight
+// neighbouring threads take kSide pieces of 8 / kSide rows, so that loads are
+// whole sectors and the images' stores hit eight different groups of banks.
 template <int TYPE, int NB>
 struct Share {
     static constexpr int kPieces = NB * (TYPE == MLB_Q8_0 ? 2 : 1);  // of a row
     static constexpr int kMost = TYPE == MLB_Q8_0 ? 4 : 2;
     static constexpr int kSide = kPieces % kMost == 0 ? kMost : (kPieces % 2 == 0 ? 2 : 1);
-    static constexpr int kAcross = kPieces / kSide;        // places next to one another
-    static constexpr int kRowsAt = kTile / kSide;          // rows of a place
-    uint4 q[kPieces];
-    unsigned short d[kPieces];
+    static constexpr int kTasks = (kPieces * kTile + kProducers - 1) / kProducers;
+    uint4 q[kTasks];
+    unsigned short d[kTasks];
 
-    __device__ __forceinline__ static int Row(int j, int id) { return j / kAcross * kRowsAt + id / kSide; }
-    __device__ __forceinline__ static int Piece(int j, int id) { return j % kAcross * kSide + id % kSide; }
+    __device__ __forceinline__ static int Row(int j, int id) { return (j * kProducers + id) / kSide % kTile; }
+    __device__ __forceinline__ static int Piece(int j, int id) {
+        return (j * kProducers + id) / (kSide * kTile) * kSide + id % kSide;
+    }
+    __device__ __forceinline__ static bool Has(int j, int id) {
+        return kPieces * kTile % kProducers == 0 || j * kProducers + id < kPieces * kTile;
+    }
     __device__ __forceinline__ static int Block(int piece) { return TYPE == MLB_Q8_0 ? piece >> 1 : piece; }
 
     // Rows of the tile at p0; those from `slots` on count as zeros.
     __device__ __forceinline__ void Load(const uint8_t* plane, const __half* scales, int p0, int slots, int last, int id) {
 #pragma unroll
-        for (int j = 0; j < kPieces; ++j) {
+        for (int j = 0; j < kTasks; ++j) {
+            d[j] = 0;
+            if (!Has(j, id)) continue;
             const int at = p0 + Row(j, id), row = min(at, last), piece = Piece(j, id);
             q[j] = __ldg(reinterpret_cast<const uint4*>(plane + size_t(row) * (kPieces * 16)) + piece);
             d[j] = __ldg(reinterpret_cast<const unsigned short*>(scales + size_t(row) * NB + Block(piece)));
@@ -234,14 +244,14 @@ struct Share {
     __device__ __forceinline__ bool Big() const {
         bool big = false;
 #pragma unroll
-        for (int j = 0; j < kPieces; ++j) big = big || (d[j] & 0x7fffu) >= 0x5C00u;  // 2^8, infinity, NaN
+        for (int j = 0; j < kTasks; ++j) big = big || (d[j] & 0x7fffu) >= 0x5C00u;  // 2^8, infinity, NaN
         return big;
     }
     // Takes out the scales that are not finite of rows from `from` on; whether there was one.
     __device__ __forceinline__ bool TakeOdd(int from, int id) {
         bool odd = false;
 #pragma unroll
-        for (int j = 0; j < kPieces; ++j)
+        for (int j = 0; j < kTasks; ++j)
             if ((d[j] & 0x7C00u) == 0x7C00u && Row(j, id) >= from) {
                 odd = true;
                 d[j] = 0;
@@ -252,7 +262,8 @@ struct Share {
     __device__ __forceinline__ void Convert(uint8_t* image, int id, bool big, uint32_t magic) const {
         constexpr int kLo = NB * 4 * kChunkPitch;  // of the lo image
 #pragma unroll
-        for (int j = 0; j < kPieces; ++j) {
+        for (int j = 0; j < kTasks; ++j) {
+            if (!Has(j, id)) continue;
             __half2 s = __half2half2(__ushort_as_half(d[j]));
             if (big) s = __hmul2(s, AsHalf2(0x18001800u));  // 2^-9
             uint8_t* to = image + Piece(j, id) * ((TYPE == MLB_Q8_0 ? 2 : 4) * kChunkPitch) + Row(j, id) * 16;
@@ -339,6 +350,7 @@ __global__ void __launch_bounds__(kTcWarps * 32, 1) TreeTcKernel(TreeArgs a, Tre
 
     if (warp < kSoftWarps) {
         // ------------------------------------------------ softmax and accumulation
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftRegs));
         const int half = warp >> 2, row = (warp & 3) * 32 + lane;
         const uint32_t lanes = tmem + ((static_cast<uint32_t>(warp & 3) * 32) << 16);
         int it = 0;  // tiles so far
@@ -523,6 +535,7 @@ __global__ void __launch_bounds__(kTcWarps * 32, 1) TreeTcKernel(TreeArgs a, Tre
         }
     } else if (warp < kSoftWarps + kProdWarps) {
         // ------------------------------------------------ producers
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kProdRegs));
         const int id = threadIdx.x - kSoftWarps * 32;
         int kt = 0, vt = 0;  // tiles of K and V so far
         uint32_t met = 0;
@@ -533,7 +546,10 @@ __global__ void __launch_bounds__(kTcWarps * 32, 1) TreeTcKernel(TreeArgs a, Tre
             const uint32_t side = met & 1;
             if (lane == 0) sh.flag[side][id / 32] = bits;
             ok = Meet(sh, &sh.prod, met, status);
-            return sh.flag[side][0] | sh.flag[side][1] | sh.flag[side][2] | sh.flag[side][3];
+            bits = 0;
+#pragma unroll
+            for (int i = 0; i < kProdWarps; ++i) bits |= sh.flag[side][i];
+            return bits;
         };
         while (ok && walk.Next(a, sp, items)) {
             const long long base = a.c.Row(walk.e.seq, a.layer, walk.head, 0);
@@ -563,7 +579,7 @@ __global__ void __launch_bounds__(kTcWarps * 32, 1) TreeTcKernel(TreeArgs a, Tre
                 if (!ok) return;
                 const bool big = flags & 1, any = flags & 2;
                 if (vt > 0 && !(ok = Wait(sh, &sh.v_empty, (vt - 1) & 1, status))) return;
-                if (any) {  // a row for each thread
+                if (any && id < kTile) {  // a row for each of four warps' threads
                     const int at = u * kTile + id;
                     for (int b = 0; b < NB; ++b) {
                         const unsigned short d =
@@ -591,7 +607,10 @@ __global__ void __launch_bounds__(kTcWarps * 32, 1) TreeTcKernel(TreeArgs a, Tre
                 if (ok) put_v(u);
             }
         }
-    } else if (lane == 0) {
+    } else {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kMmaRegs));
+    }
+    if (warp == kMmaWarp && lane == 0) {
         // ------------------------------------------------ MMA issue
         const uint32_t qk = Instruction(kTile, false), pv = Instruction(HD, true);
         // K-major images: chunks of K kChunkPitch bytes apart, groups of 8 rows 128
@@ -606,11 +625,11 @@ __global__ void __launch_bounds__(kTcWarps * 32, 1) TreeTcKernel(TreeArgs a, Tre
             if (n > 0 && !WaitOne(sh, &sh.o_empty, (n - 1) & 1, status)) return false;  // the last O has been read
             FenceAfter();
             const uint32_t p = tmem + (n & 1) * kTile;
-#pragma unroll
+#pragma unroll 2
             for (int s = 0; s < kTile / 16; ++s) MmaTensor(tmem + kOCol, p + 16 * s + 8, vd + s * kVStep, pv, s != 0);
-#pragma unroll
+#pragma unroll 2
             for (int s = 0; s < kTile / 16; ++s) MmaTensor(tmem + kOCol, p + 16 * s, vd + kLoStep + s * kVStep, pv, 1);
-#pragma unroll
+#pragma unroll 2
             for (int s = 0; s < kTile / 16; ++s) MmaTensor(tmem + kOCol, p + 16 * s, vd + s * kVStep, pv, 1);
             Commit(&sh.v_empty);
             Commit(&sh.o_full);
@@ -627,11 +646,11 @@ __global__ void __launch_bounds__(kTcWarps * 32, 1) TreeTcKernel(TreeArgs a, Tre
                 FenceAfter();
                 const uint32_t d = tmem + (it & 1) * kTile, q = tmem + kQCol;
                 const uint64_t k = kd + (it & 1) * 2 * kLoStep;
-#pragma unroll
+#pragma unroll 2
                 for (int s = 0; s < HD / 16; ++s) MmaTensor(d, q + 16 * s + 8, k + s * kKStep, qk, s != 0);
-#pragma unroll
+#pragma unroll 2
                 for (int s = 0; s < HD / 16; ++s) MmaTensor(d, q + 16 * s, k + kLoStep + s * kKStep, qk, 1);
-#pragma unroll
+#pragma unroll 2
                 for (int s = 0; s < HD / 16; ++s) MmaTensor(d, q + 16 * s, k + s * kKStep, qk, 1);
                 Commit(&sh.k_empty[it & 1]);
                 Commit(&sh.s_full[it & 1]);
