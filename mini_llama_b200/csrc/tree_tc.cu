@@ -32,7 +32,7 @@
 //   8-15   producers: quants in registers a tile ahead of the images,
 //          converted into the operand images (no swizzle: 16-byte chunks of eight
 //          elements, chunk c of row r at 2064 c + 16 r)
-//   16     tensor memory (17-19 idle); one lane issues all MMAs: QK(i + 1) before PV(i), so that
+//   16     tensor memory (17-19 idle); issues all MMAs: QK(i + 1) before PV(i), so that
 //          the tensor pipe works while the weights of tile i + 1 and the images of
 //          the next tiles are made
 // Tensor memory: two buffers of scores and weights, Q, one O.  Shared memory: two
@@ -52,8 +52,8 @@ constexpr int kProdWarps = 8;    // producer warps
 constexpr int kMmaWarp = kSoftWarps + kProdWarps;
 constexpr int kTcWarps = kMmaWarp + 4;  // a whole warpgroup, for the register split
 // Registers of a softmax, a producer and an MMA thread: five warpgroups launched
-// with 96 each, 2 x 144 + 2 x 72 + 40 of their 5 x 96.
-constexpr int kSoftRegs = 144, kProdRegs = 72, kMmaRegs = 40;
+// with 96 each, 2 x 128 + 2 x 88 + 48 of their 5 x 96.
+constexpr int kSoftRegs = 128, kProdRegs = 88, kMmaRegs = 48;
 static_assert(2 * kSoftRegs + 2 * kProdRegs + kMmaRegs <= 5 * 96, "setmaxnreg draws on the launch's registers");
 constexpr int kProducers = kProdWarps * 32;
 constexpr int kQCol = 2 * kTile, kOCol = 3 * kTile;  // tensor-memory columns of Q and of O
@@ -97,9 +97,12 @@ __device__ __forceinline__ bool Wait(TcTreeShared& sh, uint64_t* bar, uint32_t p
 __device__ __forceinline__ void Arrive(uint64_t* bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(SmemAddr(bar)) : "memory");
 }
-__device__ __forceinline__ void Commit(uint64_t* bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(SmemAddr(bar))
-                 : "memory");
+__device__ __forceinline__ void Commit(uint32_t one, uint64_t* bar) {
+    asm volatile(
+        "{\n\t.reg .pred e;\n\tsetp.ne.b32 e, %1, 0;\n\t"
+        "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}\n" ::"r"(SmemAddr(bar)),
+        "r"(one)
+        : "memory");
 }
 __device__ __forceinline__ void FenceBefore() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void FenceAfter() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
@@ -123,12 +126,20 @@ __device__ __forceinline__ uint32_t Instruction(int n, bool b_mn) {
     return (1u << 4) | (b_mn ? 1u << 16 : 0u) | (static_cast<uint32_t>(n >> 3) << 17) | (8u << 24);
 }
 
-// A from tensor memory, B from shared memory.
-__device__ __forceinline__ void MmaTensor(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+// One lane of the (converged) warp.
+__device__ __forceinline__ uint32_t ElectOne() {
+    uint32_t e;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}\n" : "=r"(e));
+    return e;
+}
+// A from tensor memory, B from shared memory; the whole warp comes here with the
+// same operands, so that they stay in uniform registers, and `one` lane issues.
+template <bool ACCUMULATE>
+__device__ __forceinline__ void MmaTensor(uint32_t one, uint32_t d, uint32_t a, uint64_t b, uint32_t idesc) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %5, %5, %5}, p;\n\t}\n" ::"r"(d),
-        "r"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(0));
+        "{\n\t.reg .pred p, e;\n\tsetp.ne.b32 e, %0, 0;\n\tsetp.ne.b32 p, %5, 0;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%1], [%2], %3, %4, {%6, %6, %6, %6}, p;\n\t}\n" ::"r"(one),
+        "r"(d), "r"(a), "l"(b), "r"(idesc), "n"(ACCUMULATE ? 1 : 0), "r"(0));
 }
 
 // 16 columns of the warp's 32 lanes.
@@ -290,6 +301,7 @@ struct Share {
                 Product(p[3], s, hi.w, lo.w);
                 *reinterpret_cast<uint4*>(to + c * kChunkPitch) = hi;
                 *reinterpret_cast<uint4*>(to + c * kChunkPitch + kLo) = lo;
+                asm volatile("" ::: "memory");  // one chunk's registers at a time
             }
         }
     }
@@ -610,7 +622,7 @@ __global__ void __launch_bounds__(kTcWarps * 32, 1) TreeTcKernel(TreeArgs a, Tre
     } else {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kMmaRegs));
     }
-    if (warp == kMmaWarp && lane == 0) {
+    if (warp == kMmaWarp) {
         // ------------------------------------------------ MMA issue
         const uint32_t qk = Instruction(kTile, false), pv = Instruction(HD, true);
         // K-major images: chunks of K kChunkPitch bytes apart, groups of 8 rows 128
@@ -618,42 +630,45 @@ __global__ void __launch_bounds__(kTcWarps * 32, 1) TreeTcKernel(TreeArgs a, Tre
         // V: groups of 8 slots 128 bytes apart, groups of 8 of head_dim kChunkPitch
         const uint64_t vd = Descriptor(SmemAddr(vi), 128, kChunkPitch);
         constexpr uint64_t kLoStep = kImage >> 4, kKStep = (2 * kChunkPitch) >> 4, kVStep = 256 >> 4;
+        const uint32_t one = ElectOne(), base = __shfl_sync(0xffffffffu, tmem, 0);
         int it = 0, item = 0;
         bool ok = true;
         auto values = [&](int n) {  // PV of running tile n
-            if (!WaitOne(sh, &sh.v_full, n & 1, status) || !WaitOne(sh, &sh.p_full[n & 1], (n >> 1) & 1, status)) return false;
-            if (n > 0 && !WaitOne(sh, &sh.o_empty, (n - 1) & 1, status)) return false;  // the last O has been read
+            if (!Wait(sh, &sh.v_full, n & 1, status) || !Wait(sh, &sh.p_full[n & 1], (n >> 1) & 1, status)) return false;
+            if (n > 0 && !Wait(sh, &sh.o_empty, (n - 1) & 1, status)) return false;  // the last O has been read
             FenceAfter();
-            const uint32_t p = tmem + (n & 1) * kTile;
-#pragma unroll 2
-            for (int s = 0; s < kTile / 16; ++s) MmaTensor(tmem + kOCol, p + 16 * s + 8, vd + s * kVStep, pv, s != 0);
-#pragma unroll 2
-            for (int s = 0; s < kTile / 16; ++s) MmaTensor(tmem + kOCol, p + 16 * s, vd + kLoStep + s * kVStep, pv, 1);
-#pragma unroll 2
-            for (int s = 0; s < kTile / 16; ++s) MmaTensor(tmem + kOCol, p + 16 * s, vd + s * kVStep, pv, 1);
-            Commit(&sh.v_empty);
-            Commit(&sh.o_full);
+            const uint32_t p = base + (n & 1) * kTile;
+            MmaTensor<false>(one, base + kOCol, p + 8, vd, pv);
+#pragma unroll
+            for (int s = 1; s < kTile / 16; ++s) MmaTensor<true>(one, base + kOCol, p + 16 * s + 8, vd + s * kVStep, pv);
+#pragma unroll
+            for (int s = 0; s < kTile / 16; ++s) MmaTensor<true>(one, base + kOCol, p + 16 * s, vd + kLoStep + s * kVStep, pv);
+#pragma unroll
+            for (int s = 0; s < kTile / 16; ++s) MmaTensor<true>(one, base + kOCol, p + 16 * s, vd + s * kVStep, pv);
+            Commit(one, &sh.v_empty);
+            Commit(one, &sh.o_full);
             return true;
         };
         while (ok && walk.Next(a, sp, items)) {
-            if (!(ok = WaitOne(sh, &sh.q_full, item & 1, status))) break;
+            if (!(ok = Wait(sh, &sh.q_full, item & 1, status))) break;
             ++item;
             for (int u = walk.u0; u < walk.u1; ++u, ++it) {
-                if (!(ok = WaitOne(sh, &sh.k_full[it & 1], (it >> 1) & 1, status))) break;
+                if (!(ok = Wait(sh, &sh.k_full[it & 1], (it >> 1) & 1, status))) break;
                 // The weights that lay in this buffer, of tile it - 2, have been multiplied: its PV is the one issued
                 // last, but at the start of an item, where PV(it - 1) has been issued after O(it - 2) was read.
-                if (it > 1 && u > walk.u0 && !(ok = WaitOne(sh, &sh.o_full, it & 1, status))) break;
+                if (it > 1 && u > walk.u0 && !(ok = Wait(sh, &sh.o_full, it & 1, status))) break;
                 FenceAfter();
-                const uint32_t d = tmem + (it & 1) * kTile, q = tmem + kQCol;
+                const uint32_t d = base + (it & 1) * kTile, q = base + kQCol;
                 const uint64_t k = kd + (it & 1) * 2 * kLoStep;
-#pragma unroll 2
-                for (int s = 0; s < HD / 16; ++s) MmaTensor(d, q + 16 * s + 8, k + s * kKStep, qk, s != 0);
-#pragma unroll 2
-                for (int s = 0; s < HD / 16; ++s) MmaTensor(d, q + 16 * s, k + kLoStep + s * kKStep, qk, 1);
-#pragma unroll 2
-                for (int s = 0; s < HD / 16; ++s) MmaTensor(d, q + 16 * s, k + s * kKStep, qk, 1);
-                Commit(&sh.k_empty[it & 1]);
-                Commit(&sh.s_full[it & 1]);
+                MmaTensor<false>(one, d, q + 8, k, qk);
+#pragma unroll
+                for (int s = 1; s < HD / 16; ++s) MmaTensor<true>(one, d, q + 16 * s + 8, k + s * kKStep, qk);
+#pragma unroll
+                for (int s = 0; s < HD / 16; ++s) MmaTensor<true>(one, d, q + 16 * s, k + kLoStep + s * kKStep, qk);
+#pragma unroll
+                for (int s = 0; s < HD / 16; ++s) MmaTensor<true>(one, d, q + 16 * s, k + s * kKStep, qk);
+                Commit(one, &sh.k_empty[it & 1]);
+                Commit(one, &sh.s_full[it & 1]);
                 if (u > walk.u0 && !(ok = values(it - 1))) {
                     ++it;
                     break;
@@ -662,7 +677,7 @@ __global__ void __launch_bounds__(kTcWarps * 32, 1) TreeTcKernel(TreeArgs a, Tre
             if (ok) ok = values(it - 1);
         }
         // every MMA issued has finished before tensor memory is freed
-        Commit(&sh.drain);
+        Commit(one, &sh.drain);
         if (!MbarWaitFor(&sh.drain, 0, kTcWait, nullptr)) Fail(sh, status);
     }
     FenceBefore();
