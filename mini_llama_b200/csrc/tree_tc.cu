@@ -29,7 +29,7 @@
 //          maximum and for the weights, so that a thread holds 16 at a time.  Q goes
 //          into tensor memory once per item: as an A operand there it leaves half of
 //          shared memory's bandwidth to the producers
-//   8-15   producers: quants in registers a tile ahead of the images,
+//   8-15   producers: quants in registers an image ahead,
 //          converted into the operand images (no swizzle: 16-byte chunks of eight
 //          elements, chunk c of row r at 2064 c + 16 r)
 //   16     tensor memory (17-19 idle); issues all MMAs: QK(i + 1) before PV(i), so that
@@ -52,8 +52,8 @@ constexpr int kProdWarps = 8;    // producer warps
 constexpr int kMmaWarp = kSoftWarps + kProdWarps;
 constexpr int kTcWarps = kMmaWarp + 4;  // a whole warpgroup, for the register split
 // Registers of a softmax, a producer and an MMA thread: five warpgroups launched
-// with 96 each, 2 x 128 + 2 x 88 + 48 of their 5 x 96.
-constexpr int kSoftRegs = 128, kProdRegs = 88, kMmaRegs = 48;
+// with 96 each, 2 x 136 + 2 x 80 + 48 of their 5 x 96.
+constexpr int kSoftRegs = 136, kProdRegs = 80, kMmaRegs = 48;
 static_assert(2 * kSoftRegs + 2 * kProdRegs + kMmaRegs <= 5 * 96, "setmaxnreg draws on the launch's registers");
 constexpr int kProducers = kProdWarps * 32;
 constexpr int kQCol = 2 * kTile, kOCol = 3 * kTile;  // tensor-memory columns of Q and of O
@@ -418,109 +418,107 @@ __global__ void __launch_bounds__(kTcWarps * 32, 1) TreeTcKernel(TreeArgs a, Tre
                 FenceBefore();
                 Arrive(&sh.q_full);
             }
-            float o[kHalf], m = kStart, l = 0.0f, m_of_o = kStart, m_last = kStart;
+            float o[kHalf], m = kStart, l0 = 0.0f, l1 = 0.0f, m_of_o = kStart, m_last = kStart;
             uint32_t poison = 0;
 #pragma unroll
             for (int i = 0; i < kHalf; ++i) o[i] = 0.0f;
             const uint64_t* mask = a.mask ? a.mask + size_t(walk.b) * a.tokens * a.words : nullptr;
 
-            // adds O of the item's tile u (running number n, complete) to the row
-            auto add = [&](int u, int n) {
-                const float keep = Exp2(m_of_o - m_last);
-                m_of_o = m_last;
-                const bool big = sh.v_big[n % kInfoBufs];
-#pragma unroll
-                for (int i = 0; i < kHalf; i += 16) {
-                    float d[16];
-                    Load16(lanes + kOCol + half * kHalf + i, d);
-                    WaitLoad();
-                    if (big)
-#pragma unroll
-                        for (int j = 0; j < 16; ++j) d[j] *= 512.0f;
-#pragma unroll
-                    for (int j = 0; j < 16; ++j) o[i + j] = fmaf(o[i + j], keep, d[j]);
-                }
-                if (sh.v_odd[n % kInfoBufs]) {
-#pragma unroll 1
-                    for (int k = 0; k < kTile / 32; ++k) {
-                        const uint32_t seen = SeenBits(mask, a.words, a.tokens, t, u * kTile + 32 * k, walk.e.len, walk.e.slots);
-                        for (int b = 0; b < NB; ++b)
-                            if (seen & sh.v_bad[n % kInfoBufs][b][k]) poison |= 1u << b;
-                    }
-                }
-                FenceBefore();
-                Arrive(&sh.o_empty);
-            };
-
-            for (int u = walk.u0; u < walk.u1; ++u, ++it) {
-                const uint32_t scores = lanes + (it & 1) * kTile + half * 64;
-                if (!(ok = Wait(sh, &sh.s_full[it & 1], (it >> 1) & 1, status))) break;
-                FenceAfter();
-                uint32_t seen[2] = {0xffffffffu, 0xffffffffu};
-                const bool edge = (u + 1) * kTile > walk.e.len;
-                if (edge)
-#pragma unroll
-                    for (int k = 0; k < 2; ++k)
-                        seen[k] = SeenBits(mask, a.words, a.tokens, t, u * kTile + half * 64 + 32 * k, walk.e.len, walk.e.slots);
-                auto hide = [&](float (&x)[16], int i) {
-                    if (edge)
-#pragma unroll
-                        for (int j = 0; j < 16; ++j)
-                            if (!((seen[i >> 5] >> ((i & 31) + j)) & 1)) x[j] = -INFINITY;
-                };
-                float top = -INFINITY;
-#pragma unroll
-                for (int i = 0; i < 64; i += 16) {
-                    float x[16];
-                    Load16(scores + i, x);
-                    WaitLoad();
-                    hide(x, i);
-#pragma unroll
-                    for (int j = 0; j < 16; ++j) top = fmaxf(top, x[j]);
-                }
-                sh.top[it & 1][half][row] = top;
-                if (!(ok = Meet(sh, &sh.soft, met, status))) break;
-                const float c = sh.k_big[it % kInfoBufs] ? cs * 512.0f : cs;
-                top = fmaxf(top, sh.top[it & 1][half ^ 1][row]) * c;
-                if (top > m + kLag) {
-                    l *= Exp2(m - top);
-                    m = top;
-                }
-                const float off = kOffset - m;
-#pragma unroll
-                for (int i = 0; i < 64; i += 16) {
-                    float x[16];
-                    Load16(scores + i, x);
-                    WaitLoad();
-                    hide(x, i);
-                    uint32_t hi[8], lo[8];
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        const float p0 = Exp2(fmaf(x[2 * j], c, off)), p1 = Exp2(fmaf(x[2 * j + 1], c, off));
-                        l += p0 + p1;
-                        SplitHalf(p0, p1, hi[j], lo[j]);
-                    }
-                    Store8(scores + i, hi);
-                    Store8(scores + i + 8, lo);
-                }
-                WaitStore();
-                FenceBefore();
-                Arrive(&sh.p_full[it & 1]);
-                if (u > walk.u0) {
-                    if (!(ok = Wait(sh, &sh.o_full, (it - 1) & 1, status))) break;
+            // Tile u's weights, then O of tile u - 1 (whose PV has had the time of a QK to finish).  The code of the
+            // roles together has to stay in the instruction cache: loops are unrolled only where registers ask for it.
+            for (int u = walk.u0; u <= walk.u1; ++u) {
+                if (u < walk.u1) {
+                    const uint32_t scores = lanes + (it & 1) * kTile + half * 64;
+                    if (!(ok = Wait(sh, &sh.s_full[it & 1], (it >> 1) & 1, status))) break;
                     FenceAfter();
-                    add(u - 1, it - 1);
+                    const bool edge = (u + 1) * kTile > walk.e.len;
+                    // 16 scores, those that the row does not see taken out
+                    auto get = [&](float (&x)[16], int i) {
+                        Load16(scores + i, x);
+                        uint32_t seen = 0xffffu;
+                        if (edge)
+                            seen = SeenBits(mask, a.words, a.tokens, t, u * kTile + half * 64 + i, walk.e.len, walk.e.slots);
+                        WaitLoad();
+                        if (edge)
+#pragma unroll
+                            for (int j = 0; j < 16; ++j)
+                                if (!((seen >> j) & 1)) x[j] = -INFINITY;
+                    };
+                    float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll 1
+                    for (int i = 0; i < 64; i += 16) {
+                        float x[16];
+                        get(x, i);
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) tops[j & 3] = fmaxf(tops[j & 3], x[j]);
+                    }
+                    float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+                    sh.top[it & 1][half][row] = top;
+                    if (!(ok = Meet(sh, &sh.soft, met, status))) break;
+                    const float c = sh.k_big[it % kInfoBufs] ? cs * 512.0f : cs;
+                    top = fmaxf(top, sh.top[it & 1][half ^ 1][row]) * c;
+                    m_last = m;
+                    if (top > m + kLag) {
+                        const float f = Exp2(m - top);
+                        l0 *= f;
+                        l1 *= f;
+                        m = top;
+                    }
+                    const float off = kOffset - m;
+#pragma unroll 1
+                    for (int i = 0; i < 64; i += 16) {
+                        float x[16];
+                        get(x, i);
+                        uint32_t hi[8], lo[8];
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) {
+                            const float p0 = Exp2(fmaf(x[2 * j], c, off)), p1 = Exp2(fmaf(x[2 * j + 1], c, off));
+                            l0 += p0;
+                            l1 += p1;
+                            SplitHalf(p0, p1, hi[j], lo[j]);
+                        }
+                        Store8(scores + i, hi);
+                        Store8(scores + i + 8, lo);
+                    }
+                    WaitStore();
+                    FenceBefore();
+                    Arrive(&sh.p_full[it & 1]);
+                } else {
+                    m_last = m;
                 }
-                m_last = m;
+                if (u > walk.u0) {
+                    const int n = it - 1;
+                    if (!(ok = Wait(sh, &sh.o_full, n & 1, status))) break;
+                    FenceAfter();
+                    const float keep = Exp2(m_of_o - m_last);
+                    m_of_o = m_last;
+                    const float times = sh.v_big[n % kInfoBufs] ? 512.0f : 1.0f;
+#pragma unroll
+                    for (int i = 0; i < kHalf; i += 16) {
+                        float d[16];
+                        Load16(lanes + kOCol + half * kHalf + i, d);
+                        WaitLoad();
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) o[i + j] = fmaf(d[j], times, o[i + j] * keep);
+                    }
+                    if (sh.v_odd[n % kInfoBufs])
+#pragma unroll 1
+                        for (int k = 0; k < kTile / 32; ++k) {
+                            const uint32_t seen =
+                                SeenBits(mask, a.words, a.tokens, t, (u - 1) * kTile + 32 * k, walk.e.len, walk.e.slots);
+                            for (int b = 0; b < NB; ++b)
+                                if (seen & sh.v_bad[n % kInfoBufs][b][k]) poison |= 1u << b;
+                        }
+                    FenceBefore();
+                    Arrive(&sh.o_empty);
+                }
+                if (u < walk.u1) ++it;
             }
-            ok = ok && Wait(sh, &sh.o_full, (it - 1) & 1, status);
             if (!ok) break;
-            FenceAfter();
-            add(walk.u1 - 1, it - 1);
             // ---- the row's result, or its part of it
-            sh.last[half][row] = l;
+            sh.last[half][row] = l0 + l1;
             if (!(ok = Meet(sh, &sh.soft, met, status))) break;
-            l = sh.last[0][row] + sh.last[1][row];
+            const float l = sh.last[0][row] + sh.last[1][row];
             if (live) {
 #pragma unroll
                 for (int i = 0; i < kHalf; ++i)
@@ -569,28 +567,28 @@ __global__ void __launch_bounds__(kTcWarps * 32, 1) TreeTcKernel(TreeArgs a, Tre
             const uint8_t* kp = static_cast<const uint8_t*>(a.c.k) + base * kRowBytes;
             const uint8_t* vp = static_cast<const uint8_t*>(a.c.v) + base * kRowBytes;
             const __half *ks = a.c.ks + base * NB, *vs = a.c.vs + base * NB;
-            Share<TYPE, NB> rk, rv;
-            auto load = [&](Share<TYPE, NB>& r, const uint8_t* plane, const __half* scales, int u) {
-                r.Load(plane, scales, u * kTile, walk.e.slots, a.c.head_slots - 1, id);
-            };
-            auto put_k = [&](int u) {
-                const bool big = together(rk.Big()) != 0;
-                if (!ok) return;
-                if (kt > 1 && !(ok = Wait(sh, &sh.k_empty[kt & 1], ((kt >> 1) - 1) & 1, status))) return;
-                if (id == 0) sh.k_big[kt % kInfoBufs] = big;
-                rk.Convert(ki + (kt & 1) * 2 * kImage, id, big, sp.magic);
-                FenceAsync();
-                Arrive(&sh.k_full[kt & 1]);
-                ++kt;
-                if (u + 1 < walk.u1) load(rk, kp, ks, u + 1);
-            };
-            auto put_v = [&](int u) {
-                // a drafted slot's scale that is not finite is taken out and noted
-                const bool odd = rv.TakeOdd(walk.e.len - u * kTile, id);
-                const uint32_t flags = together((rv.Big() ? 1u : 0u) | (odd ? 2u : 0u));
-                if (!ok) return;
+            // The images in the order of their use: K(0), K(1), V(0), K(2), V(1), ..; the quants of the next one are
+            // under way while this one waits for its place.
+            const int tiles = walk.u1 - walk.u0, all = 2 * tiles;
+            auto is_v = [&](int i) { return (i >= 2 && !(i & 1)) || i == all - 1; };
+            auto tile = [&](int i) { return walk.u0 + (is_v(i) ? (i == all - 1 ? tiles - 1 : i / 2 - 1) : (i + 1) / 2); };
+            Share<TYPE, NB> r;
+            r.Load(kp, ks, walk.u0 * kTile, walk.e.slots, a.c.head_slots - 1, id);
+#pragma unroll 1
+            for (int i = 0; i < all; ++i) {
+                const bool v = is_v(i);
+                const int u = tile(i);
+                // a drafted slot's V scale that is not finite is taken out and noted
+                const bool odd = v && r.TakeOdd(walk.e.len - u * kTile, id);
+                const uint32_t flags = together((r.Big() ? 1u : 0u) | (odd ? 2u : 0u));
+                if (!ok) break;
                 const bool big = flags & 1, any = flags & 2;
-                if (vt > 0 && !(ok = Wait(sh, &sh.v_empty, (vt - 1) & 1, status))) return;
+                const int n = v ? vt++ : kt++;
+                if (v) {
+                    if (n > 0 && !(ok = Wait(sh, &sh.v_empty, (n - 1) & 1, status))) break;
+                } else {
+                    if (n > 1 && !(ok = Wait(sh, &sh.k_empty[n & 1], ((n >> 1) - 1) & 1, status))) break;
+                }
                 if (any && id < kTile) {  // a row for each of four warps' threads
                     const int at = u * kTile + id;
                     for (int b = 0; b < NB; ++b) {
@@ -598,28 +596,23 @@ __global__ void __launch_bounds__(kTcWarps * 32, 1) TreeTcKernel(TreeArgs a, Tre
                             __ldg(reinterpret_cast<const unsigned short*>(vs + size_t(min(at, a.c.head_slots - 1)) * NB + b));
                         const bool bad = (d & 0x7C00u) == 0x7C00u && at >= walk.e.len && at < walk.e.slots;
                         const uint32_t bits = __ballot_sync(0xffffffffu, bad);
-                        if (lane == 0) sh.v_bad[vt % kInfoBufs][b][id / 32] = bits;
+                        if (lane == 0) sh.v_bad[n % kInfoBufs][b][id / 32] = bits;
                     }
                 }
                 if (id == 0) {
-                    sh.v_big[vt % kInfoBufs] = big;
-                    sh.v_odd[vt % kInfoBufs] = any;
+                    (v ? sh.v_big : sh.k_big)[n % kInfoBufs] = big;
+                    if (v) sh.v_odd[n % kInfoBufs] = any;
                 }
-                rv.Convert(vi, id, big, sp.magic);
+                r.Convert(v ? vi : ki + (n & 1) * 2 * kImage, id, big, sp.magic);
                 FenceAsync();
-                Arrive(&sh.v_full);
-                ++vt;
-                if (u + 1 < walk.u1) load(rv, vp, vs, u + 1);
-            };
-            load(rk, kp, ks, walk.u0);
-            load(rv, vp, vs, walk.u0);
-            put_k(walk.u0);
-            for (int u = walk.u0; ok && u < walk.u1; ++u) {
-                if (u + 1 < walk.u1) put_k(u + 1);
-                if (ok) put_v(u);
+                Arrive(v ? &sh.v_full : &sh.k_full[n & 1]);
+                if (i + 1 < all) {
+                    const bool w = is_v(i + 1);
+                    r.Load(w ? vp : kp, w ? vs : ks, tile(i + 1) * kTile, walk.e.slots, a.c.head_slots - 1, id);
+                }
             }
         }
-    } else {
+    } else if (warp >= kMmaWarp) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kMmaRegs));
     }
     if (warp == kMmaWarp) {
@@ -633,48 +626,48 @@ __global__ void __launch_bounds__(kTcWarps * 32, 1) TreeTcKernel(TreeArgs a, Tre
         const uint32_t one = ElectOne(), base = __shfl_sync(0xffffffffu, tmem, 0);
         int it = 0, item = 0;
         bool ok = true;
-        auto values = [&](int n) {  // PV of running tile n
-            if (!Wait(sh, &sh.v_full, n & 1, status) || !Wait(sh, &sh.p_full[n & 1], (n >> 1) & 1, status)) return false;
-            if (n > 0 && !Wait(sh, &sh.o_empty, (n - 1) & 1, status)) return false;  // the last O has been read
-            FenceAfter();
-            const uint32_t p = base + (n & 1) * kTile;
-            MmaTensor<false>(one, base + kOCol, p + 8, vd, pv);
-#pragma unroll
-            for (int s = 1; s < kTile / 16; ++s) MmaTensor<true>(one, base + kOCol, p + 16 * s + 8, vd + s * kVStep, pv);
-#pragma unroll
-            for (int s = 0; s < kTile / 16; ++s) MmaTensor<true>(one, base + kOCol, p + 16 * s, vd + kLoStep + s * kVStep, pv);
-#pragma unroll
-            for (int s = 0; s < kTile / 16; ++s) MmaTensor<true>(one, base + kOCol, p + 16 * s, vd + s * kVStep, pv);
-            Commit(one, &sh.v_empty);
-            Commit(one, &sh.o_full);
-            return true;
-        };
         while (ok && walk.Next(a, sp, items)) {
             if (!(ok = Wait(sh, &sh.q_full, item & 1, status))) break;
             ++item;
-            for (int u = walk.u0; u < walk.u1; ++u, ++it) {
-                if (!(ok = Wait(sh, &sh.k_full[it & 1], (it >> 1) & 1, status))) break;
-                // The weights that lay in this buffer, of tile it - 2, have been multiplied: its PV is the one issued
-                // last, but at the start of an item, where PV(it - 1) has been issued after O(it - 2) was read.
-                if (it > 1 && u > walk.u0 && !(ok = Wait(sh, &sh.o_full, it & 1, status))) break;
-                FenceAfter();
-                const uint32_t d = base + (it & 1) * kTile, q = base + kQCol;
-                const uint64_t k = kd + (it & 1) * 2 * kLoStep;
-                MmaTensor<false>(one, d, q + 8, k, qk);
+            for (int u = walk.u0; u <= walk.u1; ++u) {
+                if (u < walk.u1) {  // QK of tile `it`
+                    if (!(ok = Wait(sh, &sh.k_full[it & 1], (it >> 1) & 1, status))) break;
+                    // The weights that lay in this buffer, of tile it - 2, have been multiplied: its PV is the one issued
+                    // last, but at the start of an item, where PV(it - 1) has been issued after O(it - 2) was read.
+                    if (it > 1 && u > walk.u0 && !(ok = Wait(sh, &sh.o_full, it & 1, status))) break;
+                    FenceAfter();
+                    const uint32_t d = base + (it & 1) * kTile, q = base + kQCol;
+                    const uint64_t k = kd + (it & 1) * 2 * kLoStep;
+                    MmaTensor<false>(one, d, q + 8, k, qk);
 #pragma unroll
-                for (int s = 1; s < HD / 16; ++s) MmaTensor<true>(one, d, q + 16 * s + 8, k + s * kKStep, qk);
+                    for (int s = 1; s < HD / 16; ++s) MmaTensor<true>(one, d, q + 16 * s + 8, k + s * kKStep, qk);
 #pragma unroll
-                for (int s = 0; s < HD / 16; ++s) MmaTensor<true>(one, d, q + 16 * s, k + kLoStep + s * kKStep, qk);
+                    for (int s = 0; s < HD / 16; ++s) MmaTensor<true>(one, d, q + 16 * s, k + kLoStep + s * kKStep, qk);
 #pragma unroll
-                for (int s = 0; s < HD / 16; ++s) MmaTensor<true>(one, d, q + 16 * s, k + s * kKStep, qk);
-                Commit(one, &sh.k_empty[it & 1]);
-                Commit(one, &sh.s_full[it & 1]);
-                if (u > walk.u0 && !(ok = values(it - 1))) {
-                    ++it;
-                    break;
+                    for (int s = 0; s < HD / 16; ++s) MmaTensor<true>(one, d, q + 16 * s, k + s * kKStep, qk);
+                    Commit(one, &sh.k_empty[it & 1]);
+                    Commit(one, &sh.s_full[it & 1]);
                 }
+                if (u > walk.u0) {  // PV of the tile before
+                    const int n = it - 1;
+                    if (!(ok = Wait(sh, &sh.v_full, n & 1, status) && Wait(sh, &sh.p_full[n & 1], (n >> 1) & 1, status))) break;
+                    if (n > 0 && !(ok = Wait(sh, &sh.o_empty, (n - 1) & 1, status))) break;  // the last O has been read
+                    FenceAfter();
+                    const uint32_t p = base + (n & 1) * kTile;
+                    MmaTensor<false>(one, base + kOCol, p + 8, vd, pv);
+#pragma unroll
+                    for (int s = 1; s < kTile / 16; ++s)
+                        MmaTensor<true>(one, base + kOCol, p + 16 * s + 8, vd + s * kVStep, pv);
+#pragma unroll
+                    for (int s = 0; s < kTile / 16; ++s)
+                        MmaTensor<true>(one, base + kOCol, p + 16 * s, vd + kLoStep + s * kVStep, pv);
+#pragma unroll
+                    for (int s = 0; s < kTile / 16; ++s) MmaTensor<true>(one, base + kOCol, p + 16 * s, vd + s * kVStep, pv);
+                    Commit(one, &sh.v_empty);
+                    Commit(one, &sh.o_full);
+                }
+                if (u < walk.u1) ++it;
             }
-            if (ok) ok = values(it - 1);
         }
         // every MMA issued has finished before tensor memory is freed
         Commit(one, &sh.drain);
