@@ -238,3 +238,74 @@ class BatchSession:
         if self.handle:
             self.lib.call("mlb_batch_destroy", self.handle)
             self.handle = None
+
+
+class RopeTable:
+    """Rotation angles of n_positions positions on the device (mlb_rope_table), optionally scaled
+    (scale: a capi.RopeScale)."""
+
+    def __init__(self, lib: capi.Lib, device: int, n_positions: int, head_dim: int, theta: float,
+                 rope_type: int = capi.ROPE_NORMAL, rot_dim: int | None = None, scale=None):
+        self.lib, self.device = lib, device
+        rot = head_dim if rot_dim is None else rot_dim
+        self.angles = DeviceArray(lib, device, (n_positions, rot // 2, 2))
+        self.desc = capi.RopeTable(n_positions=n_positions, head_dim=head_dim, rot_dim=rot,
+                                   rope_type=rope_type, cos_sin=self.angles.ptr)
+        lib.call("mlb_rope_table_fill", device, ctypes.byref(self.desc), theta,
+                 ctypes.byref(scale) if scale is not None else None)
+
+    @property
+    def ref(self):
+        return ctypes.byref(self.desc)
+
+    def rotate(self, rows: int, positions: int, q: int, n_heads: int, k: int, n_kv_heads: int):
+        """Rotates contiguous rows of q and k in place (device pointers)."""
+        hd = self.desc.head_dim
+        self.lib.call("mlb_rope_rows", self.device, self.ref, rows, positions, q, n_heads * hd, q,
+                      n_heads * hd, n_heads, k, n_kv_heads * hd, k, n_kv_heads * hd, n_kv_heads)
+
+
+class KvCache:
+    """A KV cache (mlb_kv_cache) of F32, Q8_0 or Q4_0 values with its planes; rows of K, V and queries are
+    contiguous device arrays, passed by pointer."""
+
+    def __init__(self, lib: capi.Lib, device: int, qtype: int, n_seqs: int, n_layers: int,
+                 max_seq_len: int, n_kv_heads: int, head_dim: int):
+        self.lib, self.device = lib, device
+        self.row = n_kv_heads * head_dim
+        self.desc = capi.KvCache(type=qtype, n_seqs=n_seqs, n_layers=n_layers,
+                                 max_seq_len=max_seq_len, n_kv_heads=n_kv_heads, head_dim=head_dim)
+        plane, scale = ctypes.c_size_t(), ctypes.c_size_t()
+        lib.call("mlb_kv_cache_bytes", self.ref, ctypes.byref(plane), ctypes.byref(scale))
+        self.planes = [DeviceArray(lib, device, n, np.uint8) for n in (plane.value,) * 2 + (scale.value,) * 2]
+        self.desc.k, self.desc.v = self.planes[0].ptr, self.planes[1].ptr
+        if scale.value:
+            self.desc.k_scale, self.desc.v_scale = self.planes[2].ptr, self.planes[3].ptr
+
+    @property
+    def ref(self):
+        return ctypes.byref(self.desc)
+
+    def nbytes(self) -> int:
+        return sum(p.nbytes for p in self.planes)
+
+    def write(self, layer: int, rows: int, slots: int, k: int, v: int, seqs: int | None = None):
+        self.lib.call("mlb_kv_cache_write", self.device, self.ref, layer, rows, seqs, slots, k, self.row, v,
+                      self.row)
+
+    def write_rope(self, layer: int, rows: int, slots: int, table: RopeTable, positions: int, q: int | None,
+                   n_heads: int, k: int, v: int, seqs: int | None = None):
+        """q is rotated in place; n_heads 0: k and v only."""
+        width = n_heads * self.desc.head_dim
+        self.lib.call("mlb_kv_cache_write_rope", self.device, self.ref, layer, rows, seqs, slots, table.ref,
+                      positions, q, width, q, width, n_heads, k, self.row, v, self.row)
+
+    def read(self, layer: int, rows: int, slots: int, k: int, v: int, seqs: int | None = None):
+        self.lib.call("mlb_kv_cache_read", self.device, self.ref, layer, rows, seqs, slots, k, self.row, v,
+                      self.row)
+
+    def attend(self, layer: int, batch: int, tokens: int, lens: int, max_len: int, q: int, n_heads: int,
+               out: int, mask: int | None = None, seqs: int | None = None, scale: float = 0.0):
+        width = n_heads * self.desc.head_dim
+        self.lib.call("mlb_attention_tree", self.device, self.ref, layer, batch, tokens, seqs, lens, max_len,
+                      mask, q, width, n_heads, scale, out, width)

@@ -532,6 +532,27 @@ def test_repeated_calls_and_changing_shapes(mlb, gpu):
     assert same_bits(first, runs[0])
 
 
+@pytest.mark.parametrize("qtype", [Q80, Q40], ids=NAME.get)
+@pytest.mark.parametrize("heads,kv,hd,tokens,length,n_seqs", [(16, 4, 32, 12, 700, 48), (64, 8, 64, 20, 400, 24),
+                                                              (33, 1, 128, 1, 1500, 2)])
+def test_many_items_to_a_cta(mlb, gpu, qtype, heads, kv, hd, tokens, length, n_seqs):
+    """More row groups than SMs, several tiles each: the tensor-memory kernel's roles walk from item to item.  Every
+    wait there is bounded; one that expired shows at the synchronisation."""
+    rng = np.random.default_rng(length)
+    max_seq = length + tokens
+    c, k, v = filled(mlb, gpu, rng, qtype, n_seqs, max_seq, kv, hd)
+    q = rng.standard_normal((n_seqs, tokens, heads, hd)).astype(np.float32)
+    mask = np.stack([random_tree(rng, tokens) for _ in range(n_seqs)])
+    lens = [length - 13 * i for i in range(n_seqs)]
+    got = run_attention(mlb, gpu, c, 0, q, None, lens, length, mask)
+    for _ in range(3):
+        assert same_bits(got, run_attention(mlb, gpu, c, 0, q, None, lens, length, mask))
+    mlb.sync(gpu)
+    some = [0, n_seqs // 2, n_seqs - 1]
+    want = ref.attention(q[some], k[some], v[some], [lens[i] for i in some], range(len(some)), mask[some], hd ** -0.5, max_seq)
+    assert_attention(got[some], *want)
+
+
 def test_empty_calls(mlb, gpu):
     c = Cache(mlb, gpu, Q80, 1, 1, 8, 1, 32)
     mlb.call("mlb_kv_cache_write", gpu, c.ref, 0, 0, None, None, None, 32, None, 32)
