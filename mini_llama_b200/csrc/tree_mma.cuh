@@ -3,7 +3,7 @@
 //
 // The R = tokens x (query heads per KV head) rows that share a KV head are cut
 // into tiles of eight: the N side of mma.m16n8k16.  A warp takes 16 slots of
-// the cache at a time (the M side, S^T = K Q^T) for NT = 1 or 2 tiles of rows:
+// the cache at a time (the M side, S^T = K Q^T) for a tile of rows (fp32: NT = 1 or 2):
 //   K      the 16 x head_dim quants as A fragments (the order of the elements
 //          within a block is free, as Q is laid out in the same one), fp16 whole
 //          numbers: exact.  Q is scaled per row by a power of two and split into
@@ -54,10 +54,6 @@ constexpr float kLog2e = 1.4426950408889634f;
 
 constexpr int kSmShared = 226 * 1024;  // shared memory of an SM for its CTAs
 constexpr int kMaxStages = 4;
-#ifndef TREE_NW4
-#define TREE_NW4 4
-#define TREE_PER4 3
-#endif
 
 struct TreeSplit {
     int groups;    // items of a (sequence, KV head): ceil(R / (8 NT WQ))
@@ -304,10 +300,12 @@ __device__ __forceinline__ uint32_t LoadHalf(uint32_t at, int more) {
 }
 
 // ---------------------------------------------------------------- quantized caches
-// A warp's running result for NT tiles of rows over Q8_0 / Q4_0 slots, H steps
-// of 16 slots to a unit.
-template <int TYPE, int NB, int NT, int H>
+// A warp's running result for a tile of rows over Q8_0 / Q4_0 slots, two steps of
+// 16 slots to a unit: half the sums of the fresh accumulators and half the loads
+// of Q of one step.
+template <int TYPE, int NB>
 struct QuantWarp {
+    static constexpr int H = 2;
     static constexpr int kUnit = kSlots * H;
     static constexpr int kQuantBytes = TYPE == MLB_Q8_0 ? 32 : 16;
     static constexpr int kChunks = NB * kQuantBytes / 16;  // of a row
@@ -320,13 +318,13 @@ struct QuantWarp {
     static_assert(!kXor || kStageBytes % 128 == 0, "the chunk bits of a stage's address are free");
     static constexpr int kFrags = 2 * NB;                  // uint4 per lane and tile: (hi, hi, lo, lo)
 
-    Values<NB> v[NT];
-    Columns col[NT];
-    int e[NT];         // of row g: P' is relative to 2^e
-    float bound[NT];   // 2^e
-    __half2 down[NT];  // 2^-e
+    Values<NB> v[1];
+    Columns col[1];
+    int e;         // of row g: P' is relative to 2^e
+    float bound;   // 2^e
+    __half2 down;  // 2^-e
     // weights of the unit as B fragments: row (query) g, slots 2c, 2c + 1 (+ 8), hi and lo
-    uint32_t ph[NT][H][2], pl[NT][H][2];
+    uint32_t ph[H][2], pl[H][2];
     bool edge;         // not every row sees all of the unit
     uint32_t magic;
     const uint8_t *kp, *vp;  // the head's planes
@@ -381,10 +379,10 @@ struct QuantWarp {
         if (s.c == 0) undos[s.g] = undo;
     }
 
-    __device__ __forceinline__ void SetPower(int n, int to) {
-        e[n] = to;
-        bound[n] = Pow2(to);
-        down[n] = __float2half2_rn(Pow2(-to));
+    __device__ __forceinline__ void SetPower(int to) {
+        e = to;
+        bound = Pow2(to);
+        down = __float2half2_rn(Pow2(-to));
     }
 
     __device__ __forceinline__ void Begin(const TreeArgs& a, const TreeSplit& sp, int seq, int head) {
@@ -394,11 +392,8 @@ struct QuantWarp {
         vp = static_cast<const uint8_t*>(a.c.v) + row * NB * kQuantBytes;
         ksp = a.c.ks + row * NB;
         vsp = a.c.vs + row * NB;
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-            v[n].Clear();
-            SetPower(n, -15);
-        }
+        v[0].Clear();
+        SetPower(-15);
     }
 
     // K (or V) of the unit at p0 into a ring stage, by the COUNT threads of a group.
@@ -429,11 +424,9 @@ struct QuantWarp {
     // another unit's.
     __device__ __forceinline__ void Keys(const Step& s, const uint8_t* stage, const uint4* frags, int p0, int low) {
         edge = low + kUnit > s.len;
-        float x[NT][H][4];
+        float x[H][4];
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-            for (int h = 0; h < H; ++h) x[n][h][0] = x[n][h][1] = x[n][h][2] = x[n][h][3] = 0.0f;
+        for (int h = 0; h < H; ++h) x[h][0] = x[h][1] = x[h][2] = x[h][3] = 0.0f;
         {
             const __half* sc = reinterpret_cast<const __half*>(stage + kPlane) + s.g * NB;
             uint32_t kd[2 * H][(NB + 1) / 2];
@@ -443,12 +436,8 @@ struct QuantWarp {
             const uint32_t row = SmemAddr(stage) + s.g * kPitch + 4 * s.c + (kXor ? s.g * 16 : 0);
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
-                uint4 q0[NT], q1[NT];
-#pragma unroll
-                for (int n = 0; n < NT; ++n) {
-                    q0[n] = frags[(n * kFrags + 2 * b) * 32];
-                    q1[n] = frags[(n * kFrags + 2 * b + 1) * 32];
-                }
+                const uint4 q0 = frags[2 * b * 32];
+                const uint4 q1 = frags[(2 * b + 1) * 32];
 #pragma unroll
                 for (int h = 0; h < H; ++h) {
                     uint32_t f[2][4];
@@ -472,34 +461,28 @@ struct QuantWarp {
                         }
                     }
                     const float d0 = ScaleOf(kd[2 * h], b), d1 = ScaleOf(kd[2 * h + 1], b);
-#pragma unroll
-                    for (int n = 0; n < NT; ++n) {
-                        float d[4];
-                        MmaFirst(d, f[0], q0[n].z, q0[n].w);
-                        Mma(d, f[1], q1[n].z, q1[n].w);
-                        Mma(d, f[0], q0[n].x, q0[n].y);
-                        Mma(d, f[1], q1[n].x, q1[n].y);
-                        float(&to)[4] = x[n][h];
-                        to[0] = fmaf(d0, d[0], to[0]);
-                        to[1] = fmaf(d0, d[1], to[1]);
-                        to[2] = fmaf(d1, d[2], to[2]);
-                        to[3] = fmaf(d1, d[3], to[3]);
-                    }
+                    float d[4];
+                    MmaFirst(d, f[0], q0.z, q0.w);
+                    Mma(d, f[1], q1.z, q1.w);
+                    Mma(d, f[0], q0.x, q0.y);
+                    Mma(d, f[1], q1.x, q1.y);
+                    float(&to)[4] = x[h];
+                    to[0] = fmaf(d0, d[0], to[0]);
+                    to[1] = fmaf(d0, d[1], to[1]);
+                    to[2] = fmaf(d1, d[2], to[2]);
+                    to[3] = fmaf(d1, d[3], to[3]);
                 }
             }
         }
+        col[0].Weights(s, p0, low, edge, x, kOffset, [&](float r0, float r1) { v[0].Scale(r0, r1); });
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-            col[n].Weights(s, p0, low, edge, x[n], kOffset, [&](float r0, float r1) { v[n].Scale(r0, r1); });
+        for (int h = 0; h < H; ++h)
 #pragma unroll
-            for (int h = 0; h < H; ++h)
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    SplitHalf(x[n][h][2 * i], x[n][h][2 * i + 1], ph[n][h][i], pl[n][h][i]);
-                    ph[n][h][i] = Transpose8x8(ph[n][h][i]);
-                    pl[n][h][i] = Transpose8x8(pl[n][h][i]);
-                }
-        }
+            for (int i = 0; i < 2; ++i) {
+                SplitHalf(x[h][2 * i], x[h][2 * i + 1], ph[h][i], pl[h][i]);
+                ph[h][i] = Transpose8x8(ph[h][i]);
+                pl[h][i] = Transpose8x8(pl[h][i]);
+            }
     }
 
     // The weighted values of the unit, its V staged.
@@ -519,41 +502,35 @@ struct QuantWarp {
                         d[h][i][b] = __byte_perm(va[b >> 1], vb[b >> 1], b & 1 ? 0x7632 : 0x5410);
                 }
         }
-        uint32_t all = 0;  // the largest pair where every slot is seen
+        __half2 big = AsHalf2(0u);
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-            __half2 big = AsHalf2(0u);
+        for (int h = 0; h < H; ++h)
 #pragma unroll
-            for (int h = 0; h < H; ++h)
+            for (int i = 0; i < 2; ++i) {
+                if (edge) {  // a slot that is not seen may hold any scale, NaN too
+                    const uint32_t see = __hne2_mask(AsHalf2(ph[h][i]), AsHalf2(0u));
 #pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    if (edge) {  // a slot that is not seen may hold any scale, NaN too
-                        const uint32_t see = __hne2_mask(AsHalf2(ph[n][h][i]), AsHalf2(0u));
+                    for (int b = 0; b < NB; ++b) big = __hmax2(big, __habs2(AsHalf2(d[h][i][b] & see)));
+                } else {
 #pragma unroll
-                        for (int b = 0; b < NB; ++b) big = __hmax2(big, __habs2(AsHalf2(d[h][i][b] & see)));
-                    } else if (n == 0) {
-#pragma unroll
-                        for (int b = 0; b < NB; ++b) big = __hmax2(big, __habs2(AsHalf2(d[h][i][b])));
-                    }
+                    for (int b = 0; b < NB; ++b) big = __hmax2(big, __habs2(AsHalf2(d[h][i][b])));
                 }
-            if (n > 0 && !edge) big = AsHalf2(all);
-            if (n == 0) all = H2(big);
-            const float top = fmaxf(__low2float(big), __high2float(big));
-            if (__any_sync(0xffffffffu, top > bound[n])) {
-                float t = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-                t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 2));
-                // 2^to > t, `to` within the powers that a half can scale by
-                const int to = max(e[n], min(15, max(-15, static_cast<int>(__float_as_uint(t) >> 23) - 126)));
-                const float f = Pow2(e[n] - to);
-                SetPower(n, to);
-                v[n].Scale(__shfl_sync(0xffffffffu, f, 8 * s.c), __shfl_sync(0xffffffffu, f, 8 * s.c + 4));
             }
+        const float top = fmaxf(__low2float(big), __high2float(big));
+        if (__any_sync(0xffffffffu, top > bound)) {
+            float t = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 2));
+            // 2^to > t, `to` within the powers that a half can scale by
+            const int to = max(e, min(15, max(-15, static_cast<int>(__float_as_uint(t) >> 23) - 126)));
+            const float f = Pow2(e - to);
+            SetPower(to);
+            v[0].Scale(__shfl_sync(0xffffffffu, f, 8 * s.c), __shfl_sync(0xffffffffu, f, 8 * s.c + 4));
         }
         const uint32_t row = SmemAddr(stage) + 2 * s.c * kPitch +
                              (kXor ? ((s.g >> 2) ^ (2 * s.c)) * 16 + 4 * (s.g & 3) : (kQuantBytes / 8) * s.g);
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
-            float t[NT][2][4];
+            float t[2][4];
 #pragma unroll
             for (int h = 0; h < H; ++h) {
                 uint32_t f[2][4];
@@ -579,38 +556,30 @@ struct QuantWarp {
                         f[1][2 * r + 1] = HighNibbles(u, magic);
                     }
                 }
+                uint32_t hi[2], lo[2];
 #pragma unroll
-                for (int n = 0; n < NT; ++n) {
-                    uint32_t hi[2], lo[2];
+                for (int i = 0; i < 2; ++i) {
+                    uint32_t di = d[h][i][b];
+                    if (edge) di &= __hne2_mask(AsHalf2(ph[h][i]), AsHalf2(0u));
+                    const __half2 sc = __hmul2(AsHalf2(di), down);
+                    const __half2 p = AsHalf2(ph[h][i]), y = __hmul2(p, sc);
+                    hi[i] = H2(y);
+                    lo[i] = H2(__hfma2(AsHalf2(pl[h][i]), sc, __hfma2(p, sc, __hneg2(y))));
+                }
 #pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        uint32_t di = d[h][i][b];
-                        if (edge) di &= __hne2_mask(AsHalf2(ph[n][h][i]), AsHalf2(0u));
-                        const __half2 sc = __hmul2(AsHalf2(di), down[n]);
-                        const __half2 p = AsHalf2(ph[n][h][i]), y = __hmul2(p, sc);
-                        hi[i] = H2(y);
-                        lo[i] = H2(__hfma2(AsHalf2(pl[n][h][i]), sc, __hfma2(p, sc, __hneg2(y))));
-                    }
-#pragma unroll
-                    for (int j = 0; j < 2; ++j) {
-                        h == 0 ? MmaFirst(t[n][j], f[j], lo[0], lo[1]) : Mma(t[n][j], f[j], lo[0], lo[1]);
-                        Mma(t[n][j], f[j], hi[0], hi[1]);
-                    }
+                for (int j = 0; j < 2; ++j) {
+                    h == 0 ? MmaFirst(t[j], f[j], lo[0], lo[1]) : Mma(t[j], f[j], lo[0], lo[1]);
+                    Mma(t[j], f[j], hi[0], hi[1]);
                 }
             }
 #pragma unroll
-            for (int n = 0; n < NT; ++n)
-#pragma unroll
-                for (int j = 0; j < 2; ++j) AddTo(v[n].o[b][j], t[n][j]);
+            for (int j = 0; j < 2; ++j) AddTo(v[0].o[b][j], t[j]);
         }
     }
 
     __device__ __forceinline__ void End(const Step& s) {
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-            const float f = Pow2(e[n]);
-            v[n].Scale(__shfl_sync(0xffffffffu, f, 8 * s.c), __shfl_sync(0xffffffffu, f, 8 * s.c + 4));
-        }
+        const float f = Pow2(e);
+        v[0].Scale(__shfl_sync(0xffffffffu, f, 8 * s.c), __shfl_sync(0xffffffffu, f, 8 * s.c + 4));
     }
 };
 
@@ -801,11 +770,10 @@ struct F32Warp {
     __device__ __forceinline__ void End(const Step&) {}
 };
 
-// One tile per warp leaves registers for two steps to a unit: half the sums of
-// the fresh accumulators, half the loads of Q.
 template <int TYPE, int NB, int NT>
 struct WarpOf {
-    using T = QuantWarp<TYPE, NB, NT, NT == 1 ? 2 : 1>;
+    static_assert(NT == 1, "quantized caches: a tile per warp");
+    using T = QuantWarp<TYPE, NB>;
 };
 template <int NB, int NT>
 struct WarpOf<MLB_F32, NB, NT> {
@@ -1199,10 +1167,18 @@ bool LaunchShape(DeviceContext& ctx, const TreeArgs& a) {
     return true;
 }
 
-// Rows per KV head choose the tiles: up to 8 one tile per warp; more take two
-// per warp (the quants are converted once for both), up to four warps sharing
-// their slots.  fp32 heads above 64 elements: one tile per warp, the registers
-// and the ring hold no more.
+// Rows per KV head choose the tiles.  Up to 8: a tile, every warp its own slots;
+// more: two warps share slots, a tile each, a group of 16 rows after the other
+// (the second reads the cache from L2).  Measured at 8 sequences of 4000 slots,
+// 8 x 128 in Q8_0: 16 rows 40.8 us (43.0 with two tiles to a warp, 40.9 with a
+// group of 8 after the other; 17.2, 21.9 and 18.5 with heads 2 x 64), 32 rows 62.9
+// (57.4 with four warps a group, three CTAs per SM, but 32.0 instead of 28.7 where
+// one sequence of 8000 slots leaves few units).
+// fp32 caches are bound by the tf32 products: above 32 rows two tiles to a warp
+// halve the fragments' splits (49 rows, 2 x 64, 8 sequences of up to 16384 slots:
+// 67 us, one tile 78; 32 rows at 8000 slots: 31.0 against 24.6).  Heads of more than 64
+// elements leave no room for that: four warps a group above 16 rows (32 rows, 8 x
+// 4000 slots: 116 us, two warps 133), two above 8 (16 rows: 72 us, one 103).
 template <int TYPE, int NB>
 bool LaunchRows(DeviceContext& ctx, const TreeArgs& a) {
     const long long rows = 1LL * a.tokens * a.group;
@@ -1212,9 +1188,9 @@ bool LaunchRows(DeviceContext& ctx, const TreeArgs& a) {
         return LaunchShape<TYPE, NB, 1, 4, 4, 2>(ctx, a);
     } else {
         if (rows <= kRows) return LaunchShape<TYPE, NB, 1, 1, 6, 2>(ctx, a);
-        if (rows <= 2 * kRows) return LaunchShape<TYPE, NB, 2, 1, 6, 2>(ctx, a);
-        if (rows <= 4 * kRows) return LaunchShape<TYPE, NB, 2, 2, 6, 2>(ctx, a);
-        return LaunchShape<TYPE, NB, 2, 4, TREE_NW4, TREE_PER4>(ctx, a);
+        if constexpr (TYPE == MLB_F32)
+            if (rows > 4 * kRows) return LaunchShape<TYPE, NB, 2, 2, 6, 2>(ctx, a);
+        return LaunchShape<TYPE, NB, 1, 2, 6, 2>(ctx, a);
     }
 }
 
