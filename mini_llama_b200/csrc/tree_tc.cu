@@ -16,10 +16,12 @@
 //                 lies in the cache (the N side contiguous); a fresh accumulator per
 //                 tile, added to the running rows in registers in fp32 (the matrix
 //                 unit's own sums truncate)
-// A tile with a scale of 2^8 or more (|value| could pass fp16's range) is taken
-// times 2^-9, undone in fp32.  Slots that only some rows see may hold any bytes:
-// K touches its own column only; a V scale that is not finite in a drafted slot
-// becomes 0 and the rows that see it NaN in that block.
+// Where |d q| could pass fp16's range (a scale of 2^8 or more) quants are taken times
+// 2^-9, undone in fp32: a K slot by itself, so that no slot's scores depend on
+// another's; V a whole tile at a time, resolved to 2^-31 of its largest value.
+// Slots that only some rows see may hold any bytes: K touches its own column only; a V
+// scale that is not finite in a drafted slot becomes 0 and the rows that see it
+// NaN in that block; one of 2^8 or more that no row sees becomes 0.
 //
 // Bound: the MMAs, 6 x 128 x 128 x head_dim multiply-adds a tile (64 cycles for
 // 128 x 128 x 16), and the shared memory that they, the images' stores and the
@@ -72,6 +74,7 @@ struct TcTreeShared {
     float last[2][kTile];    // sums of the weights
     uint32_t flag[2][kProdWarps];
     int k_big[kInfoBufs], v_big[kInfoBufs], v_odd[kInfoBufs];
+    uint32_t k_bits[kInfoBufs][kTile / 32];      // slots of K taken times 2^-9, where k_big
     uint32_t v_bad[kInfoBufs][4][kTile / 32];  // [tile][block][slots]: scales that are not finite, drafted slots
 };
 constexpr int kTcHeaderBytes = 7168;
@@ -153,6 +156,11 @@ __device__ __forceinline__ void Load16(uint32_t at, float* v) {
         : "r"(at));
 #pragma unroll
     for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
+}
+__device__ __forceinline__ void Load8(uint32_t at, uint32_t (&r)[8]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+                 : "r"(at));
 }
 __device__ __forceinline__ void Store8(uint32_t at, const uint32_t (&r)[8]) {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(at), "r"(r[0]),
@@ -269,14 +277,30 @@ struct Share {
             }
         return odd;
     }
+    // Takes out the large scales of drafted slots that no token's mask shows.
+    __device__ __forceinline__ void TakeUnseen(const uint64_t* mask, int words, int tokens, int from, int id) {
+#pragma unroll
+        for (int j = 0; j < kTasks; ++j) {
+            const int draft = Row(j, id) - from;
+            if ((d[j] & 0x7fffu) < 0x5C00u || draft < 0) continue;
+            bool seen = false;
+#pragma unroll 1
+            for (int t = 0; t < tokens && !seen; ++t)
+                seen = (__ldg(mask + size_t(t) * words + (draft >> 6)) >> (draft & 63)) & 1;
+            if (!seen) d[j] = 0;
+        }
+    }
     // Into the images: within each group of four elements in the order 0, 2, 1, 3.
-    __device__ __forceinline__ void Convert(uint8_t* image, int id, bool big, uint32_t magic) const {
+    // BIG: the rows whose bit is set in `down` (null: all) times 2^-9; the quants, as the scale could lose bits.
+    template <bool BIG>
+    __device__ __forceinline__ void Convert(uint8_t* image, int id, uint32_t magic, const uint32_t* down) const {
         constexpr int kLo = NB * 4 * kChunkPitch;  // of the lo image
 #pragma unroll
         for (int j = 0; j < kTasks; ++j) {
             if (!Has(j, id)) continue;
-            __half2 s = __half2half2(__ushort_as_half(d[j]));
-            if (big) s = __hmul2(s, AsHalf2(0x18001800u));  // 2^-9
+            const __half2 s = __half2half2(__ushort_as_half(d[j]));
+            const int at = Row(j, id);
+            const __half2 factor = AsHalf2(BIG && (!down || ((down[at >> 5] >> (at & 31)) & 1)) ? 0x18001800u : 0x3C003C00u);
             uint8_t* to = image + Piece(j, id) * ((TYPE == MLB_Q8_0 ? 2 : 4) * kChunkPitch) + Row(j, id) * 16;
             const uint32_t w[4] = {q[j].x, q[j].y, q[j].z, q[j].w};
 #pragma unroll
@@ -294,6 +318,9 @@ struct Share {
                     p[2] = c < 2 ? LowNibbles(w1, magic) : HighNibbles(w1, magic);
                     p[3] = c < 2 ? LowNibbles(w1 >> 8, magic) : HighNibbles(w1 >> 8, magic);
                 }
+                if constexpr (BIG)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) p[i] = H2(__hmul2(AsHalf2(p[i]), factor));
                 uint4 hi, lo;
                 Product(p[0], s, hi.x, lo.x);
                 Product(p[1], s, hi.y, lo.y);
@@ -432,6 +459,20 @@ __global__ void __launch_bounds__(kTcWarps * 32, 1) TreeTcKernel(TreeArgs a, Tre
                     if (!(ok = Wait(sh, &sh.s_full[it & 1], (it >> 1) & 1, status))) break;
                     FenceAfter();
                     const bool edge = (u + 1) * kTile > walk.e.len;
+                    if (sh.k_big[it % kInfoBufs]) {
+#pragma unroll 1
+                        for (int i = 0; i < 64; i += 8) {
+                            const uint32_t down = sh.k_bits[it % kInfoBufs][(half * 64 + i) >> 5] >> (i & 31);
+                            uint32_t x[8];
+                            Load8(scores + i, x);
+                            WaitLoad();
+#pragma unroll
+                            for (int j = 0; j < 8; ++j)
+                                if ((down >> j) & 1) x[j] = __float_as_uint(__uint_as_float(x[j]) * 512.0f);
+                            Store8(scores + i, x);
+                        }
+                        WaitStore();
+                    }
                     // 16 scores, those that the row does not see taken out
                     auto get = [&](float (&x)[16], int i) {
                         Load16(scores + i, x);
@@ -455,8 +496,7 @@ __global__ void __launch_bounds__(kTcWarps * 32, 1) TreeTcKernel(TreeArgs a, Tre
                     float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
                     sh.top[it & 1][half][row] = top;
                     if (!(ok = Meet(sh, &sh.soft, met, status))) break;
-                    const float c = sh.k_big[it % kInfoBufs] ? cs * 512.0f : cs;
-                    top = fmaxf(top, sh.top[it & 1][half ^ 1][row]) * c;
+                    top = fmaxf(top, sh.top[it & 1][half ^ 1][row]) * cs;
                     m_last = m;
                     if (top > m + kLag) {
                         const float f = Exp2(m - top);
@@ -472,7 +512,7 @@ __global__ void __launch_bounds__(kTcWarps * 32, 1) TreeTcKernel(TreeArgs a, Tre
                         uint32_t hi[8], lo[8];
 #pragma unroll
                         for (int j = 0; j < 8; ++j) {
-                            const float p0 = Exp2(fmaf(x[2 * j], c, off)), p1 = Exp2(fmaf(x[2 * j + 1], c, off));
+                            const float p0 = Exp2(fmaf(x[2 * j], cs, off)), p1 = Exp2(fmaf(x[2 * j + 1], cs, off));
                             l0 += p0;
                             l1 += p1;
                             SplitHalf(p0, p1, hi[j], lo[j]);
@@ -580,6 +620,8 @@ __global__ void __launch_bounds__(kTcWarps * 32, 1) TreeTcKernel(TreeArgs a, Tre
                 const int u = tile(i);
                 // a drafted slot's V scale that is not finite is taken out and noted
                 const bool odd = v && r.TakeOdd(walk.e.len - u * kTile, id);
+                if (v && a.mask && r.Big())
+                    r.TakeUnseen(a.mask + size_t(walk.b) * a.tokens * a.words, a.words, a.tokens, walk.e.len - u * kTile, id);
                 const uint32_t flags = together((r.Big() ? 1u : 0u) | (odd ? 2u : 0u));
                 if (!ok) break;
                 const bool big = flags & 1, any = flags & 2;
@@ -603,7 +645,24 @@ __global__ void __launch_bounds__(kTcWarps * 32, 1) TreeTcKernel(TreeArgs a, Tre
                     (v ? sh.v_big : sh.k_big)[n % kInfoBufs] = big;
                     if (v) sh.v_odd[n % kInfoBufs] = any;
                 }
-                r.Convert(v ? vi : ki + (n & 1) * 2 * kImage, id, big, sp.magic);
+                uint8_t* image = v ? vi : ki + (n & 1) * 2 * kImage;
+                if (!big) {
+                    r.template Convert<false>(image, id, sp.magic, nullptr);
+                } else {
+                    uint32_t* down = sh.k_bits[n % kInfoBufs];
+                    if (!v) {  // the slots that need it
+                        if (id < kTile) {
+                            const size_t at = min(u * kTile + id, a.c.head_slots - 1);
+                            bool large = false;
+                            for (int b = 0; b < NB; ++b)
+                                large = large || (__ldg(reinterpret_cast<const unsigned short*>(ks + at * NB + b)) & 0x7fffu) >= 0x5C00u;
+                            const uint32_t bits = __ballot_sync(0xffffffffu, large);
+                            if (lane == 0) down[id / 32] = bits;
+                        }
+                        if (!(ok = Meet(sh, &sh.prod, met, status))) break;
+                    }
+                    r.template Convert<true>(image, id, sp.magic, v ? nullptr : down);
+                }
                 FenceAsync();
                 Arrive(v ? &sh.v_full : &sh.k_full[n & 1]);
                 if (i + 1 < all) {

@@ -553,6 +553,69 @@ def test_many_items_to_a_cta(mlb, gpu, qtype, heads, kv, hd, tokens, length, n_s
     assert_attention(got[some], *want)
 
 
+@pytest.mark.parametrize("qtype", [F32, Q80, Q40], ids=NAME.get)
+@pytest.mark.parametrize("max_seq", [1, 5, 16, 31, 100, 129])
+@pytest.mark.parametrize("heads,kv,tokens", [(2, 2, 1), (4, 1, 5), (24, 2, 7)])
+def test_short_caches(mlb, gpu, qtype, max_seq, heads, kv, tokens):
+    """Planes shorter than a unit or a tile of the matrix kernels, filled to their end; few rows and many."""
+    rng = np.random.default_rng(max_seq)
+    c, k, v = filled(mlb, gpu, rng, qtype, 3, max_seq, kv, 64)
+    q = rng.standard_normal((3, tokens, heads, 64)).astype(np.float32)
+    mask = np.stack([random_tree(rng, tokens) for _ in range(3)])
+    lens = [max(0, max_seq - tokens), max_seq, 0]
+    got = run_attention(mlb, gpu, c, 0, q, None, lens, max_seq, mask)
+    assert_attention(got, *ref.attention(q, k, v, lens, range(3), mask, 0.125, max_seq))
+
+
+@pytest.mark.parametrize("qtype", [F32, Q80, Q40], ids=NAME.get)
+@pytest.mark.parametrize("hd", [32, 96, 128])
+@pytest.mark.parametrize("byte", [0xFF, 0x7C, 0x77])  # fp16 scales: NaN, NaN, 30576
+def test_many_rows_past_unseen_slots(mlb, gpu, qtype, hd, byte):
+    """More than 32 rows per KV head: a drafted slot that only its own token sees holds NaN or huge values; a row that
+    sees nothing, an empty entry and an inactive one are zero, the others unchanged."""
+    rng = np.random.default_rng(hd + byte)
+    tokens, heads, kv, n, max_seq = 9, 10, 2, 150, 192
+    c = Cache(mlb, gpu, qtype, 4, 1, max_seq, kv, hd, fill=byte)
+    k, v = (rng.standard_normal((2, n + tokens, kv, hd)).astype(np.float32) for _ in range(2))
+    odd = n + 3
+    for s in range(2):
+        keep = [i for i in range(n + tokens) if s == 1 or i != odd]
+        c.write(0, [s] * len(keep), keep, k[s, keep], v[s, keep])
+    mask = np.zeros((4, tokens, 1), np.uint64)
+    for t in range(tokens):
+        mask[:, t, 0] = sum(1 << j for j in range(t + 1) if j != 3 or t == 3)
+    mask[1, 6] = 0  # sees what is committed: nothing
+    lens, seqs = [n, 0, 50, -1], [0, 1, 7, 0]
+    q = rng.standard_normal((4, tokens, heads, hd)).astype(np.float32)
+    got = run_attention(mlb, gpu, c, 0, q, seqs, lens, n, mask)
+    assert (got[1, 6] == 0).all() and (got[2] == 0).all() and (got[3] == 0).all()
+    kk, vv = (np.zeros((2, max_seq, kv, hd), np.float32) for _ in range(2))
+    kk[:, :n + tokens], vv[:, :n + tokens] = ref.held(k, qtype), ref.held(v, qtype)
+    kk[0, odd] = vv[0, odd] = 0
+    want = ref.attention(q[:2], kk, vv, lens[:2], seqs[:2], mask[:2], hd ** -0.5, max_seq)
+    others = [t for t in range(tokens) if t != 3]
+    assert_attention(got[:1, others], *[x[:1, others] for x in want])
+    assert_attention(got[1:2], *[x[1:2] for x in want])
+
+
+@pytest.mark.parametrize("qtype", [F32, Q80, Q40], ids=NAME.get)
+@pytest.mark.parametrize("k_mag,v_mag,q_mag", [(1e-4, 1e-4, 1e4), (30.0, 2e4, 0.05), (5e4, 1.0, 1e-5), (1.0, 1e-3, 1.0)])
+def test_magnitudes_of_many_rows(mlb, gpu, qtype, k_mag, v_mag, q_mag):
+    """As test_magnitudes, more than 32 rows per KV head; some tiles of 128 slots hold large scales, some do not."""
+    rng = np.random.default_rng(13)
+    tokens, heads, kv, hd, n = 7, 12, 2, 128, 700
+    c = Cache(mlb, gpu, qtype, 1, 1, 768, kv, hd)
+    size = np.where(np.arange(n + tokens) // 200 % 2, 1.0, 1e-3)[:, None, None]
+    k = (k_mag * size * rng.standard_normal((n + tokens, kv, hd))).astype(np.float32)
+    v = (v_mag * size * rng.standard_normal((n + tokens, kv, hd))).astype(np.float32)
+    c.write(0, None, list(range(n + tokens)), k, v)
+    q = (q_mag * rng.standard_normal((1, tokens, heads, hd))).astype(np.float32)
+    kk, vv = (np.zeros((1, 768, kv, hd), np.float32) for _ in range(2))
+    kk[0, :n + tokens], vv[0, :n + tokens] = ref.held(k, qtype), ref.held(v, qtype)
+    got = run_attention(mlb, gpu, c, 0, q, None, [n], n, None)
+    assert_attention(got, *ref.attention(q, kk, vv, [n], [0], None, hd ** -0.5, 768))
+
+
 def test_empty_calls(mlb, gpu):
     c = Cache(mlb, gpu, Q80, 1, 1, 8, 1, 32)
     mlb.call("mlb_kv_cache_write", gpu, c.ref, 0, 0, None, None, None, 32, None, 32)
