@@ -825,8 +825,10 @@ struct Joined {
 struct Cut {
     unsigned total, ctas, each, extra;
 
-    // `groups`: units that a CTA works on at a time.
-    __device__ __forceinline__ Cut(const TreeArgs& a, unsigned unit, unsigned items, unsigned groups, unsigned grid) {
+    // `groups`: units that a CTA works on at a time; `small`: an item that a CTA keeps to itself, as joining its parts
+    // would take longer (131 slots of 2 x 64 in Q8_0: 7.8 us whole, 10.2 cut).
+    __device__ __forceinline__ Cut(const TreeArgs& a, unsigned unit, unsigned items, unsigned groups, unsigned small,
+                                   unsigned grid) {
         const int lane = threadIdx.x & 31;
         unsigned live = 0;
         total = 0;
@@ -836,7 +838,8 @@ struct Cut {
             live += __popc(__ballot_sync(0xffffffffu, n != 0));
         }
         // a unit for each group, or an item for each CTA, at least
-        ctas = max(1u, min(max((total + groups - 1) / groups, min(live * items, total)), grid));
+        const unsigned whole = min(live * items, total);
+        ctas = max(1u, min(total <= small * whole ? whole : max((total + groups - 1) / groups, whole), grid));
         each = total / ctas;
         extra = total - each * ctas;
     }
@@ -920,7 +923,7 @@ __global__ void __launch_bounds__(NW * 32, PER_SM) TreeMmaKernel(TreeArgs a, Tre
     }
 
     GridDepLaunch();  // the joining kernel may come up as CTAs leave
-    const Cut cut(a, kUnit, items, kGroups, gridDim.x);
+    const Cut cut(a, kUnit, items, kGroups, 2 * kGroups, gridDim.x);
     if (cut.total == 0 || blockIdx.x >= cut.ctas) return;
     unsigned cur = cut.Start(blockIdx.x);
     const unsigned end = cut.Start(blockIdx.x + 1);
@@ -1078,19 +1081,21 @@ __global__ void __launch_bounds__(NW * 32, PER_SM) TreeMmaKernel(TreeArgs a, Tre
     }
 }
 
-// Items that are cut between CTAs: a warp per row adds up their parts, in the
-// order of the CTAs.  blockIdx.x: item, blockIdx.y: rows y, y + gridDim.y, ..
+// Items that are cut between CTAs: `share` warps to a row add up its parts, in
+// the order of the CTAs, and one of them joins their sums.  blockIdx.x: item,
+// blockIdx.y: rows, kJoinWarps / share of them at a time.
 constexpr int kJoinWarps = 8;
-constexpr int kJoinBatch = 8;  // parts in flight
+constexpr int kJoinBatch = 4;  // parts in flight
 
-template <int NB>
-__global__ void __launch_bounds__(kJoinWarps * 32) TreeJoinKernel(TreeArgs a, TreeSplit sp, int unit, int groups,
-                                                                  int item_rows, int grid) {
+template <int NB, bool SHARED>
+__global__ void __launch_bounds__(kJoinWarps * 32) TreeJoinKernel(TreeArgs a, TreeSplit sp, int unit, int groups, int small,
+                                                                  int item_rows, int grid, int shared) {
+    const int share = SHARED ? shared : 1;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const unsigned items = a.c.n_kv * sp.groups;
     const int b = blockIdx.x / items;
     const unsigned item = blockIdx.x - b * items;
-    const Cut cut(a, unit, items, groups, grid);
+    const Cut cut(a, unit, items, groups, small, grid);
     const unsigned units = EntryUnits(a, b, unit, 1);
     if (units == 0) return;
     unsigned first = 0;  // of the entry
@@ -1101,40 +1106,59 @@ __global__ void __launch_bounds__(kJoinWarps * 32) TreeJoinKernel(TreeArgs a, Tr
     if (c0 == c1) return;
     GridDepWait();
     const int head = item / sp.groups, row0 = (item - head * sp.groups) * item_rows;
-    const int rows = min(item_rows, sp.rows - row0);
+    const int rows = min(item_rows, sp.rows - row0), at_once = kJoinWarps / share;
     const size_t part = size_t(item_rows) * (NB * 32 + 2);
-    for (int r = blockIdx.y * kJoinWarps + warp; r < rows; r += gridDim.y * kJoinWarps) {
-        const int d = min(lane, NB * 8 - 1) * 4;
+    const unsigned each = (c1 - c0 + share) / share;  // parts of a warp
+    const unsigned begin = c0 + warp % share * each, end = min(begin + each, c1 + 1);
+    for (int base = blockIdx.y * at_once; base < rows; base += gridDim.y * at_once) {
+        const int r = base + warp / share, d = min(lane, NB * 8 - 1) * 4;
         Joined x;
-        for (unsigned k = c0; k <= c1; k += kJoinBatch) {
-            float pm[kJoinBatch], pl[kJoinBatch];
-            float4 po[kJoinBatch];
+        if (r < rows)
+            for (unsigned k = begin; k < end; k += kJoinBatch) {
+                float pm[kJoinBatch], pl[kJoinBatch];
+                float4 po[kJoinBatch];
 #pragma unroll
-            for (int j = 0; j < kJoinBatch; ++j) {
-                // a CTA has two parts: of the item that it goes on with, and of one that it begins
-                const unsigned cta = min(k + j, c1);
-                const float* p = sp.parts + (2 * size_t(cta) + (cut.Start(cta) <= u0 ? 1 : 0)) * part;
-                pm[j] = __ldcg(p + item_rows * NB * 32 + r);
-                pl[j] = __ldcg(p + item_rows * (NB * 32 + 1) + r);
-                po[j] = __ldcg(reinterpret_cast<const float4*>(p + r * NB * 32 + d));
+                for (int j = 0; j < kJoinBatch; ++j) {
+                    // a CTA has two parts: of the item that it goes on with, and of one that it begins
+                    const unsigned cta = min(k + j, end - 1);
+                    const float* p = sp.parts + (2 * size_t(cta) + (cut.Start(cta) <= u0 ? 1 : 0)) * part;
+                    pm[j] = __ldcg(p + item_rows * NB * 32 + r);
+                    pl[j] = __ldcg(p + item_rows * (NB * 32 + 1) + r);
+                    po[j] = __ldcg(reinterpret_cast<const float4*>(p + r * NB * 32 + d));
+                }
+#pragma unroll
+                for (int j = 0; j < kJoinBatch; ++j)
+                    if (k + j < end) x.Add(pm[j], pl[j], po[j]);
             }
-#pragma unroll
-            for (int j = 0; j < kJoinBatch; ++j)
-                if (k + j <= c1) x.Add(pm[j], pl[j], po[j]);
+        if constexpr (SHARED) {
+            __shared__ float sm[kJoinWarps], sl[kJoinWarps];
+            __shared__ float4 so[kJoinWarps][32];
+            if (lane == 0) {
+                sm[warp] = x.m;
+                sl[warp] = x.l;
+            }
+            so[warp][lane] = x.o;
+            __syncthreads();
+            if (warp % share == 0)
+                for (int j = 1; j < share; ++j) x.Add(sm[warp + j], sl[warp + j], so[warp + j][lane]);
+            __syncthreads();
         }
-        if (lane < NB * 8) StoreOut(a, OutRow(a, b, head, row0 + r), d, x.Result());
+        if (r < rows && warp % share == 0 && lane < NB * 8) StoreOut(a, OutRow(a, b, head, row0 + r), d, x.Result());
     }
 }
 
-// Comes up while the main kernel's last CTAs run.
+// Comes up while the main kernel's last CTAs run.  Warps share a row where an item
+// is cut into more parts than one has in flight.
 template <int NB>
-void LaunchJoin(DeviceContext& ctx, const TreeArgs& a, const TreeSplit& sp, int unit, int groups, int item_rows, int grid) {
+void LaunchJoin(DeviceContext& ctx, const TreeArgs& a, const TreeSplit& sp, int unit, int groups, int small, int item_rows,
+                int grid) {
     const int all = a.batch * a.c.n_kv * sp.groups;
-    // a row for each warp, as long as that is not many more CTAs than the device holds
+    int share = 1;
+    while (share < kJoinWarps && share * kJoinBatch * all < grid) share *= 2;
+    // as many rows at once as do not make many more CTAs than the device holds
     const int rows = std::min(item_rows, sp.rows);
-    const int per_item = std::max(1, std::min<int>(CeilDiv(rows, kJoinWarps), 16 * ctx.sm_count / all));
-    Launch("TreeJoinKernel", TreeJoinKernel<NB>, dim3(all, per_item), dim3(kJoinWarps * 32), 0, ctx.stream, true, a, sp, unit,
-           groups, item_rows, grid);
+    const int per_item = std::max(1, std::min<int>(CeilDiv(rows * share, kJoinWarps), 16 * ctx.sm_count / all));
+    Launch("TreeJoinKernel", share > 1 ? TreeJoinKernel<NB, true> : TreeJoinKernel<NB, false>, dim3(all, per_item), dim3(kJoinWarps * 32), 0, ctx.stream, true, a, sp, unit, groups, small, item_rows, grid, share);
 }
 
 template <int TYPE, int NB, int NT, int WQ, int NW, int PER_SM>
@@ -1163,7 +1187,7 @@ bool LaunchShape(DeviceContext& ctx, const TreeArgs& a) {
     kernel<<<grid, NW * 32, Shape::kBytes, ctx.stream>>>(a, sp);
     CheckCuda(cudaGetLastError(), "TreeMmaKernel");
     if (grid == 1) return true;  // nothing is cut
-    LaunchJoin<NB>(ctx, a, sp, Shape::Warp::kUnit, Shape::kGroups, Shape::kItemRows, grid);
+    LaunchJoin<NB>(ctx, a, sp, Shape::Warp::kUnit, Shape::kGroups, 2 * Shape::kGroups, Shape::kItemRows, grid);
     return true;
 }
 
@@ -1187,10 +1211,10 @@ bool LaunchRows(DeviceContext& ctx, const TreeArgs& a) {
         if (rows <= 2 * kRows) return LaunchShape<TYPE, NB, 1, 2, 4, 2>(ctx, a);
         return LaunchShape<TYPE, NB, 1, 4, 4, 2>(ctx, a);
     } else {
-        if (rows <= kRows) return LaunchShape<TYPE, NB, 1, 1, 6, 2>(ctx, a);
+        if (rows <= kRows) return LaunchShape<TYPE, NB, 1, 1, 4, 3>(ctx, a);
         if constexpr (TYPE == MLB_F32)
-            if (rows > 4 * kRows) return LaunchShape<TYPE, NB, 2, 2, 6, 2>(ctx, a);
-        return LaunchShape<TYPE, NB, 1, 2, 6, 2>(ctx, a);
+            if (rows > 4 * kRows) return LaunchShape<TYPE, NB, 2, 2, 4, 3>(ctx, a);
+        return LaunchShape<TYPE, NB, 1, 2, 4, 3>(ctx, a);
     }
 }
 

@@ -353,7 +353,7 @@ __global__ void __launch_bounds__(kTcWarps * 32, 1) TreeTcKernel(TreeArgs a, Tre
                 a.out[(size_t(b) * a.tokens + t) * a.out_stride + i] = 0.0f;
     }
     GridDepLaunch();  // the joining kernel may come up as CTAs leave
-    const Cut cut(a, kTile, items, 1, gridDim.x);
+    const Cut cut(a, kTile, items, 1, 1, gridDim.x);
     if (cut.total == 0 || blockIdx.x >= cut.ctas) return;
     Walk walk;
     walk.cur = cut.Start(blockIdx.x);
@@ -763,7 +763,7 @@ bool LaunchTc(DeviceContext& ctx, const TreeArgs& a) {
     kernel<<<grid, kTcWarps * 32, kBytes, ctx.stream>>>(a, sp, ctx.status);
     CheckCuda(cudaGetLastError(), "TreeTcKernel");
     if (grid == 1) return true;  // nothing is cut
-    LaunchJoin<NB>(ctx, a, sp, kTile, 1, kTile, grid);
+    LaunchJoin<NB>(ctx, a, sp, kTile, 1, 1, kTile, grid);
     return true;
 }
 
