@@ -83,10 +83,10 @@ __global__ void __launch_bounds__(kRowWarps * 32) TreeRowKernel(TreeArgs a) {
 }
 
 // Head sizes up to 128 (fp32 caches: rows that allow 16-byte copies) and planes
-// of a unit or more.  Above 32 rows per KV head the tensor-memory kernel: a sequence of
-// 8000 slots, 8 x 128 in Q8_0, takes it 34.8 us at 32 rows and 34.9 at 40, the warp-level
-// one 28.7 and 38.6; 8 sequences of 4000 68 and 70 against 63 and 104; 2 x 64 24.6
-// and 24.6 against 21.2 and 28.7.
+// of a unit or more.  Above 32 rows per KV head the tensor-memory kernel: 8
+// sequences of 4000 slots, 8 x 128, take it 69.6 us at 32 rows and 69.8 at 40 in Q8_0,
+// the warp-level kernel 61.3 and 82.3 (Q4_0: 63.5 and 64.2 against 57.3 and 77.9); one
+// sequence of 8000 slots 32.2 and 32.8 against 26.6 and 30.7.
 bool LaunchTreeMma(DeviceContext& ctx, const TreeArgs& a) {
     if (a.c.type == MLB_F32) return a.cache_vec && LaunchTreeF32(ctx, a);
     if (1LL * a.tokens * a.group > 32 && LaunchTreeTc(ctx, a)) return true;

@@ -23,7 +23,14 @@
 // the matrix unit's own additions truncate, which over a long context would
 // cost several times the fp32 rounding.
 //
-// The units of 16 slots of all (sequence, KV head, row group) items are one
+// Bound: a decode step over long sequences (4 rows, 32 sequences, 304 MB in Q8_0)
+// runs at 4.2 TB/s, 64 % of the copy rate; the instructions of a unit (conversion,
+// fragments, softmax) take about as long as its bytes, and overlap them in part.
+// In 4 bits (151 MB, 32 K slots) the instructions alone bound it: 2.5 TB/s.  From 16
+// rows on it is instructions and matrix products, for fp32 the tf32 products (three
+// for one: 48 % of the tensor pipe's cycles).
+//
+// The units (32 slots, fp32 16) of all (sequence, KV head, row group) items are one
 // list, cut evenly over the CTAs (the lengths are on the device, so every CTA
 // works the cut out from them): sequences of any lengths balance.  A CTA's
 // stretch is dealt out to groups of WQ warps, one tile pair of the item's rows
@@ -1192,17 +1199,16 @@ bool LaunchShape(DeviceContext& ctx, const TreeArgs& a) {
 }
 
 // Rows per KV head choose the tiles.  Up to 8: a tile, every warp its own slots;
-// more: two warps share slots, a tile each, a group of 16 rows after the other
-// (the second reads the cache from L2).  Measured at 8 sequences of 4000 slots,
-// 8 x 128 in Q8_0: 16 rows 40.8 us (43.0 with two tiles to a warp, 40.9 with a
-// group of 8 after the other; 17.2, 21.9 and 18.5 with heads 2 x 64), 32 rows 62.9
-// (57.4 with four warps a group, three CTAs per SM, but 32.0 instead of 28.7 where
-// one sequence of 8000 slots leaves few units).
+// more: two warps share slots, a tile each, a group of 16 rows after the other (the
+// second reads the cache from L2).  8 sequences of 4000 slots, 8 x 128 in Q8_0: 16
+// rows 36.9 us (groups of 8: 39.2), 32 rows 61.3 (63.0); in Q4_0 34.8 (36.9), 57.3 (59.4).
+// Three CTAs of four warps begin and end their items independently: 32 sequences
+// of 500 to 8192 slots, four rows, take 73 us, with two CTAs of six warps 84.
 // fp32 caches are bound by the tf32 products: above 32 rows two tiles to a warp
-// halve the fragments' splits (49 rows, 2 x 64, 8 sequences of up to 16384 slots:
-// 67 us, one tile 78; 32 rows at 8000 slots: 31.0 against 24.6).  Heads of more than 64
-// elements leave no room for that: four warps a group above 16 rows (32 rows, 8 x
-// 4000 slots: 116 us, two warps 133), two above 8 (16 rows: 72 us, one 103).
+// halve the splits of K and V (49 rows, 2 x 64, 8 sequences of 2000 to 16384 slots:
+// 64.6 us, one tile 77.1; 32 rows of 8000 slots: 24.4 against 20.6).  Heads of more
+// than 64 elements leave no room for that: four warps a group above 16 rows (32 rows,
+// 8 x 4000 slots of 8 x 128: 116 us, two warps 133), two above 8 (16 rows: 72 us, one 103).
 template <int TYPE, int NB>
 bool LaunchRows(DeviceContext& ctx, const TreeArgs& a) {
     const long long rows = 1LL * a.tokens * a.group;
