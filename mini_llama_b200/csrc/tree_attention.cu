@@ -23,9 +23,13 @@ __device__ __forceinline__ float CachedElement(const void* plane, const __half* 
     return d * static_cast<float>((((e & 16) ? n >> 4 : n & 15)) - 8);
 }
 
-// One CTA per query row (sequence, token, head): warp w takes every eighth slot
-// from w, lane i the elements i, i + 32, .., with a running maximum and sum; the
-// warps' results are joined at the end.
+// Any head size, alignment and length; for what the matrix kernels do not take (fp32
+// rows without 16-byte alignment, planes of fewer slots than their unit).  One CTA per
+// query row (sequence, token, head): warp w takes every eighth slot from w, lane i
+// the elements i, i + 32, .., with a running maximum and sum; the warps' results
+// are joined at the end.  Bound: a dot product's latency (shuffles) per slot and warp,
+// and each row reads the cache again: 32 heads over 4000 slots of 8 x 256 in Q8_0
+// 912 us, the matrix kernel 19.
 template <int TYPE>
 __global__ void __launch_bounds__(kRowWarps * 32) TreeRowKernel(TreeArgs a) {
     __shared__ float so[kRowWarps][kMaxBlocks * 32];
@@ -82,8 +86,8 @@ __global__ void __launch_bounds__(kRowWarps * 32) TreeRowKernel(TreeArgs a) {
     }
 }
 
-// Head sizes up to 128 (fp32 caches: rows that allow 16-byte copies) and planes
-// of a unit or more.  Above 32 rows per KV head the tensor-memory kernel: 8
+// fp32 caches whose rows allow 16-byte copies, and planes of a unit or more.  Above
+// 32 rows per KV head the tensor-memory kernel: 8
 // sequences of 4000 slots, 8 x 128, take it 69.6 us at 32 rows and 69.8 at 40 in Q8_0,
 // the warp-level kernel 61.3 and 82.3 (Q4_0: 63.5 and 64.2 against 57.3 and 77.9); one
 // sequence of 8000 slots 32.2 and 32.8 against 26.6 and 30.7.

@@ -318,7 +318,7 @@ struct QuantWarp {
     static constexpr int kChunks = NB * kQuantBytes / 16;  // of a row
     // Rows of eight chunks are stored with chunk j at j ^ (row % 8), others an odd number of chunks apart: either
     // way the rows that a fragment load touches lie in different banks.
-    static constexpr bool kXor = kChunks == 8;
+    static constexpr bool kXor = TYPE == MLB_Q8_0 && kChunks == 8;
     static constexpr int kPitch = kXor ? 128 : (kChunks | 1) * 16;
     static constexpr int kPlane = kUnit * kPitch, kScales = kUnit * NB * 2;
     static constexpr int kStageBytes = kPlane + kScales;   // of K, and of V
@@ -1117,40 +1117,44 @@ __global__ void __launch_bounds__(kJoinWarps * 32) TreeJoinKernel(TreeArgs a, Tr
     const size_t part = size_t(item_rows) * (NB * 32 + 2);
     const unsigned each = (c1 - c0 + share) / share;  // parts of a warp
     const unsigned begin = c0 + warp % share * each, end = min(begin + each, c1 + 1);
+    constexpr int kFours = NB * 8;
     for (int base = blockIdx.y * at_once; base < rows; base += gridDim.y * at_once) {
-        const int r = base + warp / share, d = min(lane, NB * 8 - 1) * 4;
-        Joined x;
-        if (r < rows)
-            for (unsigned k = begin; k < end; k += kJoinBatch) {
-                float pm[kJoinBatch], pl[kJoinBatch];
-                float4 po[kJoinBatch];
 #pragma unroll
-                for (int j = 0; j < kJoinBatch; ++j) {
-                    // a CTA has two parts: of the item that it goes on with, and of one that it begins
-                    const unsigned cta = min(k + j, end - 1);
-                    const float* p = sp.parts + (2 * size_t(cta) + (cut.Start(cta) <= u0 ? 1 : 0)) * part;
-                    pm[j] = __ldcg(p + item_rows * NB * 32 + r);
-                    pl[j] = __ldcg(p + item_rows * (NB * 32 + 1) + r);
-                    po[j] = __ldcg(reinterpret_cast<const float4*>(p + r * NB * 32 + d));
+        for (int d0 = 0; d0 < kFours; d0 += 32) {
+            const int r = base + warp / share, d = min(d0 + lane, kFours - 1) * 4;
+            Joined x;
+            if (r < rows)
+                for (unsigned k = begin; k < end; k += kJoinBatch) {
+                    float pm[kJoinBatch], pl[kJoinBatch];
+                    float4 po[kJoinBatch];
+#pragma unroll
+                    for (int j = 0; j < kJoinBatch; ++j) {
+                        // a CTA has two parts: of the item that it goes on with, and of one that it begins
+                        const unsigned cta = min(k + j, end - 1);
+                        const float* p = sp.parts + (2 * size_t(cta) + (cut.Start(cta) <= u0 ? 1 : 0)) * part;
+                        pm[j] = __ldcg(p + item_rows * NB * 32 + r);
+                        pl[j] = __ldcg(p + item_rows * (NB * 32 + 1) + r);
+                        po[j] = __ldcg(reinterpret_cast<const float4*>(p + r * NB * 32 + d));
+                    }
+#pragma unroll
+                    for (int j = 0; j < kJoinBatch; ++j)
+                        if (k + j < end) x.Add(pm[j], pl[j], po[j]);
                 }
-#pragma unroll
-                for (int j = 0; j < kJoinBatch; ++j)
-                    if (k + j < end) x.Add(pm[j], pl[j], po[j]);
+            if constexpr (SHARED) {
+                __shared__ float sm[kJoinWarps], sl[kJoinWarps];
+                __shared__ float4 so[kJoinWarps][32];
+                if (lane == 0) {
+                    sm[warp] = x.m;
+                    sl[warp] = x.l;
+                }
+                so[warp][lane] = x.o;
+                __syncthreads();
+                if (warp % share == 0)
+                    for (int j = 1; j < share; ++j) x.Add(sm[warp + j], sl[warp + j], so[warp + j][lane]);
+                __syncthreads();
             }
-        if constexpr (SHARED) {
-            __shared__ float sm[kJoinWarps], sl[kJoinWarps];
-            __shared__ float4 so[kJoinWarps][32];
-            if (lane == 0) {
-                sm[warp] = x.m;
-                sl[warp] = x.l;
-            }
-            so[warp][lane] = x.o;
-            __syncthreads();
-            if (warp % share == 0)
-                for (int j = 1; j < share; ++j) x.Add(sm[warp + j], sl[warp + j], so[warp + j][lane]);
-            __syncthreads();
+            if (r < rows && warp % share == 0 && d0 + lane < kFours) StoreOut(a, OutRow(a, b, head, row0 + r), d, x.Result());
         }
-        if (r < rows && warp % share == 0 && lane < NB * 8) StoreOut(a, OutRow(a, b, head, row0 + r), d, x.Result());
     }
 }
 
@@ -1209,10 +1213,16 @@ bool LaunchShape(DeviceContext& ctx, const TreeArgs& a) {
 // 64.6 us, one tile 77.1; 32 rows of 8000 slots: 24.4 against 20.6).  Heads of more
 // than 64 elements leave no room for that: four warps a group above 16 rows (32 rows,
 // 8 x 4000 slots of 8 x 128: 116 us, two warps 133), two above 8 (16 rows: 72 us, one 103).
+// Heads of more than 128: one CTA per SM, as many groups as shared memory holds
+// (4 rows, 4000 slots of 8 x 256: Q8_0 18.9 us, Q4_0 18.4, fp32 36.4).
 template <int TYPE, int NB>
 bool LaunchRows(DeviceContext& ctx, const TreeArgs& a) {
     const long long rows = 1LL * a.tokens * a.group;
-    if constexpr (TYPE == MLB_F32 && NB > 2) {
+    if constexpr (NB > 4) {
+        constexpr int NW = TYPE == MLB_F32 ? 3 : 6;
+        if (rows <= kRows) return LaunchShape<TYPE, NB, 1, 1, NW, 1>(ctx, a);
+        return LaunchShape<TYPE, NB, 1, 2, TYPE == MLB_F32 ? 4 : 8, 1>(ctx, a);
+    } else if constexpr (TYPE == MLB_F32 && NB > 2) {
         if (rows <= kRows) return LaunchShape<TYPE, NB, 1, 1, 3, 2>(ctx, a);
         if (rows <= 2 * kRows) return LaunchShape<TYPE, NB, 1, 2, 4, 2>(ctx, a);
         return LaunchShape<TYPE, NB, 1, 4, 4, 2>(ctx, a);
@@ -1231,6 +1241,10 @@ bool LaunchBlocks(DeviceContext& ctx, const TreeArgs& a) {
         case 2: return LaunchRows<TYPE, 2>(ctx, a);
         case 3: return LaunchRows<TYPE, 3>(ctx, a);
         case 4: return LaunchRows<TYPE, 4>(ctx, a);
+        case 5: return LaunchRows<TYPE, 5>(ctx, a);
+        case 6: return LaunchRows<TYPE, 6>(ctx, a);
+        case 7: return LaunchRows<TYPE, 7>(ctx, a);
+        case 8: return LaunchRows<TYPE, 8>(ctx, a);
         default: return false;
     }
 }

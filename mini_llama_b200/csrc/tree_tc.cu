@@ -23,6 +23,11 @@
 // scale that is not finite in a drafted slot becomes 0 and the rows that see it
 // NaN in that block; one of 2^8 or more that no row sees becomes 0.
 //
+// Measured: 61-token trees of 16 sequences of 1024 to 4096 slots, 32 / 8 x 128 in Q4_0
+// 184 us, 683 TFLOP/s of fp16 products (42 % of the measured matrix rate).  A tile
+// takes some 7950 cycles, the softmax warps' time: 2460 of them the weights, 1700 the
+// maximum and the scores' wait, 1150 the item's start and end; the MMAs alone 3100.
+//
 // Bound: the MMAs, 6 x 128 x 128 x head_dim multiply-adds a tile (64 cycles for
 // 128 x 128 x 16), and the shared memory that they, the images' stores and the
 // other loads share.  One CTA per SM, roles by warp:
