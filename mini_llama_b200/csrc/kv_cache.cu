@@ -7,8 +7,8 @@
 // table, two stores); a cache unit is four elements of a 32-element block, so
 // the eight lanes of a block share its maximum by shuffles and store its quants
 // as 32 contiguous bytes (Q4_0: 16).  Measured: 4096 rows of 64 x 128 rotated 46 us (5.8
-// TB/s); 4096 rows of K and V of 8 x 128 into Q4_0 27 us (2.9 TB/s; 0.3 KB are read for
-// each write of 80 bytes, and the call is a few waves long), 32768 rows read from
+// TB/s); 4096 rows of K and V of 8 x 128 into Q4_0 27 us (2.9 TB/s: 128 bytes
+// read for 18 written, a call of few waves), 32768 rows read from
 // Q8_0 68 us (5.0 TB/s); decode steps of a few rows 6 to 11 us, a launch.  Each kernel has a form for shapes,
 // strides or addresses that do not allow 16-byte accesses.  All arithmetic uses
 // explicitly rounded operations in the order of mlb_rope and mlb_quantize, so
