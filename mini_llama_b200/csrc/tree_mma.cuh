@@ -33,13 +33,13 @@
 // The units (32 slots, fp32 16) of all (sequence, KV head, row group) items are one
 // list, cut evenly over the CTAs (the lengths are on the device, so every CTA
 // works the cut out from them): sequences of any lengths balance.  A CTA's
-// stretch is dealt out to groups of WQ warps, one tile pair of the item's rows
+// stretch is dealt out to groups of WQ warps, a tile (fp32: or two) of the item's rows
 // each; a group brings its units into a ring of S stages in shared memory
 // (cp.async, S - 1 units ahead; rows an odd number of 16-byte chunks apart, so
 // every fragment load is free of bank conflicts) and meets at a named barrier
 // once per unit.  The groups join their results in shared memory, and a second
 // kernel joins the items that are cut between CTAs (partials in the workspace,
-// added in the order of the CTAs).
+// added in a fixed order).
 #pragma once
 
 #include <algorithm>
