@@ -121,6 +121,10 @@ class TreeDecoder:
     def forward(self, tokens, parents) -> list[int]:
         """One pass over tree nodes whose root sits at position self.len; the model's choice after each node."""
         s, n, call = self.model.spec, len(tokens), self.lib.call
+        if not 1 <= n <= self.max_rows or len(parents) != n:
+            raise ValueError(f"a pass takes 1 to {self.max_rows} nodes with a parent each, not {n} and {len(parents)}")
+        if self.len + n > s["max_seq_len"]:
+            raise ValueError(f"{n} nodes after {self.len} tokens pass the cache's {s['max_seq_len']} slots")
         d, f, V = s["dim"], s["hidden_dim"], s["vocab_size"]
         depth = []
         for p in parents:
@@ -174,7 +178,13 @@ class TreeDecoder:
         """Greedy tokens after `prompt`, at most `draft` tree nodes to a pass: (tokens, passes)."""
         history, out, passes = [int(t) for t in prompt], [], 0
         room = self.model.spec["max_seq_len"]
-        assert len(history) + n_new + draft <= room, "the cache is too short"
+        if not history:
+            raise ValueError("the prompt is empty")
+        if draft > self.max_rows:
+            raise ValueError(f"{draft} nodes to a pass, but the decoder was made for {self.max_rows}")
+        if self.len + len(history) + n_new + draft > room:
+            raise ValueError(f"the cache's {room} slots are too few for {self.len} + {len(history)} tokens, {n_new} new ones "
+                             f"and {draft} drafted")
         for i in range(0, len(history) - 1, self.max_rows):  # the prompt but its last token, as chains
             part = history[i:min(i + self.max_rows, len(history) - 1)]
             self.forward(part, list(range(-1, len(part) - 1)))

@@ -1,7 +1,9 @@
 """Host side of decoding with drafted tokens: the tree of guesses, its masks and the accepted path."""
 import numpy as np
+import pytest
 
-from mini_llama_b200.tree_decode import accepted_path, draft_tree, tree_mask
+from mini_llama_b200 import capi
+from mini_llama_b200.tree_decode import SPECS, TreeDecoder, accepted_path, draft_tree, tree_mask
 
 
 def test_draft_tree_shares_beginnings_and_stays_in_size():
@@ -38,3 +40,61 @@ def test_accepted_path():
     tokens, parents = [4, 7, 8, 9], [-1, 0, 0, 2]
     assert accepted_path(tokens, parents, [8, 0, 9, 3]) == ([0, 2, 3], 3)
     assert accepted_path(tokens, parents, [5, 0, 0, 0]) == ([0], 5)
+
+
+class HostLib:
+    """Stands in for the library: notes the calls' names, hands out addresses."""
+
+    def __init__(self):
+        self.names, self.at = [], 1 << 20
+
+    def malloc(self, device, nbytes):
+        self.at += nbytes + 256
+        return self.at
+
+    def free(self, device, ptr):
+        pass
+
+    def call(self, name, *args):
+        self.names.append(name)
+
+
+class HostModel:
+    device, spec = 0, SPECS["tiny"]
+
+    def __init__(self):
+        self.lib = HostLib()
+
+    def weight(self, layer, kind):
+        return 1 << 16, 0
+
+
+@pytest.mark.parametrize("nodes,parents", [(17, 17), (0, 0), (5, 4)])
+def test_a_pass_of_too_many_nodes_is_refused(nodes, parents):
+    """The device buffers hold max_rows rows: more are refused before anything is copied or launched."""
+    d = TreeDecoder(HostModel(), capi.Q8_0, 16)
+    before = len(d.lib.names)
+    with pytest.raises(ValueError, match="nodes"):
+        d.forward([1] * nodes, list(range(-1, parents - 1)))
+    assert len(d.lib.names) == before
+
+
+def test_a_pass_beyond_the_cache_is_refused():
+    d = TreeDecoder(HostModel(), capi.Q8_0, 16)
+    d.len = SPECS["tiny"]["max_seq_len"] - 3
+    before = len(d.lib.names)
+    with pytest.raises(ValueError, match="slots"):
+        d.forward([1, 2, 3, 4], [-1, 0, 1, 2])
+    assert len(d.lib.names) == before
+
+
+@pytest.mark.parametrize("prompt,n_new,draft,kept", [([1, 2], 4, 17, 0), ([], 4, 4, 0), ([1] * 300, 200, 16, 0),
+                                                     ([1, 2], 100, 8, 405)])
+def test_generation_that_does_not_fit_is_refused(prompt, n_new, draft, kept):
+    """More drafted nodes than rows, no prompt, or more tokens than the cache has slots left."""
+    d = TreeDecoder(HostModel(), capi.Q8_0, 16)
+    d.len = kept
+    before = len(d.lib.names)
+    with pytest.raises(ValueError):
+        d.generate(prompt, n_new, draft)
+    assert len(d.lib.names) == before
