@@ -175,7 +175,8 @@ class TreeDecoder:
         self.len += len(path)
 
     def generate(self, prompt, n_new: int, draft: int):
-        """Greedy tokens after `prompt`, at most `draft` tree nodes to a pass: (tokens, passes)."""
+        """Greedy tokens after `prompt`, at most `draft` tree nodes to a pass: (tokens, passes).  The cache then holds
+        the prompt and all of them but the last, which a further call's prompt begins with."""
         history, out, passes = [int(t) for t in prompt], [], 0
         room = self.model.spec["max_seq_len"]
         if not history:
@@ -193,12 +194,15 @@ class TreeDecoder:
             tokens, parents = draft_tree(history, max(1, draft))
             choice = self.forward(tokens, parents)
             path, follow = accepted_path(tokens, parents, choice)
+            if len(path) > n_new - len(out):  # the cache keeps what is returned and no more
+                path = path[:n_new - len(out)]
+                follow = choice[path[-1]]
             self.keep(path)
             fresh = [tokens[i] for i in path[1:]] + [follow]
             history += fresh
             out += fresh
             passes += 1
-        return out[:n_new], passes
+        return out, passes
 
 
 def main(argv=None) -> int:

@@ -98,3 +98,25 @@ def test_generation_that_does_not_fit_is_refused(prompt, n_new, draft, kept):
     with pytest.raises(ValueError):
         d.generate(prompt, n_new, draft)
     assert len(d.lib.names) == before
+
+
+class CountingDecoder(TreeDecoder):
+    """The model's choice after a token is a fixed function of it, in a cycle of five, so that drafts are accepted."""
+
+    def forward(self, tokens, parents):
+        assert self.len + len(tokens) <= self.model.spec["max_seq_len"] and len(tokens) <= self.max_rows
+        return [(t + 1) % 5 for t in tokens]
+
+
+@pytest.mark.parametrize("draft", [1, 3, 8, 16])
+@pytest.mark.parametrize("n_new", [1, 6, 23, 24, 25])
+def test_the_cache_holds_what_was_returned(draft, n_new):
+    """A pass may accept more tokens than are asked for: those are not kept, and a further call goes on from the text."""
+    d = CountingDecoder(HostModel(), capi.Q8_0, 16)
+    prompt = [0, 1, 2, 3, 4] * 3
+    text, _ = d.generate(prompt, n_new, draft)
+    assert text == [i % 5 for i in range(n_new)]
+    assert d.len == len(prompt) + n_new - 1
+    more, _ = d.generate(text[-1:], 7, draft)
+    assert more == [(n_new + i) % 5 for i in range(7)]
+    assert d.len == len(prompt) + n_new + 6
