@@ -1104,14 +1104,16 @@ __global__ void __launch_bounds__(kJoinWarps * 32) TreeJoinKernel(TreeArgs a, Tr
     const unsigned item = blockIdx.x - b * items;
     const Cut cut(a, unit, items, groups, small, grid);
     const unsigned units = EntryUnits(a, b, unit, 1);
-    if (units == 0) return;
     unsigned first = 0;  // of the entry
     for (int b0 = 0; b0 < b; b0 += 32)
         first += __reduce_add_sync(0xffffffffu, b0 + lane < b ? EntryUnits(a, b0 + lane, unit, items) : 0);
+    // CTAs with nothing to join wait too: the next kernel may be a dependent of this one, whose wait covers the main
+    // kernel only if this one has not ended before it.
+    GridDepWait();
+    if (units == 0) return;
     const unsigned u0 = first + item * units;
     const unsigned c0 = cut.Owner(u0), c1 = cut.Owner(u0 + units - 1);
     if (c0 == c1) return;
-    GridDepWait();
     const int head = item / sp.groups, row0 = (item - head * sp.groups) * item_rows;
     const int rows = min(item_rows, sp.rows - row0), at_once = kJoinWarps / share;
     const size_t part = size_t(item_rows) * (NB * 32 + 2);

@@ -623,3 +623,48 @@ def test_empty_calls(mlb, gpu):
     mlb.call("mlb_attention_tree", gpu, c.ref, 0, 0, 1, None, None, 0, None, None, 32, 1, 0.0, None, 32)
     mlb.call("mlb_attention_tree", gpu, c.ref, 0, 1, 0, None, None, 0, None, None, 32, 1, 0.0, None, 32)
     mlb.sync(gpu)
+
+
+@pytest.mark.parametrize("qtype", [F32, Q80, Q40], ids=NAME.get)
+@pytest.mark.parametrize("heads,kv", [(32, 8), (16, 16)])
+@pytest.mark.parametrize("tokens,length", [(12, 20), (12, 100), (24, 90), (16, 1000)])
+def test_a_linear_right_behind_attention(mlb, gpu, qtype, heads, kv, tokens, length):
+    """The output projection queued right behind an attention call, both behind a longer kernel so that they run back
+    to back: the bits of the same calls one by one.  The linear's first kernel is a programmatic dependent of the
+    attention's last one; contexts of one unit (nothing to join) and longer ones, results alternating."""
+    rng = np.random.default_rng(tokens + length)
+    hd, dim = 64, 1024
+    n = heads * hd
+    c, _, _ = filled(mlb, gpu, rng, qtype, 1, length + tokens, kv, hd)
+    up = lambda a: DeviceArray.from_host(mlb, gpu, a)  # noqa: E731
+    qs = [up(rng.standard_normal((1, tokens, heads, hd)).astype(np.float32)) for _ in range(2)]
+    weights, blocks = up(rng.standard_normal((dim, n)).astype(np.float32)), DeviceArray(mlb, gpu, (dim * n // 32 * 34,), np.uint8)
+    mlb.call("mlb_quantize", gpu, Q80, weights.ptr, dim, n, blocks.ptr)
+    lens, mask = up(np.array([length], np.int32)), up(random_tree(rng, tokens)[None])
+    att, out = DeviceArray(mlb, gpu, (tokens, n)), [DeviceArray(mlb, gpu, (tokens, dim)) for _ in range(6)]
+    big = DeviceArray(mlb, gpu, (1 << 31,), np.uint8)
+
+    def attend(i):
+        mlb.call("mlb_attention_tree", gpu, c.ref, 0, 1, tokens, None, lens.ptr, length, mask.ptr, qs[i % 2].ptr, n, heads, 0.0,
+                 att.ptr, n)
+
+    def project(i):
+        mlb.call("mlb_quant_linear", gpu, Q80, att.ptr, blocks.ptr, dim * n // 32, tokens, n, dim, None, out[i].ptr)
+
+    want = []
+    for i in range(2):
+        attend(i)
+        mlb.sync(gpu)
+        project(i)
+        mlb.sync(gpu)
+        want.append(out[i].download())
+    assert np.isfinite(want[0]).all() and not same_bits(want[0], want[1])
+    for _ in range(5):
+        mlb.call("mlb_memset", gpu, att.ptr, 0xFF, att.nbytes)
+        mlb.call("mlb_memset", gpu, big.ptr, 0, big.nbytes)
+        for i in range(len(out)):
+            attend(i)
+            project(i)
+        mlb.sync(gpu)
+        for i, o in enumerate(out):
+            assert same_bits(o.download(), want[i % 2]), i
