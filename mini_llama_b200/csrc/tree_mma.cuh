@@ -15,8 +15,10 @@
 //   V      O^T = V^T P^T: quants as exact fp16 A fragments again (byte
 //          transposition in registers); the slot's scale of a block goes into
 //          the weights, P' = hi + lo of p d by one product and two FMAs on half
-//          pairs, relative to a power of two per row that covers the largest d
-//          seen.  Two MMAs per fragment.
+//          pairs, relative to a power of two that all scales of the unit lie close
+//          below, so that d 2^-e is a normal half, exact.  Where they spread wider
+//          (one slot with large values among others) the unit is summed in levels,
+//          each relative to its own power.  Two MMAs per fragment.
 // fp32 caches take the same path with mma.m16n8k8 on tf32 hi + lo pairs (three
 // products; no ranges to mind).  A unit's weighted values are summed in fresh
 // accumulators and added to the running ones in fp32 with rounding to nearest:
@@ -327,9 +329,11 @@ struct QuantWarp {
 
     Values<NB> v[1];
     Columns col[1];
-    int e;         // of row g: P' is relative to 2^e
-    float bound;   // 2^e
-    __half2 down;  // 2^-e
+    // P' is relative to 2^e, and takes scales above 2^(e - kSpan): with fewer binades than the 14 of the normal halves
+    // the products with small weights keep the rest.  (Every nonzero scale for the lowest e.)
+    static constexpr int kSpan = 8, kLowest = -15, kHighest = 15;  // powers that a half can scale by
+    float bound, least;  // 2^e, 2^(e - kSpan)
+    __half2 down;        // 2^-e
     // weights of the unit as B fragments: row (query) g, slots 2c, 2c + 1 (+ 8), hi and lo
     uint32_t ph[H][2], pl[H][2];
     bool edge;         // not every row sees all of the unit
@@ -387,8 +391,8 @@ struct QuantWarp {
     }
 
     __device__ __forceinline__ void SetPower(int to) {
-        e = to;
         bound = Pow2(to);
+        least = to > kLowest ? Pow2(to - kSpan) : 0.0f;
         down = __float2half2_rn(Pow2(-to));
     }
 
@@ -400,7 +404,7 @@ struct QuantWarp {
         ksp = a.c.ks + row * NB;
         vsp = a.c.vs + row * NB;
         v[0].Clear();
-        SetPower(-15);
+        SetPower(kLowest);
     }
 
     // K (or V) of the unit at p0 into a ring stage, by the COUNT threads of a group.
@@ -509,7 +513,7 @@ struct QuantWarp {
                         d[h][i][b] = __byte_perm(va[b >> 1], vb[b >> 1], b & 1 ? 0x7632 : 0x5410);
                 }
         }
-        __half2 big = AsHalf2(0u);
+        __half2 big = AsHalf2(0u), small = AsHalf2(0x7C007C00u);
 #pragma unroll
         for (int h = 0; h < H; ++h)
 #pragma unroll
@@ -517,22 +521,48 @@ struct QuantWarp {
                 if (edge) {  // a slot that is not seen may hold any scale, NaN too
                     const uint32_t see = __hne2_mask(AsHalf2(ph[h][i]), AsHalf2(0u));
 #pragma unroll
-                    for (int b = 0; b < NB; ++b) big = __hmax2(big, __habs2(AsHalf2(d[h][i][b] & see)));
-                } else {
+                    for (int b = 0; b < NB; ++b) d[h][i][b] &= see;
+                }
 #pragma unroll
-                    for (int b = 0; b < NB; ++b) big = __hmax2(big, __habs2(AsHalf2(d[h][i][b])));
+                for (int b = 0; b < NB; ++b) {
+                    const __half2 x = __habs2(AsHalf2(d[h][i][b]));
+                    big = __hmax2(big, x);
+                    small = __hmin2(small, x);
                 }
             }
-        const float top = fmaxf(__low2float(big), __high2float(big));
-        if (__any_sync(0xffffffffu, top > bound)) {
-            float t = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-            t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 2));
-            // 2^to > t, `to` within the powers that a half can scale by
-            const int to = max(e, min(15, max(-15, static_cast<int>(__float_as_uint(t) >> 23) - 126)));
-            const float f = Pow2(e - to);
-            SetPower(to);
-            v[0].Scale(__shfl_sync(0xffffffffu, f, 8 * s.c), __shfl_sync(0xffffffffu, f, 8 * s.c + 4));
+        const bool levels = __any_sync(0xffffffffu, fmaxf(__low2float(big), __high2float(big)) > bound ||
+                                                        !(fminf(__low2float(small), __high2float(small)) > least));
+        if (!levels) {
+            AddLevel<false>(s, stage, d);
+            return;
         }
+        // the largest scales, then the largest of those left, ..: at most six times: 40 binades, seven or more each
+        for (bool more = true; more;) {
+            const uint32_t t = __reduce_max_sync(0xffffffffu, __float_as_uint(fmaxf(__low2float(big), __high2float(big))));
+            SetPower(min(kHighest, max(kLowest, static_cast<int>(t >> 23) - 126)));  // 2^e > the largest
+            AddLevel<true>(s, stage, d);
+            big = AsHalf2(0u);
+#pragma unroll
+            for (int h = 0; h < H; ++h)
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+#pragma unroll
+                    for (int b = 0; b < NB; ++b) {
+                        d[h][i][b] &= ~Taken(d[h][i][b]);
+                        big = __hmax2(big, __habs2(AsHalf2(d[h][i][b])));
+                    }
+            more = __any_sync(0xffffffffu, H2(big) != 0);
+        }
+    }
+
+    // Which of a pair of scales the level takes (of the largest left; NaN too).
+    __device__ __forceinline__ uint32_t Taken(uint32_t d) const {
+        return ~__hle2_mask(__habs2(AsHalf2(d)), __float2half2_rn(least));
+    }
+
+    // The weighted values of the unit's slots with the scales d; LEVEL: those that it takes.
+    template <bool LEVEL>
+    __device__ __forceinline__ void AddLevel(const Step& s, const uint8_t* stage, const uint32_t (&d)[H][2][NB]) {
         const uint32_t row = SmemAddr(stage) + 2 * s.c * kPitch +
                              (kXor ? ((s.g >> 2) ^ (2 * s.c)) * 16 + 4 * (s.g & 3) : (kQuantBytes / 8) * s.g);
 #pragma unroll
@@ -567,7 +597,7 @@ struct QuantWarp {
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
                     uint32_t di = d[h][i][b];
-                    if (edge) di &= __hne2_mask(AsHalf2(ph[h][i]), AsHalf2(0u));
+                    if constexpr (LEVEL) di &= Taken(di);
                     const __half2 sc = __hmul2(AsHalf2(di), down);
                     const __half2 p = AsHalf2(ph[h][i]), y = __hmul2(p, sc);
                     hi[i] = H2(y);
@@ -580,13 +610,10 @@ struct QuantWarp {
                 }
             }
 #pragma unroll
-            for (int j = 0; j < 2; ++j) AddTo(v[0].o[b][j], t[j]);
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) v[0].o[b][j][i] = fmaf(t[j][i], bound, v[0].o[b][j][i]);
         }
-    }
-
-    __device__ __forceinline__ void End(const Step& s) {
-        const float f = Pow2(e);
-        v[0].Scale(__shfl_sync(0xffffffffu, f, 8 * s.c), __shfl_sync(0xffffffffu, f, 8 * s.c + 4));
     }
 };
 
@@ -773,8 +800,6 @@ struct F32Warp {
             }
         }
     }
-
-    __device__ __forceinline__ void End(const Step&) {}
 };
 
 template <int TYPE, int NB, int NT>
@@ -1027,7 +1052,6 @@ __global__ void __launch_bounds__(NW * 32, PER_SM) TreeMmaKernel(TreeArgs a, Tre
             if (tile < sp.rows) w.Sum(s, ring_ptr + kRing + stage);
             stage = stage + kStageBytes == kRing ? 0 : stage + kStageBytes;
         }
-        w.End(s);
         asm volatile("cp.async.wait_group 0;" ::: "memory");
         __syncthreads();  // the ring is free for the join
 #pragma unroll

@@ -668,3 +668,31 @@ def test_a_linear_right_behind_attention(mlb, gpu, qtype, heads, kv, tokens, len
         mlb.sync(gpu)
         for i, o in enumerate(out):
             assert same_bits(o.download(), want[i % 2]), i
+
+
+@pytest.mark.parametrize("qtype", [F32, Q80, Q40], ids=NAME.get)
+@pytest.mark.parametrize("heads,tokens", [(4, 2), (8, 4)])
+@pytest.mark.parametrize("hd", [64, 128, 160])
+@pytest.mark.parametrize("n", [40, 300])
+@pytest.mark.parametrize("common,outlier", [(0.05, 1e4), (0.05, 1e5), (1.0, 1e5)])
+@pytest.mark.parametrize("where", ["early", "block", "middle", "drafted"])
+def test_a_large_value_costs_the_others_no_precision(mlb, gpu, qtype, heads, tokens, hd, n, common, outlier, where):
+    """One slot (or one block of it) holds large values with next to no weight, or is a drafted one that a single token
+    sees: the rest is as exact as without it.  The slot's weight is e^-24 or less, so that the 2^-38 that a weight is off
+    by at most adds 2^-38 2e6 / 1 < 2^-17 of what the row sums, within (2^-19 24 + 2^-19) of it."""
+    rng = np.random.default_rng(n + hd)
+    c = Cache(mlb, gpu, qtype, 1, 1, n + tokens, 1, hd)
+    k = (0.3 * rng.standard_normal((n + tokens, 1, hd))).astype(np.float32)
+    v = (common * rng.standard_normal((n + tokens, 1, hd))).astype(np.float32)
+    q = np.abs(rng.standard_normal((1, tokens, heads, hd))).astype(np.float32)
+    at = {"early": 3, "block": 3, "middle": n // 2, "drafted": n + 1}[where]
+    part = slice(32, 64) if where == "block" else slice(None)
+    v[at, 0, part] = outlier * rng.standard_normal(v[at, 0, part].shape)
+    k[at] = -24.0 / (q[0].sum(-1).min() * hd ** -0.5)
+    mask = np.zeros((1, tokens, 1), np.uint64)
+    for t in range(tokens):
+        mask[0, t, 0] = 1 << t
+    c.write(0, None, list(range(n + tokens)), k, v)
+    kk, vv = ref.held(k, qtype)[None], ref.held(v, qtype)[None]
+    got = run_attention(mlb, gpu, c, 0, q, None, [n], n, mask)
+    assert_attention(got, *ref.attention(q, kk, vv, [n], [0], mask, hd ** -0.5, n + tokens))
