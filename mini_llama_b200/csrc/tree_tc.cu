@@ -17,11 +17,11 @@
 //                 tile, added to the running rows in registers in fp32 (the matrix
 //                 unit's own sums truncate)
 // Where |d q| could pass fp16's range (a scale of 2^8 or more) quants are taken times
-// 2^-9, undone in fp32: a K slot by itself, so that no slot's scores depend on
-// another's; V a whole tile at a time, resolved to 2^-31 of its largest value.
-// Slots that only some rows see may hold any bytes: K touches its own column only; a V
-// scale that is not finite in a drafted slot becomes 0 and the rows that see it
-// NaN in that block; one of 2^8 or more that no row sees becomes 0.
+// 2^-9, undone in fp32: a K slot by itself; a V tile with such scales is multiplied
+// twice, first its other blocks as they are, then these.  So no slot's values depend
+// on another's.  Slots that only some rows see may hold any bytes: K touches its own
+// column only; a V scale that is not finite in a drafted slot becomes 0 and the rows
+// that see it NaN in that block.
 //
 // Measured: 61-token trees of 16 sequences of 1024 to 4096 slots, 32 / 8 x 128 in Q4_0
 // 184 us, 683 TFLOP/s of fp16 products (42 % of the measured matrix rate).  A tile
@@ -66,7 +66,7 @@ constexpr int kProducers = kProdWarps * 32;
 constexpr int kQCol = 2 * kTile, kOCol = 3 * kTile;  // tensor-memory columns of Q and of O
 constexpr int kChunkPitch = 16 * kTile + 16;  // bytes between the chunks of eight elements in an image
 constexpr uint64_t kTcWait = 2000000000ull;
-constexpr int kInfoBufs = 4;     // tiles whose flags are kept
+constexpr int kInfoBufs = 4;     // images of K, and of V, whose flags are kept
 
 struct TcTreeShared {
     uint64_t q_full, v_full, v_empty, o_full, o_empty, drain;
@@ -78,10 +78,12 @@ struct TcTreeShared {
     float sum[2][kTile];     // the largest |q|
     float last[2][kTile];    // sums of the weights
     uint32_t flag[2][kProdWarps];
-    int k_big[kInfoBufs], v_big[kInfoBufs], v_odd[kInfoBufs];
+    int k_big[kInfoBufs], v_info[kInfoBufs];  // kOdd, kMore
     uint32_t k_bits[kInfoBufs][kTile / 32];      // slots of K taken times 2^-9, where k_big
-    uint32_t v_bad[kInfoBufs][4][kTile / 32];  // [tile][block][slots]: scales that are not finite, drafted slots
+    uint32_t v_bad[kInfoBufs][4][kTile / 32];  // [image][block][slots]: scales that are not finite, drafted slots
 };
+// Of an image of V: v_bad holds something; a second one of the same tile follows, of its large scales times 2^-9.
+constexpr int kOdd = 1, kMore = 2;
 constexpr int kTcHeaderBytes = 7168;
 static_assert(sizeof(TcTreeShared) <= kTcHeaderBytes, "header");
 
@@ -265,10 +267,11 @@ struct Share {
             if (at >= slots) d[j] = 0;
         }
     }
+    __device__ __forceinline__ static bool IsLarge(unsigned short d) { return (d & 0x7fffu) >= 0x5C00u; }  // 2^8, infinity, NaN
     __device__ __forceinline__ bool Big() const {
         bool big = false;
 #pragma unroll
-        for (int j = 0; j < kTasks; ++j) big = big || (d[j] & 0x7fffu) >= 0x5C00u;  // 2^8, infinity, NaN
+        for (int j = 0; j < kTasks; ++j) big = big || IsLarge(d[j]);
         return big;
     }
     // Takes out the scales that are not finite of rows from `from` on; whether there was one.
@@ -282,59 +285,63 @@ struct Share {
             }
         return odd;
     }
-    // Takes out the large scales of drafted slots that no token's mask shows.
-    __device__ __forceinline__ void TakeUnseen(const uint64_t* mask, int words, int tokens, int from, int id) {
+    // Piece q with the scale d into an image, within each group of four elements in the order 0, 2, 1, 3.
+    // BIG: the quants times `factor` (the scale itself could lose bits).
+    template <bool BIG>
+    __device__ __forceinline__ static void Convert(uint8_t* image, int row, int piece, const uint4& q, unsigned short d,
+                                                   uint32_t magic, uint32_t factor) {
+        constexpr int kLo = NB * 4 * kChunkPitch;  // of the lo image
+        const __half2 s = __half2half2(__ushort_as_half(d));
+        uint8_t* to = image + piece * ((TYPE == MLB_Q8_0 ? 2 : 4) * kChunkPitch) + row * 16;
+        const uint32_t w[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
-        for (int j = 0; j < kTasks; ++j) {
-            const int draft = Row(j, id) - from;
-            if ((d[j] & 0x7fffu) < 0x5C00u || draft < 0) continue;
-            bool seen = false;
-#pragma unroll 1
-            for (int t = 0; t < tokens && !seen; ++t)
-                seen = (__ldg(mask + size_t(t) * words + (draft >> 6)) >> (draft & 63)) & 1;
-            if (!seen) d[j] = 0;
+        for (int c = 0; c < (TYPE == MLB_Q8_0 ? 2 : 4); ++c) {  // eight elements each
+            const uint32_t w0 = w[2 * (c & 1)], w1 = w[2 * (c & 1) + 1];
+            uint32_t p[4];
+            if constexpr (TYPE == MLB_Q8_0) {
+                p[0] = EvenBytes(w0, magic);
+                p[1] = EvenBytes(w0 >> 8, magic);
+                p[2] = EvenBytes(w1, magic);
+                p[3] = EvenBytes(w1 >> 8, magic);
+            } else {
+                p[0] = c < 2 ? LowNibbles(w0, magic) : HighNibbles(w0, magic);
+                p[1] = c < 2 ? LowNibbles(w0 >> 8, magic) : HighNibbles(w0 >> 8, magic);
+                p[2] = c < 2 ? LowNibbles(w1, magic) : HighNibbles(w1, magic);
+                p[3] = c < 2 ? LowNibbles(w1 >> 8, magic) : HighNibbles(w1 >> 8, magic);
+            }
+            if constexpr (BIG)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) p[i] = H2(__hmul2(AsHalf2(p[i]), AsHalf2(factor)));
+            uint4 hi, lo;
+            Product(p[0], s, hi.x, lo.x);
+            Product(p[1], s, hi.y, lo.y);
+            Product(p[2], s, hi.z, lo.z);
+            Product(p[3], s, hi.w, lo.w);
+            *reinterpret_cast<uint4*>(to + c * kChunkPitch) = hi;
+            *reinterpret_cast<uint4*>(to + c * kChunkPitch + kLo) = lo;
+            asm volatile("" ::: "memory");  // one chunk's registers at a time
         }
     }
-    // Into the images: within each group of four elements in the order 0, 2, 1, 3.
-    // BIG: the rows whose bit is set in `down` (null: all) times 2^-9; the quants, as the scale could lose bits.
-    template <bool BIG>
-    __device__ __forceinline__ void Convert(uint8_t* image, int id, uint32_t magic, const uint32_t* down) const {
-        constexpr int kLo = NB * 4 * kChunkPitch;  // of the lo image
+    __device__ __forceinline__ void Convert(uint8_t* image, int id, uint32_t magic) const {
 #pragma unroll
+        for (int j = 0; j < kTasks; ++j)
+            if (Has(j, id)) Convert<false>(image, Row(j, id), Piece(j, id), q[j], d[j], magic, 0);
+    }
+    // A tile with large scales, read again (rare, and so without registers of its own): quants times `large` in the rows
+    // whose bit is set in `down` (null: in the blocks with a large scale), times `other` in the rest.  Scales that are
+    // not finite count as 0 from row `odd_from` on.
+    __device__ __forceinline__ static void ConvertLarge(uint8_t* image, const uint8_t* plane, const __half* scales, int p0,
+                                                        int slots, int last, int odd_from, int id, uint32_t magic,
+                                                        const uint32_t* down, uint32_t large, uint32_t other) {
+#pragma unroll 1
         for (int j = 0; j < kTasks; ++j) {
-            if (!Has(j, id)) continue;
-            const __half2 s = __half2half2(__ushort_as_half(d[j]));
-            const int at = Row(j, id);
-            const __half2 factor = AsHalf2(BIG && (!down || ((down[at >> 5] >> (at & 31)) & 1)) ? 0x18001800u : 0x3C003C00u);
-            uint8_t* to = image + Piece(j, id) * ((TYPE == MLB_Q8_0 ? 2 : 4) * kChunkPitch) + Row(j, id) * 16;
-            const uint32_t w[4] = {q[j].x, q[j].y, q[j].z, q[j].w};
-#pragma unroll
-            for (int c = 0; c < (TYPE == MLB_Q8_0 ? 2 : 4); ++c) {  // eight elements each
-                const uint32_t w0 = w[2 * (c & 1)], w1 = w[2 * (c & 1) + 1];
-                uint32_t p[4];
-                if constexpr (TYPE == MLB_Q8_0) {
-                    p[0] = EvenBytes(w0, magic);
-                    p[1] = EvenBytes(w0 >> 8, magic);
-                    p[2] = EvenBytes(w1, magic);
-                    p[3] = EvenBytes(w1 >> 8, magic);
-                } else {
-                    p[0] = c < 2 ? LowNibbles(w0, magic) : HighNibbles(w0, magic);
-                    p[1] = c < 2 ? LowNibbles(w0 >> 8, magic) : HighNibbles(w0 >> 8, magic);
-                    p[2] = c < 2 ? LowNibbles(w1, magic) : HighNibbles(w1, magic);
-                    p[3] = c < 2 ? LowNibbles(w1 >> 8, magic) : HighNibbles(w1 >> 8, magic);
-                }
-                if constexpr (BIG)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) p[i] = H2(__hmul2(AsHalf2(p[i]), factor));
-                uint4 hi, lo;
-                Product(p[0], s, hi.x, lo.x);
-                Product(p[1], s, hi.y, lo.y);
-                Product(p[2], s, hi.z, lo.z);
-                Product(p[3], s, hi.w, lo.w);
-                *reinterpret_cast<uint4*>(to + c * kChunkPitch) = hi;
-                *reinterpret_cast<uint4*>(to + c * kChunkPitch + kLo) = lo;
-                asm volatile("" ::: "memory");  // one chunk's registers at a time
-            }
+            if (!Has(j, id)) break;
+            const int at = Row(j, id), row = min(p0 + at, last), piece = Piece(j, id);
+            const uint4 x = __ldg(reinterpret_cast<const uint4*>(plane + size_t(row) * (kPieces * 16)) + piece);
+            unsigned short y = __ldg(reinterpret_cast<const unsigned short*>(scales + size_t(row) * NB + Block(piece)));
+            if (p0 + at >= slots || ((y & 0x7C00u) == 0x7C00u && at >= odd_from)) y = 0;
+            const bool take = down ? (down[at >> 5] >> (at & 31)) & 1 : IsLarge(y);
+            Convert<true>(image, at, piece, x, y, magic, take ? large : other);
         }
     }
 };
@@ -397,7 +404,7 @@ __global__ void __launch_bounds__(kTcWarps * 32, 1) TreeTcKernel(TreeArgs a, Tre
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftRegs));
         const int half = warp >> 2, row = (warp & 3) * 32 + lane;
         const uint32_t lanes = tmem + ((static_cast<uint32_t>(warp & 3) * 32) << 16);
-        int it = 0;  // tiles so far
+        int it = 0, pv = 0;  // tiles, and images of V, so far
         uint32_t met = 0;
         bool ok = true;
         while (ok && walk.Next(a, sp, items)) {
@@ -532,30 +539,45 @@ __global__ void __launch_bounds__(kTcWarps * 32, 1) TreeTcKernel(TreeArgs a, Tre
                     m_last = m;
                 }
                 if (u > walk.u0) {
-                    const int n = it - 1;
-                    if (!(ok = Wait(sh, &sh.o_full, n & 1, status))) break;
+                    if (!(ok = Wait(sh, &sh.o_full, pv & 1, status))) break;
                     FenceAfter();
                     const float keep = Exp2(m_of_o - m_last);
                     m_of_o = m_last;
-                    const float times = sh.v_big[n % kInfoBufs] ? 512.0f : 1.0f;
 #pragma unroll
                     for (int i = 0; i < kHalf; i += 16) {
                         float d[16];
                         Load16(lanes + kOCol + half * kHalf + i, d);
                         WaitLoad();
 #pragma unroll
-                        for (int j = 0; j < 16; ++j) o[i + j] = fmaf(d[j], times, o[i + j] * keep);
+                        for (int j = 0; j < 16; ++j) o[i + j] = fmaf(o[i + j], keep, d[j]);
                     }
-                    if (sh.v_odd[n % kInfoBufs])
+                    const int info = sh.v_info[pv % kInfoBufs];
+                    if (info & kOdd)
 #pragma unroll 1
                         for (int k = 0; k < kTile / 32; ++k) {
                             const uint32_t seen =
                                 SeenBits(mask, a.words, a.tokens, t, (u - 1) * kTile + 32 * k, walk.e.len, walk.e.slots);
                             for (int b = 0; b < NB; ++b)
-                                if (seen & sh.v_bad[n % kInfoBufs][b][k]) poison |= 1u << b;
+                                if (seen & sh.v_bad[pv % kInfoBufs][b][k]) poison |= 1u << b;
                         }
                     FenceBefore();
                     Arrive(&sh.o_empty);
+                    ++pv;
+                    if (info & kMore) {  // the tile's large scales
+                        if (!(ok = Wait(sh, &sh.o_full, pv & 1, status))) break;
+                        FenceAfter();
+#pragma unroll
+                        for (int i = 0; i < kHalf; i += 8) {
+                            uint32_t d[8];
+                            Load8(lanes + kOCol + half * kHalf + i, d);
+                            WaitLoad();
+#pragma unroll
+                            for (int j = 0; j < 8; ++j) o[i + j] = fmaf(__uint_as_float(d[j]), 512.0f, o[i + j]);
+                        }
+                        FenceBefore();
+                        Arrive(&sh.o_empty);
+                        ++pv;
+                    }
                 }
                 if (u < walk.u1) ++it;
             }
@@ -592,7 +614,7 @@ __global__ void __launch_bounds__(kTcWarps * 32, 1) TreeTcKernel(TreeArgs a, Tre
         // ------------------------------------------------ producers
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kProdRegs));
         const int id = threadIdx.x - kSoftWarps * 32;
-        int kt = 0, vt = 0;  // tiles of K and V so far
+        int kt = 0, vt = 0;  // images of K and V so far
         uint32_t met = 0;
         bool ok = true;
         // what the producers' `bits` hold together
@@ -625,8 +647,6 @@ __global__ void __launch_bounds__(kTcWarps * 32, 1) TreeTcKernel(TreeArgs a, Tre
                 const int u = tile(i);
                 // a drafted slot's V scale that is not finite is taken out and noted
                 const bool odd = v && r.TakeOdd(walk.e.len - u * kTile, id);
-                if (v && a.mask && r.Big())
-                    r.TakeUnseen(a.mask + size_t(walk.b) * a.tokens * a.words, a.words, a.tokens, walk.e.len - u * kTile, id);
                 const uint32_t flags = together((r.Big() ? 1u : 0u) | (odd ? 2u : 0u));
                 if (!ok) break;
                 const bool big = flags & 1, any = flags & 2;
@@ -646,13 +666,11 @@ __global__ void __launch_bounds__(kTcWarps * 32, 1) TreeTcKernel(TreeArgs a, Tre
                         if (lane == 0) sh.v_bad[n % kInfoBufs][b][id / 32] = bits;
                     }
                 }
-                if (id == 0) {
-                    (v ? sh.v_big : sh.k_big)[n % kInfoBufs] = big;
-                    if (v) sh.v_odd[n % kInfoBufs] = any;
-                }
+                const bool twice = v && big;  // a tile of V with large scales goes out as two images
+                if (id == 0) (v ? sh.v_info : sh.k_big)[n % kInfoBufs] = v ? (any ? kOdd : 0) | (twice ? kMore : 0) : int(big);
                 uint8_t* image = v ? vi : ki + (n & 1) * 2 * kImage;
                 if (!big) {
-                    r.template Convert<false>(image, id, sp.magic, nullptr);
+                    r.Convert(image, id, sp.magic);
                 } else {
                     uint32_t* down = sh.k_bits[n % kInfoBufs];
                     if (!v) {  // the slots that need it
@@ -660,13 +678,24 @@ __global__ void __launch_bounds__(kTcWarps * 32, 1) TreeTcKernel(TreeArgs a, Tre
                             const size_t at = min(u * kTile + id, a.c.head_slots - 1);
                             bool large = false;
                             for (int b = 0; b < NB; ++b)
-                                large = large || (__ldg(reinterpret_cast<const unsigned short*>(ks + at * NB + b)) & 0x7fffu) >= 0x5C00u;
+                                large = large || r.IsLarge(__ldg(reinterpret_cast<const unsigned short*>(ks + at * NB + b)));
                             const uint32_t bits = __ballot_sync(0xffffffffu, large);
                             if (lane == 0) down[id / 32] = bits;
                         }
                         if (!(ok = Meet(sh, &sh.prod, met, status))) break;
                     }
-                    r.template Convert<true>(image, id, sp.magic, v ? nullptr : down);
+                    constexpr uint32_t kOne = 0x3C003C00u, kDown = 0x18001800u;  // 1, 2^-9
+                    r.ConvertLarge(image, v ? vp : kp, v ? vs : ks, u * kTile, walk.e.slots, a.c.head_slots - 1,
+                                   v ? walk.e.len - u * kTile : kTile, id, sp.magic, v ? nullptr : down, v ? 0 : kDown, kOne);
+                    if (twice) {
+                        FenceAsync();
+                        Arrive(&sh.v_full);
+                        if (!(ok = Wait(sh, &sh.v_empty, n & 1, status))) break;
+                        ++vt;
+                        if (id == 0) sh.v_info[(n + 1) % kInfoBufs] = 0;
+                        r.ConvertLarge(image, vp, vs, u * kTile, walk.e.slots, a.c.head_slots - 1, walk.e.len - u * kTile, id,
+                                       sp.magic, nullptr, kDown, 0);
+                    }
                 }
                 FenceAsync();
                 Arrive(v ? &sh.v_full : &sh.k_full[n & 1]);
@@ -681,14 +710,14 @@ __global__ void __launch_bounds__(kTcWarps * 32, 1) TreeTcKernel(TreeArgs a, Tre
     }
     if (warp == kMmaWarp) {
         // ------------------------------------------------ MMA issue
-        const uint32_t qk = Instruction(kTile, false), pv = Instruction(HD, true);
+        const uint32_t qk = Instruction(kTile, false), pv_op = Instruction(HD, true);
         // K-major images: chunks of K kChunkPitch bytes apart, groups of 8 rows 128
         const uint64_t kd = Descriptor(SmemAddr(ki), kChunkPitch, 128);
         // V: groups of 8 slots 128 bytes apart, groups of 8 of head_dim kChunkPitch
         const uint64_t vd = Descriptor(SmemAddr(vi), 128, kChunkPitch);
         constexpr uint64_t kLoStep = kImage >> 4, kKStep = (2 * kChunkPitch) >> 4, kVStep = 256 >> 4;
         const uint32_t one = ElectOne(), base = __shfl_sync(0xffffffffu, tmem, 0);
-        int it = 0, item = 0;
+        int it = 0, pv = 0, item = 0;  // tiles, images of V, items
         bool ok = true;
         while (ok && walk.Next(a, sp, items)) {
             if (!(ok = Wait(sh, &sh.q_full, item & 1, status))) break;
@@ -698,7 +727,7 @@ __global__ void __launch_bounds__(kTcWarps * 32, 1) TreeTcKernel(TreeArgs a, Tre
                     if (!(ok = Wait(sh, &sh.k_full[it & 1], (it >> 1) & 1, status))) break;
                     // The weights that lay in this buffer, of tile it - 2, have been multiplied: its PV is the one issued
                     // last, but at the start of an item, where PV(it - 1) has been issued after O(it - 2) was read.
-                    if (it > 1 && u > walk.u0 && !(ok = Wait(sh, &sh.o_full, it & 1, status))) break;
+                    if (pv > 0 && u > walk.u0 && !(ok = Wait(sh, &sh.o_full, (pv - 1) & 1, status))) break;
                     FenceAfter();
                     const uint32_t d = base + (it & 1) * kTile, q = base + kQCol;
                     const uint64_t k = kd + (it & 1) * 2 * kLoStep;
@@ -712,24 +741,28 @@ __global__ void __launch_bounds__(kTcWarps * 32, 1) TreeTcKernel(TreeArgs a, Tre
                     Commit(one, &sh.k_empty[it & 1]);
                     Commit(one, &sh.s_full[it & 1]);
                 }
-                if (u > walk.u0) {  // PV of the tile before
-                    const int n = it - 1;
-                    if (!(ok = Wait(sh, &sh.v_full, n & 1, status) && Wait(sh, &sh.p_full[n & 1], (n >> 1) & 1, status))) break;
-                    if (n > 0 && !(ok = Wait(sh, &sh.o_empty, (n - 1) & 1, status))) break;  // the last O has been read
+                const int n = it - 1;  // PV of the tile before
+                if (u > walk.u0 && !(ok = Wait(sh, &sh.p_full[n & 1], (n >> 1) & 1, status))) break;
+#pragma unroll 1
+                for (bool more = u > walk.u0; more; ++pv) {
+                    if (!(ok = Wait(sh, &sh.v_full, pv & 1, status))) break;
+                    if (pv > 0 && !(ok = Wait(sh, &sh.o_empty, (pv - 1) & 1, status))) break;  // the last O has been read
                     FenceAfter();
                     const uint32_t p = base + (n & 1) * kTile;
-                    MmaTensor<false>(one, base + kOCol, p + 8, vd, pv);
+                    MmaTensor<false>(one, base + kOCol, p + 8, vd, pv_op);
 #pragma unroll
                     for (int s = 1; s < kTile / 16; ++s)
-                        MmaTensor<true>(one, base + kOCol, p + 16 * s + 8, vd + s * kVStep, pv);
+                        MmaTensor<true>(one, base + kOCol, p + 16 * s + 8, vd + s * kVStep, pv_op);
 #pragma unroll
                     for (int s = 0; s < kTile / 16; ++s)
-                        MmaTensor<true>(one, base + kOCol, p + 16 * s, vd + kLoStep + s * kVStep, pv);
+                        MmaTensor<true>(one, base + kOCol, p + 16 * s, vd + kLoStep + s * kVStep, pv_op);
 #pragma unroll
-                    for (int s = 0; s < kTile / 16; ++s) MmaTensor<true>(one, base + kOCol, p + 16 * s, vd + s * kVStep, pv);
+                    for (int s = 0; s < kTile / 16; ++s) MmaTensor<true>(one, base + kOCol, p + 16 * s, vd + s * kVStep, pv_op);
                     Commit(one, &sh.v_empty);
                     Commit(one, &sh.o_full);
+                    more = sh.v_info[pv % kInfoBufs] & kMore;
                 }
+                if (!ok) break;
                 if (u < walk.u1) ++it;
             }
         }

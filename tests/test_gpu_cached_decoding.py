@@ -671,7 +671,7 @@ def test_a_linear_right_behind_attention(mlb, gpu, qtype, heads, kv, tokens, len
 
 
 @pytest.mark.parametrize("qtype", [F32, Q80, Q40], ids=NAME.get)
-@pytest.mark.parametrize("heads,tokens", [(4, 2), (8, 4)])
+@pytest.mark.parametrize("heads,tokens", [(4, 2), (8, 4), (8, 9)])
 @pytest.mark.parametrize("hd", [64, 128, 160])
 @pytest.mark.parametrize("n", [40, 300])
 @pytest.mark.parametrize("common,outlier", [(0.05, 1e4), (0.05, 1e5), (1.0, 1e5)])
@@ -696,3 +696,27 @@ def test_a_large_value_costs_the_others_no_precision(mlb, gpu, qtype, heads, tok
     kk, vv = ref.held(k, qtype)[None], ref.held(v, qtype)[None]
     got = run_attention(mlb, gpu, c, 0, q, None, [n], n, mask)
     assert_attention(got, *ref.attention(q, kk, vv, [n], [0], mask, hd ** -0.5, n + tokens))
+
+
+@pytest.mark.parametrize("qtype", [Q80, Q40], ids=NAME.get)
+@pytest.mark.parametrize("share", [0.004, 0.5])
+def test_tiles_with_large_values_among_many_items(mlb, gpu, qtype, share):
+    """Row groups that follow one another in a CTA, some tiles with large V scales and some without: a tile that is
+    multiplied twice leaves the waits of the next ones in order (one that expired shows at the synchronisation)."""
+    rng = np.random.default_rng(17)
+    heads, kv, hd, tokens, length, n_seqs = 64, 8, 64, 20, 400, 24
+    c = Cache(mlb, gpu, qtype, n_seqs, 1, length + tokens, kv, hd)
+    k, v = (rng.standard_normal((n_seqs, length + tokens, kv, hd)).astype(np.float32) for _ in range(2))
+    v *= np.where(rng.random(v.shape[:3]) < share, 4e4, 1.0)[..., None].astype(np.float32)
+    for s in range(n_seqs):
+        c.write(0, [s] * (length + tokens), list(range(length + tokens)), k[s], v[s])
+    q = rng.standard_normal((n_seqs, tokens, heads, hd)).astype(np.float32)
+    mask = np.stack([random_tree(rng, tokens) for _ in range(n_seqs)])
+    lens = [length - 13 * i for i in range(n_seqs)]
+    got = run_attention(mlb, gpu, c, 0, q, None, lens, length, mask)
+    assert same_bits(got, run_attention(mlb, gpu, c, 0, q, None, lens, length, mask))
+    mlb.sync(gpu)
+    some = [0, n_seqs // 2, n_seqs - 1]
+    want = ref.attention(q[some], ref.held(k[some], qtype), ref.held(v[some], qtype), [lens[i] for i in some],
+                         range(len(some)), mask[some], hd ** -0.5, length + tokens)
+    assert_attention(got[some], *want)
