@@ -59,9 +59,10 @@ constexpr int kProdWarps = 8;    // producer warps
 constexpr int kMmaWarp = kSoftWarps + kProdWarps;
 constexpr int kTcWarps = kMmaWarp + 4;  // a whole warpgroup, for the register split
 // Registers of a softmax, a producer and an MMA thread: five warpgroups launched
-// with 96 each, 2 x 136 + 2 x 80 + 48 of their 5 x 96.
-constexpr int kSoftRegs = 136, kProdRegs = 80, kMmaRegs = 48;
-static_assert(2 * kSoftRegs + 2 * kProdRegs + kMmaRegs <= 5 * 96, "setmaxnreg draws on the launch's registers");
+// with 96 each, 2 x 136 + 2 x 80 + 48 of their 5 x 96.  (A launch with fewer would leave
+// setmaxnreg waiting for good: the launcher checks the compiled number.)
+constexpr int kSoftRegs = 136, kProdRegs = 80, kMmaRegs = 48, kLaunchRegs = 96;
+static_assert(2 * kSoftRegs + 2 * kProdRegs + kMmaRegs <= 5 * kLaunchRegs, "setmaxnreg draws on the launch's registers");
 constexpr int kProducers = kProdWarps * 32;
 constexpr int kQCol = 2 * kTile, kOCol = 3 * kTile;  // tensor-memory columns of Q and of O
 constexpr int kChunkPitch = 16 * kTile + 16;  // bytes between the chunks of eight elements in an image
@@ -796,6 +797,9 @@ bool LaunchTc(DeviceContext& ctx, const TreeArgs& a) {
     if (ctx.device >= 64 || !configured[ctx.device]) {
         CheckCuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kBytes),
                   "cudaFuncSetAttribute(TreeTcKernel)");
+        cudaFuncAttributes attr;
+        CheckCuda(cudaFuncGetAttributes(&attr, kernel), "cudaFuncGetAttributes(TreeTcKernel)");
+        Require(attr.numRegs >= kLaunchRegs, "mlb_attention_tree", "compiled with too few registers", MLB_ERR_UNSUPPORTED);
         if (ctx.device < 64) configured[ctx.device] = 1;
     }
     kernel<<<grid, kTcWarps * 32, kBytes, ctx.stream>>>(a, sp, ctx.status);
