@@ -346,6 +346,10 @@ int mlb_kv_cache_read(int device, const mlb_kv_cache* cache, int layer, int rows
  * knows (larger lens are taken as max_len); slots from max_seq_len on do not
  * exist.  scale 0: 1 / sqrt(head_dim).  head_dim up to 256.  out does not
  * overlap q.
+ * A K, V, scale or query that is not finite (an fp32 one of 2^128 (1 - 2^-12)
+ * or more counts as infinite) leaves the rows that see it or hold it without
+ * a specified value: NaN, infinite, or as if a slot whose score is -infinity
+ * were not there.  Other rows, heads, tokens and sequences are not affected.
  * Extends include/cuda_attention.h:10-14, which has one token of one sequence
  * over an fp32 cache. */
 int mlb_attention_tree(int device, const mlb_kv_cache* cache, int layer, int batch, int tokens,

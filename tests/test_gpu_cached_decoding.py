@@ -720,3 +720,62 @@ def test_tiles_with_large_values_among_many_items(mlb, gpu, qtype, share):
     want = ref.attention(q[some], ref.held(k[some], qtype), ref.held(v[some], qtype), [lens[i] for i in some],
                          range(len(some)), mask[some], hd ** -0.5, length + tokens)
     assert_attention(got[some], *want)
+
+
+@pytest.mark.parametrize("heads,kv,hd,tokens", [(4, 2, 64, 1), (12, 2, 64, 3), (8, 1, 64, 6), (8, 2, 128, 4), (2, 1, 160, 3),
+                                                (3, 1, 7, 2)])
+def test_fp32_values_up_to_the_largest(mlb, gpu, heads, kv, hd, tokens):
+    """Keys and values up to the largest that count as finite, the number below 2^128 (1 - 2^-12).  Each row sees one
+    slot, so that no weighted sum of its own passes fp32."""
+    rng = np.random.default_rng(hd)
+    top = np.array([0x7F7FEFFF], np.uint32).view(np.float32)[0]
+    c = Cache(mlb, gpu, F32, 1, 1, 40, kv, hd)
+    shape = (tokens, kv, hd)
+    k, v = ((top * rng.choice([1.0, -1.0, 0.51, 1 - 2.0 ** -12], shape)).astype(np.float32) for _ in range(2))
+    c.write(0, None, list(range(tokens)), k, v)
+    q = (1e-30 * rng.standard_normal((1, tokens, heads, hd))).astype(np.float32)
+    scale = np.float32(1e-10)
+    mask = np.array([[[1 << t] for t in range(tokens)]], np.uint64)
+    got = run_attention(mlb, gpu, c, 0, q, None, [0], 0, mask, scale=float(scale))
+    assert_attention(got, *ref.attention(q, k[None], v[None], [0], [0], mask, np.float64(scale), tokens))
+
+
+@pytest.mark.parametrize("qtype", [F32, Q80, Q40], ids=NAME.get)
+@pytest.mark.parametrize("heads,kv,hd,tokens", [(8, 2, 64, 1), (16, 2, 64, 3), (24, 2, 128, 5), (8, 2, 160, 3), (6, 2, 7, 2)])
+@pytest.mark.parametrize("value", [np.inf, -np.inf, np.nan])
+@pytest.mark.parametrize("where", ["k", "v", "query"])
+def test_committed_values_that_are_not_finite_stay_with_their_rows(mlb, gpu, qtype, heads, kv, hd, tokens, value, where):
+    """A committed slot of one KV head of one sequence, or one head of one query token, holds an infinity or NaN: all
+    other rows, of the same tile too, are as exact as ever, and calls after it as well."""
+    rng = np.random.default_rng(hd + tokens)
+    n, max_seq = 70, 96
+    c = Cache(mlb, gpu, qtype, 2, 1, max_seq, kv, hd)
+    k, v = (rng.standard_normal((2, n + tokens, kv, hd)).astype(np.float32) for _ in range(2))
+    q = rng.standard_normal((2, tokens, heads, hd)).astype(np.float32)
+    x = {"k": k, "v": v}
+    if where != "query":
+        x[where][0, 33, 1, 2] = value
+    for s in range(2):
+        c.write(0, [s] * (n + tokens), list(range(n + tokens)), k[s], v[s])
+    if qtype != F32 and where != "query":  # the quantizer keeps infinities as a scale, NaN not at all: put the scale in
+        at = ((0 * kv + 1) * max_seq + 33) * ((hd + 31) // 32) * 2
+        bits = np.array([value], np.float16)
+        mlb.call("mlb_memcpy_h2d", gpu, c.bufs[2 if where == "k" else 3].ptr + at, bits.ctypes.data, 2)
+        mlb.sync(gpu)
+    if where == "query":
+        q[0, tokens - 1, heads // 2 + 1, 3] = value
+    if where != "query":
+        x[where][0, 33, 1, 2] = 0
+    kk, vv = ref.held(k, qtype), ref.held(v, qtype)
+    safe = np.where(np.isfinite(q), q, 0)
+    want = ref.attention(safe, kk, vv, [n, n], [0, 1], None, hd ** -0.5, n + tokens)
+    touched = np.zeros((2, tokens, heads), bool)
+    if where == "query":
+        touched[0, tokens - 1, heads // 2 + 1] = True
+    else:
+        touched[0, :, heads // 2:] = True
+    got = run_attention(mlb, gpu, c, 0, q, None, [n, n], n, None)
+    mlb.sync(gpu)
+    assert_attention(got[~touched], *[w[~touched] for w in want])
+    if where != "k" and not np.isneginf(value):  # an element of V or a whole query: nothing hides it
+        assert not np.isfinite(got[touched]).all()
