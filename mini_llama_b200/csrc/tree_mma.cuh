@@ -55,11 +55,12 @@ namespace {
 
 constexpr int kSlots = 16;          // slots of a matrix step
 constexpr int kRows = 8;            // query rows of a tile
-constexpr float kStart = -1.7e38f;  // running maximum before the first score (finite: no inf - inf)
+constexpr float kStart = -3.4028235e38f;  // running maximum before the first score (the lowest finite: no inf - inf)
 constexpr float kLag = 2.0f;        // how far scores may pass the running maximum, in powers of two
 constexpr float kOffset = 12.0f;    // weights are relative to 2^12: at most 2^14, and the fp16 pairs resolve
                                     // 2^-37 of the largest, for slots that weigh little where the heavy ones hold zeros
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLeast = 1e-45f;  // a score factor is not 0: no inf * 0
 
 constexpr int kSmShared = 226 * 1024;  // shared memory of an SM for its CTAs
 constexpr int kMaxStages = 4;
@@ -119,6 +120,13 @@ __device__ __forceinline__ float Exp2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
+}
+
+// Exponent s with (top * 2^s) in [2^14, 2^15), for queries of any size: ScaleExp of the linears stops at 2^100 either
+// way.  Below 2^-112 the result stays smaller, with bits to spare, so that 2^-s is a normal number.
+__device__ __forceinline__ int QueryExp(float top) {
+    if (!(top > 0.0f) || !isfinite(top)) return 0;
+    return min(126, 14 - (static_cast<int>(__float_as_uint(top) >> 23) - 127));
 }
 
 __device__ __forceinline__ uint32_t H2(__half2 v) { return *reinterpret_cast<uint32_t*>(&v); }
@@ -199,8 +207,16 @@ __device__ __forceinline__ bool Sees(const Step& s, int t, int slot) {
     return slot < s.len || (draft && slot < s.slots);
 }
 
+// Whether a largest score `top` moves the running maximum m (both before their factor cs).
+__device__ __forceinline__ bool Passes(float top, float m, float cs) {
+    return (top - m) * cs > kLag;
+}
+// A part's maximum with its factor, in powers of two; l: the sum of its weights (0: nothing seen).
+__device__ __forceinline__ float Scaled(float m, float cs, float l) { return l > 0.0f ? fmaxf(m * cs, kStart) : kStart; }
+
 // One tile of rows: drafted tokens, running maxima and sums of the thread's two
-// score columns (queries 2c, 2c + 1).
+// score columns (queries 2c, 2c + 1).  The maxima are scores before their factor: only
+// differences are multiplied by it, so that scores of any size weigh 2^0 at their maximum.
 struct Columns {
     int t0, t1;
     float m[2], l[2], cs[2];
@@ -240,29 +256,26 @@ struct Columns {
             top0 = fmaxf(top0, fmaxf(x[h][0], x[h][2]));
             top1 = fmaxf(top1, fmaxf(x[h][1], x[h][3]));
         }
-        top0 *= cs[0];
-        top1 *= cs[1];
-        if (__any_sync(0xffffffffu, top0 > m[0] + kLag || top1 > m[1] + kLag)) {
+        if (__any_sync(0xffffffffu, Passes(top0, m[0], cs[0]) || Passes(top1, m[1], cs[1]))) {
 #pragma unroll
             for (int o = 4; o < 32; o <<= 1) {
                 top0 = fmaxf(top0, __shfl_xor_sync(0xffffffffu, top0, o));
                 top1 = fmaxf(top1, __shfl_xor_sync(0xffffffffu, top1, o));
             }
             const float n0 = fmaxf(m[0], top0), n1 = fmaxf(m[1], top1);
-            const float r0 = Exp2(m[0] - n0), r1 = Exp2(m[1] - n1);
+            const float r0 = Exp2((m[0] - n0) * cs[0]), r1 = Exp2((m[1] - n1) * cs[1]);
             m[0] = n0;
             m[1] = n1;
             l[0] *= r0;
             l[1] *= r1;
             rescale(r0, r1);
         }
-        const float o0 = offset - m[0], o1 = offset - m[1];
 #pragma unroll
         for (int h = 0; h < H; ++h) {
-            x[h][0] = Exp2(fmaf(x[h][0], cs[0], o0));
-            x[h][1] = Exp2(fmaf(x[h][1], cs[1], o1));
-            x[h][2] = Exp2(fmaf(x[h][2], cs[0], o0));
-            x[h][3] = Exp2(fmaf(x[h][3], cs[1], o1));
+            x[h][0] = Exp2(fmaf(x[h][0] - m[0], cs[0], offset));
+            x[h][1] = Exp2(fmaf(x[h][1] - m[1], cs[1], offset));
+            x[h][2] = Exp2(fmaf(x[h][2] - m[0], cs[0], offset));
+            x[h][3] = Exp2(fmaf(x[h][3] - m[1], cs[1], offset));
             l[0] += x[h][0] + x[h][2];
             l[1] += x[h][1] + x[h][3];
         }
@@ -376,8 +389,8 @@ struct QuantWarp {
         }
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        const int up = ScaleExp(top);  // largest |q| into [2^14, 2^15)
-        const float sc = Pow2(up), undo = fmaxf(Pow2(-up) * a.scale * kLog2e, 1e-37f);
+        const int up = QueryExp(top);  // largest |q| into [2^14, 2^15)
+        const float sc = Pow2(up), undo = fmaxf(Pow2(-up) * a.scale * kLog2e, kLeast);
 #pragma unroll
         for (int b = 0; b < NB; ++b)
 #pragma unroll
@@ -650,7 +663,7 @@ struct F32Warp {
                 SplitTf32(q && d + 1 < a.c.hd ? __ldg(q + d + 1) : 0.0f, f.y, f.w);
                 frags[(4 * b + i) * 32 + s.lane] = f;
             }
-        if (s.c == 0) undos[s.g] = fmaxf(a.scale * kLog2e, 1e-37f);
+        if (s.c == 0) undos[s.g] = fmaxf(a.scale * kLog2e, kLeast);
     }
 
     __device__ __forceinline__ void Begin(const TreeArgs& a, const TreeSplit&, int seq, int head) {
@@ -1077,8 +1090,8 @@ __global__ void __launch_bounds__(NW * 32, PER_SM) TreeMmaKernel(TreeArgs a, Tre
                         to[kPitch + d] = w.v[n].o[i][j][2 * h + 1];
                     }
             if (s.g == 0) {
-                sm[at] = col.m[0];
-                sm[at + 1] = col.m[1];
+                sm[at] = Scaled(col.m[0], col.cs[0], col.l[0]);
+                sm[at + 1] = Scaled(col.m[1], col.cs[1], col.l[1]);
                 sl[at] = col.l[0];
                 sl[at + 1] = col.l[1];
             }

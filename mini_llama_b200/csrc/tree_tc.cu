@@ -177,6 +177,17 @@ __device__ __forceinline__ void Store8(uint32_t at, const uint32_t (&r)[8]) {
 __device__ __forceinline__ void WaitLoad() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void WaitStore() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
+// Exponents of the weights of a pair of scores, (x - m) cs + offset: two adds and two FMAs as one of each.
+__device__ __forceinline__ void Exponents(float& x, float& y, uint64_t minus_m, uint64_t cs, uint64_t offset) {
+    asm("{\n\t.reg .b64 t;\n\tmov.b64 t, {%0, %1};\n\tadd.rn.f32x2 t, t, %2;\n\tfma.rn.f32x2 t, t, %3, %4;\n\t"
+        "mov.b64 {%0, %1}, t;\n\t}\n"
+        : "+f"(x), "+f"(y)
+        : "l"(minus_m), "l"(cs), "l"(offset));
+}
+__device__ __forceinline__ uint64_t Pair(float x, float y) {
+    return static_cast<uint64_t>(__float_as_uint(x)) | (static_cast<uint64_t>(__float_as_uint(y)) << 32);
+}
+
 // The items of a CTA, one after the other; every role walks them alike.
 struct Walk {
     unsigned cur, end, first;
@@ -439,9 +450,9 @@ __global__ void __launch_bounds__(kTcWarps * 32, 1) TreeTcKernel(TreeArgs a, Tre
                 sh.sum[half][row] = top;
                 if (!(ok = Meet(sh, &sh.soft, met, status))) break;
                 top = fmaxf(sh.sum[0][row], sh.sum[1][row]);
-                const int up = ScaleExp(top);
+                const int up = QueryExp(top);
                 const float sc = Pow2(up);
-                cs = fmaxf(Pow2(-up) * a.scale * kLog2e, 1e-37f);
+                cs = fmaxf(Pow2(-up) * a.scale * kLog2e, kLeast);
 #pragma unroll
                 for (int i = 0; i < kHalf; i += 16) {  // a k step: 8 columns of hi, 8 of lo
                     uint32_t hi[8], lo[8];
@@ -509,15 +520,14 @@ __global__ void __launch_bounds__(kTcWarps * 32, 1) TreeTcKernel(TreeArgs a, Tre
                     float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
                     sh.top[it & 1][half][row] = top;
                     if (!(ok = Meet(sh, &sh.soft, met, status))) break;
-                    top = fmaxf(top, sh.top[it & 1][half ^ 1][row]) * cs;
+                    top = fmaxf(top, sh.top[it & 1][half ^ 1][row]);
                     m_last = m;
-                    if (top > m + kLag) {
-                        const float f = Exp2(m - top);
+                    if (Passes(top, m, cs)) {
+                        const float f = Exp2((m - top) * cs);
                         l0 *= f;
                         l1 *= f;
                         m = top;
                     }
-                    const float off = kOffset - m;
 #pragma unroll 1
                     for (int i = 0; i < 64; i += 16) {
                         float x[16];
@@ -525,7 +535,8 @@ __global__ void __launch_bounds__(kTcWarps * 32, 1) TreeTcKernel(TreeArgs a, Tre
                         uint32_t hi[8], lo[8];
 #pragma unroll
                         for (int j = 0; j < 8; ++j) {
-                            const float p0 = Exp2(fmaf(x[2 * j], cs, off)), p1 = Exp2(fmaf(x[2 * j + 1], cs, off));
+                            Exponents(x[2 * j], x[2 * j + 1], Pair(-m, -m), Pair(cs, cs), Pair(kOffset, kOffset));
+                            const float p0 = Exp2(x[2 * j]), p1 = Exp2(x[2 * j + 1]);
                             l0 += p0;
                             l1 += p1;
                             SplitHalf(p0, p1, hi[j], lo[j]);
@@ -542,7 +553,7 @@ __global__ void __launch_bounds__(kTcWarps * 32, 1) TreeTcKernel(TreeArgs a, Tre
                 if (u > walk.u0) {
                     if (!(ok = Wait(sh, &sh.o_full, pv & 1, status))) break;
                     FenceAfter();
-                    const float keep = Exp2(m_of_o - m_last);
+                    const float keep = Exp2((m_of_o - m_last) * cs);
                     m_of_o = m_last;
 #pragma unroll
                     for (int i = 0; i < kHalf; i += 16) {
@@ -604,7 +615,7 @@ __global__ void __launch_bounds__(kTcWarps * 32, 1) TreeTcKernel(TreeArgs a, Tre
                         __stcg(reinterpret_cast<float4*>(part + row * HD + half * kHalf + i),
                                make_float4(o[i], o[i + 2], o[i + 1], o[i + 3]));
                     if (half == 0) {
-                        __stcg(part + kTile * HD + row, m);
+                        __stcg(part + kTile * HD + row, Scaled(m, cs, l));
                         __stcg(part + kTile * (HD + 1) + row, l);
                     }
                 }

@@ -779,3 +779,39 @@ def test_committed_values_that_are_not_finite_stay_with_their_rows(mlb, gpu, qty
     assert_attention(got[~touched], *[w[~touched] for w in want])
     if where != "k" and not np.isneginf(value):  # an element of V or a whole query: nothing hides it
         assert not np.isfinite(got[touched]).all()
+
+
+@pytest.mark.parametrize("qtype", [F32, Q80, Q40], ids=NAME.get)
+@pytest.mark.parametrize("heads,tokens", [(4, 1), (8, 4), (12, 6)])
+@pytest.mark.parametrize("k_mag,q_mag,scale", [(1e-4, 1e36, 1e-33), (3e4, 1e-36, 3e30), (3e4, 1e32, 1e-38)])
+def test_queries_and_scales_of_any_size(mlb, gpu, qtype, heads, tokens, k_mag, q_mag, scale):
+    """Queries near the ends of fp32's range, with scales that bring the scores back to the order of one."""
+    rng = np.random.default_rng(heads)
+    hd, n = 128, 150
+    c = Cache(mlb, gpu, qtype, 1, 1, n + tokens, 1, hd)
+    k = (k_mag * rng.standard_normal((n + tokens, 1, hd))).astype(np.float32)
+    v = rng.standard_normal((n + tokens, 1, hd)).astype(np.float32)
+    q = (q_mag * rng.standard_normal((1, tokens, heads, hd))).astype(np.float32)
+    c.write(0, None, list(range(n + tokens)), k, v)
+    kk, vv = ref.held(k, qtype)[None], ref.held(v, qtype)[None]
+    factor = float(np.float32(scale))
+    got = run_attention(mlb, gpu, c, 0, q, None, [n], n, None, scale=factor)
+    assert_attention(got, *ref.attention(q, kk, vv, [n], [0], None, factor, n + tokens))
+
+
+@pytest.mark.parametrize("qtype", [F32, Q80, Q40], ids=NAME.get)
+@pytest.mark.parametrize("heads,tokens", [(4, 1), (8, 4), (12, 6)])
+def test_a_single_slot_with_a_score_near_the_lowest(mlb, gpu, qtype, heads, tokens):
+    """One visible slot has all the weight, whatever its score: -64 q k down to -2.2e38 (-3.2e38 in powers of two)."""
+    rng = np.random.default_rng(tokens)
+    hd = 64
+    c = Cache(mlb, gpu, qtype, 1, 1, 40, 1, hd)
+    k = np.full((tokens, 1, hd), -1e5, np.float32)
+    v = rng.standard_normal((tokens, 1, hd)).astype(np.float32)
+    q = np.full((1, tokens, heads, hd), 2.2e38 / 64 / 1e5, np.float32)
+    q[0, :, ::2] *= 0.6
+    c.write(0, None, list(range(tokens)), k, v)
+    mask = np.array([[[1 << t] for t in range(tokens)]], np.uint64)
+    got = run_attention(mlb, gpu, c, 0, q, None, [0], 0, mask, scale=1.0)
+    want = np.broadcast_to(ref.held(v, qtype)[:, 0][None, :, None], got.shape)
+    assert (np.abs(got - want) <= 2.0 ** -19 * np.abs(want)).all()
