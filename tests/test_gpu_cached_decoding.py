@@ -17,7 +17,7 @@ import pytest
 
 import cached_decoding_ref as ref
 from mini_llama_b200 import capi
-from mini_llama_b200.device import DeviceArray
+from mini_llama_b200.device import DeviceArray, KvCache, RopeTable
 
 pytestmark = pytest.mark.gpu
 
@@ -815,3 +815,167 @@ def test_a_single_slot_with_a_score_near_the_lowest(mlb, gpu, qtype, heads, toke
     got = run_attention(mlb, gpu, c, 0, q, None, [0], 0, mask, scale=1.0)
     want = np.broadcast_to(ref.held(v, qtype)[:, 0][None, :, None], got.shape)
     assert (np.abs(got - want) <= 2.0 ** -19 * np.abs(want)).all()
+
+
+# ------------------------------------------------------------------------------------------------ rows, further
+def rows_of_planes(c):
+    """The cache's planes as [n_seqs, n_layers, kv, slot, bytes] views of fresh downloads."""
+    d, out = c.desc, []
+    blocks, stored = (d.head_dim + 31) // 32, (d.max_seq_len + 7) // 8 * 8
+    for i, p in enumerate(c.planes()):
+        if d.type == F32:
+            if i < 2:
+                out.append(p.reshape(d.n_seqs, d.n_layers, d.max_seq_len, d.n_kv_heads, d.head_dim * 4).swapaxes(2, 3))
+        else:
+            width = blocks * (2 if i > 1 else 32 if d.type == Q80 else 16)
+            out.append(p.reshape(d.n_seqs, d.n_layers, d.n_kv_heads, stored, width))
+    return out
+
+
+@pytest.mark.parametrize("qtype", [F32, Q80, Q40], ids=NAME.get)
+@pytest.mark.parametrize("kv,hd", [(2, 64), (3, 80), (1, 33)])
+def test_a_write_touches_its_rows_alone(mlb, gpu, qtype, kv, hd):
+    """Every byte of the planes outside the named slots of the named layer stays as it was."""
+    rng = np.random.default_rng(hd)
+    n_seqs, layers, max_seq, rows = 3, 2, 45, 67
+    c = Cache(mlb, gpu, qtype, n_seqs, layers, max_seq, kv, hd, fill=0x5A)
+    at = rng.permutation(n_seqs * max_seq)[:rows]
+    seqs, slots = (at // max_seq).astype(np.int32), (at % max_seq).astype(np.int32)
+    slots[[1, 5]], seqs[[2, 9]], slots[3], seqs[4] = -1, n_seqs, max_seq, -1
+    k, v = (rng.standard_normal((rows, kv, hd)).astype(np.float32) for _ in range(2))
+    c.write(1, seqs, slots, k, v)
+    kept = (slots >= 0) & (slots < max_seq) & (seqs >= 0) & (seqs < n_seqs)
+    for p in rows_of_planes(c):
+        named = np.zeros(p.shape[:4], bool)
+        named[seqs[kept], 1, :, slots[kept]] = True
+        assert (p[~named] == 0x5A).all()
+        assert (p[named] != 0x5A).any(axis=-1).all()
+    got_k, got_v = c.read(1, seqs, slots)
+    assert same_bits(got_k[kept], ref.held(k, qtype)[kept]) and same_bits(got_v[kept], ref.held(v, qtype)[kept])
+
+
+@pytest.mark.parametrize("qtype", [F32, Q80, Q40], ids=NAME.get)
+@pytest.mark.parametrize("layers,rows", [(1, 2401), (3, 803)])
+def test_large_calls_of_rows(mlb, gpu, qtype, layers, rows):
+    """More than 75776 blocks (two to a group of lanes), a remainder, skipped rows: write, rotate and write, read."""
+    rng = np.random.default_rng(rows)
+    kv, hd, heads, max_seq = 8, 128, 4, rows + 60
+    assert layers * rows * kv * hd // 32 > 75776 and rows % 2
+    slots = rng.permutation(max_seq)[:rows].astype(np.int32)
+    skip = rng.random(rows) < 0.02
+    slots[skip] = -1
+    slots[-1] = max_seq
+    kept = (slots >= 0) & (slots < max_seq)
+    k, v = (rng.standard_normal((layers, rows, kv, hd)).astype(np.float32) for _ in range(2))
+    up = lambda a: DeviceArray.from_host(mlb, gpu, a)  # noqa: E731
+    kd, vd, sd, n = up(k), up(v), up(slots), kv * hd
+    layer = capi.ALL_LAYERS if layers > 1 else 0
+    c = Cache(mlb, gpu, qtype, 1, layers, max_seq, kv, hd, fill=0x33)
+    mlb.call("mlb_kv_cache_write", gpu, c.ref, layer, rows, None, sd.ptr, kd.ptr, n, vd.ptr, n)
+    for p in rows_of_planes(c):
+        named = np.zeros(p.shape[:4], bool)
+        named[:, :, :, slots[kept]] = True
+        assert (p[~named] == 0x33).all()
+    kr, vr = (DeviceArray.from_host(mlb, gpu, np.full(k.shape, 7, np.float32)) for _ in range(2))
+    mlb.call("mlb_kv_cache_read", gpu, c.ref, layer, rows, None, sd.ptr, kr.ptr, n, vr.ptr, n)
+    for got, x in ((kr.download(), k), (vr.download(), v)):
+        assert same_bits(got[:, kept], ref.held(x, qtype)[:, kept]) and (got[:, ~kept] == 0).all()
+    if layers > 1:
+        return
+    table, buf = make_table(mlb, gpu, max_seq, hd, 64, True)
+    cs, pos = buf.download(), rng.integers(0, max_seq, rows).astype(np.int32)
+    q = rng.standard_normal((rows, heads, hd)).astype(np.float32)
+    qd, qo, pd = up(q), DeviceArray(mlb, gpu, q.shape), up(pos)
+    mlb.call("mlb_kv_cache_write_rope", gpu, c.ref, 0, rows, None, sd.ptr, ctypes.byref(table), pd.ptr, qd.ptr, heads * hd,
+             qo.ptr, heads * hd, heads, kd.ptr, n, vd.ptr, n)
+    mlb.call("mlb_kv_cache_read", gpu, c.ref, 0, rows, None, sd.ptr, kr.ptr, n, vr.ptr, n)
+    turn = lambda x: ref.rotate(x, cs[pos, :, 0], cs[pos, :, 1], 64, True)  # noqa: E731
+    assert same_bits(qo.download(), turn(q))
+    assert same_bits(kr.download()[0, kept], ref.held(turn(k[0]), qtype)[kept])
+    assert same_bits(vr.download()[0, kept], ref.held(v[0], qtype)[kept])
+
+
+@pytest.mark.parametrize("qtype", [F32, Q80, Q40], ids=NAME.get)
+def test_unaligned_values(mlb, gpu, qtype):
+    """V at odd addresses and strides, written and read."""
+    kv, hd, rows, gap = 2, 64, 6, 3
+    n = kv * hd
+    x = np.random.default_rng(3).standard_normal((rows, n + gap)).astype(np.float32)
+    xd = DeviceArray.from_host(mlb, gpu, x)
+    sd = DeviceArray.from_host(mlb, gpu, np.arange(rows, dtype=np.int32))
+    back = DeviceArray.from_host(mlb, gpu, np.full((rows, n + 5), 7, np.float32))
+    c = Cache(mlb, gpu, qtype, 1, 1, 8, kv, hd)
+    mlb.call("mlb_kv_cache_write", gpu, c.ref, 0, rows, None, sd.ptr, xd.ptr + 4, n + gap, xd.ptr + 8, n + gap)
+    flat = x.reshape(-1)
+    want = ref.held(np.stack([flat[2 + r * (n + gap):][:n] for r in range(rows)]).reshape(rows, kv, hd), qtype)
+    assert same_bits(c.read(0, None, list(range(rows)))[1], want)
+    mlb.call("mlb_kv_cache_read", gpu, c.ref, 0, rows, None, sd.ptr, None, 0, back.ptr + 4, n + 5)
+    got = back.download().reshape(-1)
+    assert same_bits(np.stack([got[1 + r * (n + 5):][:n] for r in range(rows)]).reshape(rows, kv, hd), want)
+    for r in range(rows - 1):
+        assert (got[1 + r * (n + 5) + n:1 + (r + 1) * (n + 5)] == 7).all()
+
+
+def test_python_wrappers(mlb, gpu):
+    """RopeTable and KvCache: rotate in place, write, read and attend give what the calls give."""
+    rng = np.random.default_rng(21)
+    heads, kv, hd, rows = 4, 2, 64, 5
+    q, k, v = (rng.standard_normal((rows, h, hd)).astype(np.float32) for h in (heads, kv, kv))
+    pos, slots = np.array([4, 0, 9, 2, 7], np.int32), np.arange(rows, dtype=np.int32)
+    qd, kd, vd, pd, sd = (DeviceArray.from_host(mlb, gpu, a) for a in (q, k, v, pos, slots))
+    table = RopeTable(mlb, gpu, 10, hd, 1e4, capi.ROPE_NEOX)
+    cs = table.angles.download()
+    table.rotate(rows, pd.ptr, qd.ptr, heads, kd.ptr, kv)
+    turned = [ref.rotate(x, cs[pos, :, 0], cs[pos, :, 1], hd, True) for x in (q, k)]
+    assert same_bits(qd.download(), turned[0]) and same_bits(kd.download(), turned[1])
+    for qtype in (F32, Q80, Q40):
+        c = KvCache(mlb, gpu, qtype, 1, 2, 24, kv, hd)
+        c.write(1, rows, sd.ptr, kd.ptr, vd.ptr)
+        kr, vr = DeviceArray(mlb, gpu, k.shape), DeviceArray(mlb, gpu, v.shape)
+        c.read(1, rows, sd.ptr, kr.ptr, vr.ptr)
+        kk, vv = ref.held(turned[1], qtype), ref.held(v, qtype)
+        assert same_bits(kr.download(), kk) and same_bits(vr.download(), vv)
+        lens, out = DeviceArray.from_host(mlb, gpu, np.zeros(1, np.int32)), DeviceArray(mlb, gpu, q.shape)
+        c.attend(1, 1, rows, lens.ptr, 0, qd.ptr, heads, out.ptr)
+        assert_attention(out.download()[None], *ref.attention(turned[0][None], kk[None], vv[None], [0], [0], None, hd ** -0.5, rows))
+
+
+@pytest.mark.parametrize("qtype", [F32, Q80, Q40], ids=NAME.get)
+@pytest.mark.parametrize("heads,tokens", [(4, 1), (8, 5)])
+def test_a_long_context(mlb, gpu, qtype, heads, tokens):
+    """40000 slots of one KV head, cut over every CTA."""
+    rng = np.random.default_rng(heads)
+    hd, n = 64, 40000
+    c, k, v = filled(mlb, gpu, rng, qtype, 1, n + tokens, 1, hd, k_scale=2.0)
+    q = rng.standard_normal((1, tokens, heads, hd)).astype(np.float32)
+    got = run_attention(mlb, gpu, c, 0, q, None, [n], n, None)
+    assert_attention(got, *ref.attention(q, k, v, [n], [0], None, hd ** -0.5, n + tokens))
+
+
+def test_calls_in_a_row_share_the_workspace(mlb, gpu):
+    """Attention calls of different shapes queued behind a longer kernel, no download between: the bits of each alone."""
+    rng = np.random.default_rng(31)
+    shapes = [(Q80, 32, 8, 128, 900, 5), (F32, 14, 2, 64, 3000, 3), (Q40, 16, 1, 128, 2500, 20), (Q80, 4, 1, 64, 5000, 1)]
+    up = lambda a: DeviceArray.from_host(mlb, gpu, a)  # noqa: E731
+    calls = []
+    for qtype, heads, kv, hd, n, tokens in shapes:
+        c, _, _ = filled(mlb, gpu, rng, qtype, 1, n + tokens, kv, hd)
+        q = up(rng.standard_normal((tokens, heads * hd)).astype(np.float32))
+        outs = [DeviceArray(mlb, gpu, (tokens, heads * hd)) for _ in range(3)]
+        calls.append((c, tokens, up(np.array([n], np.int32)), n, q, heads, heads * hd, outs))
+
+    def attend(call, out):
+        c, tokens, lens, n, q, heads, width, _ = call
+        mlb.call("mlb_attention_tree", gpu, c.ref, 0, 1, tokens, None, lens.ptr, n, None, q.ptr, width, heads, 0.0, out.ptr, width)
+
+    want = []
+    for call in calls:
+        attend(call, call[-1][0])
+        want.append(call[-1][0].download())
+    big = DeviceArray(mlb, gpu, (1 << 31,), np.uint8)
+    mlb.call("mlb_memset", gpu, big.ptr, 0, big.nbytes)
+    for i in (1, 2):
+        for call in calls:
+            attend(call, call[-1][i])
+    for call, w in zip(calls, want):
+        assert same_bits(call[-1][1].download(), w) and same_bits(call[-1][2].download(), w)
