@@ -434,7 +434,8 @@ struct QuantWarp {
             const int row = i / kChunks, chunk = i % kChunks;
             CopyChunk(stage + row * kPitch + (kXor ? chunk ^ (row & 7) : chunk) * 16, from + i * 16);
         }
-        constexpr int kSc = kScales / 16;  // at most 16
+        constexpr int kSc = kScales / 16;
+        static_assert(kSc <= COUNT, "a piece of scales to a thread");
         if (id < kSc) CopyChunk(stage + kPlane + id * 16, scales + size_t(p0) * NB + id * 8);
     }
     template <int COUNT>
