@@ -398,6 +398,8 @@ RotRows CheckedRot(const char* c, const char* name, const float* in, size_t in_s
     const size_t n = size_t(heads) * hd;
     Require(in_stride >= n && out_stride >= n, c, std::string(name) + " stride is shorter than a row");
     Require(in != out || in_stride == out_stride, c, std::string(name) + " in place needs equal strides");
+    RequireAligned(c, name, in, 4);
+    RequireAligned(c, (std::string(name) + " output").c_str(), out, 4);
     return {in, out, in_stride, out_stride, heads, in != out && rot < hd};
 }
 
@@ -438,13 +440,17 @@ void LaunchKvWrite(const char* caller, DeviceContext& ctx, const KvView& c, cons
     ByType(c.type, type);
 }
 
-void CheckKvRows(const char* c, const KvView& v, int rows, const int* slots, const void* k, size_t k_stride, const void* vv,
-                 size_t v_stride) {
+void CheckKvRows(const char* c, const KvView& v, int rows, const int* seqs, const int* slots, const void* k, size_t k_stride,
+                 const void* vv, size_t v_stride) {
     Require(rows >= 0, c, "row count is negative");
     if (rows == 0) return;
     Require(slots != nullptr, c, "slots is null");
     const size_t n = size_t(v.n_kv) * v.hd;
     Require((!k || k_stride >= n) && (!vv || v_stride >= n), c, "row stride is shorter than a row");
+    RequireAligned(c, "seqs", seqs, 4);
+    RequireAligned(c, "slots", slots, 4);
+    RequireAligned(c, "k", k, 4);
+    RequireAligned(c, "v", vv, 4);
 }
 
 // The pair frequencies of a table, scaled, in fp32.
@@ -588,8 +594,9 @@ int mlb_rope_rows(int device, const mlb_rope_table* table, int rows, const int* 
         const int hd = table->head_dim;
         Require(rows >= 0, c, "row count is negative");
         Require(n_heads >= 0 && n_kv_heads >= 0, c, "head count is negative");
-        if (rows == 0 || n_heads + n_kv_heads == 0) return;
+        if (rows == 0 || (n_heads == 0 && n_kv_heads == 0)) return;
         Require(positions != nullptr, c, "positions is null");
+        RequireAligned(c, "positions", positions, 4);
         const RotRows tq = CheckedRot(c, "q", q, q_stride, q_out, q_out_stride, n_heads, hd, r.rot);
         const RotRows tk = CheckedRot(c, "k", k, k_stride, k_out, k_out_stride, n_kv_heads, hd, r.rot);
         const bool vec = RopeVec(r, hd) && RotVec(tq) && RotVec(tk);
@@ -622,7 +629,7 @@ int mlb_kv_cache_write(int device, const mlb_kv_cache* cache, int layer, int row
         const char* c = "mlb_kv_cache_write";
         const KvView view = CheckedKvView(c, cache, true);
         CheckKvLayer(c, view, layer, true);
-        CheckKvRows(c, view, rows, slots, k, k_stride, v, v_stride);
+        CheckKvRows(c, view, rows, seqs, slots, k, k_stride, v, v_stride);
         if (rows == 0) return;
         Require(k && v, c, "k or v is null");
         const bool all = layer == MLB_ALL_LAYERS;
@@ -641,11 +648,12 @@ int mlb_kv_cache_write_rope(int device, const mlb_kv_cache* cache, int layer, in
         CheckKvLayer(c, view, layer, false);
         const RopeView r = CheckedRope(c, table);
         Require(table->head_dim == view.hd, c, "rope table and cache have different head_dim");
-        CheckKvRows(c, view, rows, slots, k, k_stride, v, v_stride);
+        CheckKvRows(c, view, rows, seqs, slots, k, k_stride, v, v_stride);
         Require(n_heads >= 0, c, "head count is negative");
         if (rows == 0) return;
         Require(k && v, c, "k or v is null");
         Require(positions != nullptr, c, "positions is null");
+        RequireAligned(c, "positions", positions, 4);
         const RotRows tq = CheckedRot(c, "q", q, q_stride, q_out, q_out_stride, n_heads, view.hd, r.rot);
         LaunchKvWrite<true>(c, Ctx(device), view, {seqs, slots, rows, k_stride, v_stride}, layer, 1, k, v, r, positions,
                             tq);
@@ -658,7 +666,7 @@ int mlb_kv_cache_read(int device, const mlb_kv_cache* cache, int layer, int rows
         const char* c = "mlb_kv_cache_read";
         const KvView view = CheckedKvView(c, cache, true);
         CheckKvLayer(c, view, layer, true);
-        CheckKvRows(c, view, rows, slots, k, k_stride, v, v_stride);
+        CheckKvRows(c, view, rows, seqs, slots, k, k_stride, v, v_stride);
         if (rows == 0) return;
         Require(k || v, c, "k and v are null");
         const bool all = layer == MLB_ALL_LAYERS;

@@ -122,6 +122,11 @@ int mlb_attention_tree(int device, const mlb_kv_cache* cache, int layer, int bat
         Require(lens && q && out, c, "lens, q or out is null");
         const size_t n = size_t(n_heads) * a.c.hd;
         Require(q_stride >= n && out_stride >= n, c, "row stride is shorter than a row");
+        RequireAligned(c, "lens", lens, 4);
+        RequireAligned(c, "seqs", seqs, 4);
+        RequireAligned(c, "mask", mask, 8);
+        RequireAligned(c, "q", q, 4);
+        RequireAligned(c, "out", out, 4);
         Require(seqs || batch <= a.c.n_seqs, c, "batch is larger than the cache's sequences");
         Require(1.0 * batch * tokens * n_heads < 2147483648.0, c, "too many query rows", MLB_ERR_UNSUPPORTED);
         a.layer = layer;

@@ -1219,11 +1219,12 @@ void LaunchJoin(DeviceContext& ctx, const TreeArgs& a, const TreeSplit& sp, int 
                 int grid) {
     const int all = a.batch * a.c.n_kv * sp.groups;
     int share = 1;
-    while (share < kJoinWarps && share * kJoinBatch * all < grid) share *= 2;
+    while (share < kJoinWarps && 1LL * share * kJoinBatch * all < grid) share *= 2;
     // as many rows at once as do not make many more CTAs than the device holds
     const int rows = std::min(item_rows, sp.rows);
     const int per_item = std::max(1, std::min<int>(CeilDiv(rows * share, kJoinWarps), 16 * ctx.sm_count / all));
-    Launch("TreeJoinKernel", share > 1 ? TreeJoinKernel<NB, true> : TreeJoinKernel<NB, false>, dim3(all, per_item), dim3(kJoinWarps * 32), 0, ctx.stream, true, a, sp, unit, groups, small, item_rows, grid, share);
+    Launch("TreeJoinKernel", share > 1 ? TreeJoinKernel<NB, true> : TreeJoinKernel<NB, false>, dim3(all, per_item),
+           dim3(kJoinWarps * 32), 0, ctx.stream, true, a, sp, unit, groups, small, item_rows, grid, share);
 }
 
 template <int TYPE, int NB, int NT, int WQ, int NW, int PER_SM>

@@ -136,3 +136,36 @@ def test_bytes(lib, qtype, hd, plane, scale):
     p, s = ctypes.c_size_t(), ctypes.c_size_t()
     lib.call("mlb_kv_cache_bytes", ref(c), ctypes.byref(p), ctypes.byref(s))
     assert (p.value, s.value) == (plane * 2 * 2 * 2, scale * 2 * 2 * 2)
+
+
+@pytest.mark.parametrize("which,text", [("seqs", "seqs is not 4-byte"), ("slots", "slots is not 4-byte"), ("k", "k is not 4-byte"),
+                                        ("v", "v is not 4-byte")])
+def test_rows_off_their_boundary(lib, which, text):
+    """Pointers that are not on their elements' boundary are refused, not sent to the device."""
+    a = dict(seqs=P, slots=P, k=P, v=P)
+    a[which] += 2
+    for name in ("mlb_kv_cache_write", "mlb_kv_cache_read"):
+        refused(lib, BAD, text, name, 0, ref(cache()), 0, 1, a["seqs"], a["slots"], a["k"], 128, a["v"], 128)
+    refused(lib, BAD, text, "mlb_kv_cache_write_rope", 0, ref(cache()), 0, 1, a["seqs"], a["slots"], ref(table()), P, P, 256, P,
+            256, 4, a["k"], 128, a["v"], 128)
+
+
+@pytest.mark.parametrize("which,text", [("positions", "positions"), ("q", "q is not"), ("q_out", "q output"), ("k", "k is not"),
+                                        ("k_out", "k output")])
+def test_rotated_rows_off_their_boundary(lib, which, text):
+    a = dict(positions=P, q=P, q_out=4 * P, k=P, k_out=4 * P)
+    a[which] += 1
+    refused(lib, BAD, text, "mlb_rope_rows", 0, ref(table()), 1, a["positions"], a["q"], 256, a["q_out"], 256, 4, a["k"], 128,
+            a["k_out"], 128, 2)
+    refused(lib, BAD, "positions", "mlb_kv_cache_write_rope", 0, ref(cache()), 0, 1, P, P, ref(table()), P + 2, P, 256, P, 256, 4,
+            P, 128, P, 128)
+
+
+@pytest.mark.parametrize("which,step,text", [("seqs", 2, "seqs is not 4-byte"), ("lens", 1, "lens is not 4-byte"),
+                                             ("mask", 4, "mask is not 8-byte"), ("q", 2, "q is not 4-byte"),
+                                             ("out", 2, "out is not 4-byte")])
+def test_attention_off_its_boundary(lib, which, step, text):
+    a = dict(seqs=P, lens=P, mask=P, q=P, out=P)
+    a[which] += step
+    refused(lib, BAD, text, "mlb_attention_tree", 0, ref(cache()), 0, 1, 2, a["seqs"], a["lens"], 8, a["mask"], a["q"], 256, 4, 0.0,
+            a["out"], 256)
