@@ -306,8 +306,11 @@ int mlb_kv_cache_bytes(const mlb_kv_cache* cache, size_t* plane_bytes, size_t* s
  * seqs NULL: sequence 0), quantized by the rule of mlb_quantize with the scale
  * as fp16(amax * fl(1/127)) (Q4_0: fl(1/7)), a product where mlb_quantize
  * divides; the two differ in the last bit of about one Q4_0 scale in 40 000.
- * MLB_F32: copied.  A row whose sequence or slot is outside the cache is skipped, so -1
- * marks padding; the other rows must name different (sequence, slot) pairs.
+ * As there, a NaN becomes a finite value (Q8_0: 0, Q4_0: -8 times the scale),
+ * and a block with an infinity, or with a value that takes the scale past
+ * fp16's range (65504 * 127, 65504 * 7), an infinite scale.  MLB_F32: copied.
+ * A row whose sequence or slot is outside the cache is skipped, so -1 marks
+ * padding; the other rows must name different (sequence, slot) pairs.
  * layer MLB_ALL_LAYERS: k and v hold `rows` rows for each layer, layer after
  * layer, and every layer takes its own at the same slots. */
 int mlb_kv_cache_write(int device, const mlb_kv_cache* cache, int layer, int rows, const int* seqs,

@@ -6,13 +6,17 @@
 // them once.  A rotation unit is four pairs (two 16-byte loads, two of the
 // table, two stores); a cache unit is four elements of a 32-element block, so
 // the eight lanes of a block share its maximum by shuffles and store its quants
-// as 32 contiguous bytes (Q4_0: 16).  Measured: 4096 rows of 64 x 128 rotated 46 us (5.8
-// TB/s); 4096 rows of K and V of 8 x 128 into Q4_0 27 us (2.9 TB/s: 128 bytes
-// read for 18 written, a call of few waves), 32768 rows read from
-// Q8_0 68 us (5.0 TB/s); decode steps of a few rows 6 to 11 us, a launch.  Each kernel has a form for shapes,
+// as 32 contiguous bytes (Q4_0: 16).  Measured, each call by itself: 4096 rows of 64 x 128
+// rotated 47 us (5.7 TB/s); 4096 rows of K and V of 8 x 128 written to Q4_0 / Q8_0 / fp32
+// 16.4 / 15.0 / 14.4 us (2.3 / 2.8 / 4.7 TB/s) and read 12.3 / 12.3 / 14.3 (3.1 / 3.5 / 4.7),
+// with 32 query heads rotated and written 43 / 43 / 39 (4.1 / 4.2 / 5.2); 32768 rows
+// written 96 / 94 / 83 (3.2 / 3.6 / 6.4) and read 68 / 68 / 84 (4.5 / 5.0 / 6.4); decode
+// steps of a few rows 4.5 to 6.5 us, a launch.  So fp32 rows run at the copy rate,
+// and the quantizing write at half of it.  Each kernel has a form for shapes,
 // strides or addresses that do not allow 16-byte accesses.  All arithmetic uses
-// explicitly rounded operations in the order of mlb_rope and mlb_quantize, so
-// the results equal theirs bit for bit.
+// explicitly rounded operations: rotations equal mlb_rope's and blocks mlb_quantize's
+// bit for bit, except that a scale is amax times fl(1/127) or fl(1/7) where
+// mlb_quantize divides, which differs in the last bit of about one Q4_0 scale in 40 000.
 #include <algorithm>
 #include <cmath>
 #include <type_traits>

@@ -87,10 +87,12 @@ __global__ void __launch_bounds__(kRowWarps * 32) TreeRowKernel(TreeArgs a) {
 }
 
 // fp32 caches whose rows allow 16-byte copies, and planes of a unit or more.  Above
-// 32 rows per KV head the tensor-memory kernel: 8
-// sequences of 4000 slots, 8 x 128, take it 69.6 us at 32 rows and 69.8 at 40 in Q8_0,
-// the warp-level kernel 61.3 and 82.3 (Q4_0: 63.5 and 64.2 against 57.3 and 77.9); one
-// sequence of 8000 slots 32.2 and 32.8 against 26.6 and 30.7.
+// 32 rows per KV head the tensor-memory kernel.  At 32, 40 and 64 rows it takes 67.7, 68.8
+// and 70.3 us for 8 sequences of 4000 slots, 8 x 128 in Q8_0, the warp-level kernel 61.5,
+// 84.0 and 107.3 (Q4_0: 65.0, 65.5, 67.6 against 57.3, 77.8, 99.3); for one of 2000 slots
+// 18.4, 18.4, 20.1 against 18.4, 20.5, 22.5.  For one of 8000 it gains later: 32.8, 32.8,
+// 34.8 against 28.0, 32.8, 36.9 in Q8_0 and 31.4, 32.8, 34.8 against 26.7, 30.7, 36.5 in
+// Q4_0, where the rule by rows alone costs 7 % at 40.
 bool LaunchTreeMma(DeviceContext& ctx, const TreeArgs& a) {
     if (a.c.type == MLB_F32) return a.cache_vec && LaunchTreeF32(ctx, a);
     if (1LL * a.tokens * a.group > 32 && LaunchTreeTc(ctx, a)) return true;

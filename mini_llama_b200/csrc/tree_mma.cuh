@@ -26,11 +26,12 @@
 // cost several times the fp32 rounding.
 //
 // Bound: a decode step over long sequences (4 rows, 32 sequences, 304 MB in Q8_0)
-// runs at 4.2 TB/s, 64 % of the copy rate; the instructions of a unit (conversion,
+// runs at 4.1 TB/s, 62 % of the copy rate; the instructions of a unit (conversion,
 // fragments, softmax) take about as long as its bytes, and overlap them in part.
-// In 4 bits (151 MB, 32 K slots) the instructions alone bound it: 2.5 TB/s.  From 16
-// rows on it is instructions and matrix products, for fp32 the tf32 products (three
-// for one: 48 % of the tensor pipe's cycles).
+// In 4 bits (151 MB, 32 K slots) it is the instructions: 2.5 TB/s.  Neither the issue
+// slots (58 and 55 %) nor a pipe is full: with three warps to a scheduler the
+// dependences within a unit show.  From 16 rows on it is instructions and matrix products,
+// for fp32 the tf32 products (three for one: 49 % of the tensor pipe's cycles).
 //
 // The units (32 slots, fp32 16) of all (sequence, KV head, row group) items are one
 // list, cut evenly over the CTAs (the lengths are on the device, so every CTA
@@ -1262,14 +1263,14 @@ bool LaunchShape(DeviceContext& ctx, const TreeArgs& a) {
 // second reads the cache from L2).  8 sequences of 4000 slots, 8 x 128 in Q8_0: 16
 // rows 36.9 us (groups of 8: 39.2), 32 rows 61.3 (63.0); in Q4_0 34.8 (36.9), 57.3 (59.4).
 // Three CTAs of four warps begin and end their items independently: 32 sequences
-// of 500 to 8192 slots, four rows, take 73 us, with two CTAs of six warps 84.
+// of 500 to 8192 slots, four rows, took 73 us, with two CTAs of six warps 84.
 // fp32 caches are bound by the tf32 products: above 32 rows two tiles to a warp
 // halve the splits of K and V (49 rows, 2 x 64, 8 sequences of 2000 to 16384 slots:
-// 64.6 us, one tile 77.1; 32 rows of 8000 slots: 24.4 against 20.6).  Heads of more
+// 65 us, one tile 77; 32 rows of 8000 slots: 24.4 against 20.6).  Heads of more
 // than 64 elements leave no room for that: four warps a group above 16 rows (32 rows,
-// 8 x 4000 slots of 8 x 128: 116 us, two warps 133), two above 8 (16 rows: 72 us, one 103).
+// 8 x 4000 slots of 8 x 128: 117 us, two warps 133), two above 8 (16 rows: 76 us, one 103).
 // Heads of more than 128: one CTA per SM, as many groups as shared memory holds
-// (4 rows, 4000 slots of 8 x 256: Q8_0 18.9 us, Q4_0 18.4, fp32 36.4).
+// (4 rows, 4000 slots of 8 x 256: Q8_0 19.5 us, Q4_0 18.4, fp32 36.9).
 template <int TYPE, int NB>
 bool LaunchRows(DeviceContext& ctx, const TreeArgs& a) {
     const long long rows = 1LL * a.tokens * a.group;

@@ -17,15 +17,15 @@
 //                 tile, added to the running rows in registers in fp32 (the matrix
 //                 unit's own sums truncate)
 // Where |d q| could pass fp16's range (a scale of 2^8 or more) quants are taken times
-// 2^-9, undone in fp32: a K slot by itself; a V tile with such scales is multiplied
-// twice, first its other blocks as they are, then these.  So no slot's values depend
-// on another's.  Slots that only some rows see may hold any bytes: K touches its own
-// column only; a V scale that is not finite in a drafted slot becomes 0 and the rows
-// that see it NaN in that block.
+// 2^-9, undone in fp32: a K slot by itself (its other blocks then resolve to 2^-16);
+// a V tile with such scales is multiplied twice, first its other blocks as they are,
+// then these.  So no slot's values depend on another's.  Slots that only some rows see
+// may hold any bytes: K touches its own column only; a V scale that is not finite in a
+// drafted slot becomes 0 and the rows that see it NaN in that block.
 //
 // Measured: 61-token trees of 16 sequences of 1024 to 4096 slots, 32 / 8 x 128 in Q4_0
-// 184 us, 683 TFLOP/s of fp16 products (42 % of the measured matrix rate).  A tile
-// takes some 7950 cycles, the softmax warps' time: 2460 of them the weights, 1700 the
+// 187 us, 673 TFLOP/s of fp16 products (41 % of the measured matrix rate); where one
+// slot in 500 has a large V scale 208.  A tile takes some 7950 cycles, the softmax warps' time: 2460 of them the weights, 1700 the
 // maximum and the scores' wait, 1150 the item's start and end; the MMAs alone 3100.
 //
 // Bound: the MMAs, 6 x 128 x 128 x head_dim multiply-adds a tile (64 cycles for

@@ -7,7 +7,8 @@ tree rows go through the linears together, mlb_kv_cache_write_rope rotates q and
 bits, or fp32), mlb_attention_tree attends with all rows at once, each seeing its ancestors.  The guesses come
 from the text so far (what followed earlier occurrences of the last tokens), so no second model is needed; the
 longest path that the model itself would have chosen is kept, which leaves the greedy text unchanged.  Prints one
-JSON line.
+JSON line.  It shows the calls in use and is not the fast way to decode: a pass is hundreds of small launches from
+Python (630 tokens/s with drafts on the Qwen2-0.5B shape, where the decode session makes 2411).
 """
 from __future__ import annotations
 
