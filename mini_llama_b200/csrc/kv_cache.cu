@@ -403,7 +403,7 @@ RotRows CheckedRot(const char* c, const char* name, const float* in, size_t in_s
     Require(in_stride >= n && out_stride >= n, c, std::string(name) + " stride is shorter than a row");
     Require(in != out || in_stride == out_stride, c, std::string(name) + " in place needs equal strides");
     RequireAligned(c, name, in, 4);
-    RequireAligned(c, (std::string(name) + " output").c_str(), out, 4);
+    RequireAligned(c, name, out, 4, " output");
     return {in, out, in_stride, out_stride, heads, in != out && rot < hd};
 }
 

@@ -24,10 +24,11 @@ struct KvView {
 
 // Checks the descriptor's shape, and with `pointers` its planes too.
 KvView CheckedKvView(const char* caller, const mlb_kv_cache* cache, bool pointers);
-// A pointer that is not on its elements' boundary (null is) would fault on the device.
-inline void RequireAligned(const char* caller, const char* name, const void* p, unsigned bytes) {
-    Require(reinterpret_cast<uintptr_t>(p) % bytes == 0, caller,
-            std::string(name) + " is not " + std::to_string(bytes) + "-byte aligned");
+// A pointer that is not on its elements' boundary (null is) would fault on the device.  The text is put together
+// only for a refusal: small calls take no longer than their host side.
+inline void RequireAligned(const char* caller, const char* name, const void* p, unsigned bytes, const char* part = "") {
+    if (reinterpret_cast<uintptr_t>(p) % bytes != 0)
+        Require(false, caller, std::string(name) + part + " is not " + std::to_string(bytes) + "-byte aligned");
 }
 // Checks a layer index (all_ok: MLB_ALL_LAYERS is allowed).
 void CheckKvLayer(const char* caller, const KvView& c, int layer, bool all_ok);
